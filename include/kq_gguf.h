@@ -313,6 +313,83 @@ int kq_moe_align(const int32_t* topk_ids, int64_t total, int64_t experts, int32_
 int kq_moe_combine(const void* y, int dtype, const void* weights, int w_dtype, int64_t tokens, int64_t n, int top_k, void* out,
                    void* stream);
 
+/* ---------------------------------------------------------------- between the projections of a decode step
+ * The operators that stand between the q/k/v projection and the output projection, and between a router and the experts'
+ * products.  The reference leaves them to vLLM (its linear method is called from vLLM's model code); they have no counterpart
+ * in its tree.  All of them read lengths, tables and indices on the device, so a captured call follows their values at each
+ * replay.
+ *
+ * Paged cache: k_cache and v_cache hold num_pages pages of page_size tokens of kv_heads heads of head_dim values of `dtype`;
+ * k_strides / v_strides (host arrays) = elements from page to page, token to token and head to head, head_dim is dense.  Slot s
+ * is token s % page_size of page s / page_size. */
+
+/* Norms of queries and keys per head and the position rotation in one launch, optionally with the write into a paged cache.
+ *   qkv        [tokens, (heads + 2 * kv_heads) * head_dim], row stride stride_t elements: the merged projection's output
+ *   positions  int32 (positions64 = 0) or int64, one per token
+ *   inv_freq   float[rotated / 2]; value pair i turns by position * inv_freq[i] (product and reduction in 64 bits), its cosine and
+ *              sine times `factor`.  interleaved = 0: pair (i, i + rotated / 2), 1: pair (2i, 2i + 1).  Values from `rotated` on
+ *              (rotated <= head_dim, even) are not turned
+ *   q_weight, k_weight  head_dim norm weights of w_dtype (KQ_F32 or dtype), each may be NULL: no norm.  y = x * rsqrt(mean(x^2) +
+ *              eps) * w, then the rotation, all in fp32 with one rounding to dtype
+ *   q_out      [tokens, heads, head_dim] dense
+ *   v_cache = NULL: k_out = [tokens, kv_heads, head_dim] dense, the values are left alone; otherwise k_out is the key cache, and
+ *              keys and values of token t go to slots[t] (int32 / int64 as slots64); a slot outside [0, num_pages * page_size) is
+ *              skipped, and two tokens with the same slot leave it with values of either
+ * head_dim: even, at most 512.  Outputs must not overlap the inputs. */
+int kq_qk_norm_rope(const void* qkv, int dtype, int64_t tokens, int64_t stride_t, int64_t heads, int64_t kv_heads,
+                    int64_t head_dim, const void* positions, int positions64, const float* inv_freq, int64_t rotated,
+                    int interleaved, float factor, const void* q_weight, const void* k_weight, int w_dtype, float eps,
+                    void* q_out, void* k_out, const int64_t* k_strides, void* v_cache, const int64_t* v_strides,
+                    const void* slots, int slots64, int64_t num_pages, int64_t page_size, void* stream);
+
+/* Attention of one new token per sequence over its cached keys: out[b, h] = sum_j softmax_j(f(scale * q[b, h] . k_j)) v_j over
+ * j in [max(0, seq_lens[b] - window), seq_lens[b]) (window = 0: from 0 on), f(x) = x, or softcap * tanh(x / softcap) for
+ * softcap > 0.  Query head h reads key head h / (heads / kv_heads).  Token j of sequence b stands in page
+ * block_table[b * table_stride + j / page_size] at place j % page_size.
+ *   - only pages of visible tokens are read, and of the last one only the tokens below seq_lens[b]
+ *   - a table entry outside [0, num_pages) and tokens beyond table_width * page_size count as absent
+ *   - a sequence that shows no token: zeros, lse = -infinity
+ * q: [batch, heads, head_dim] with strides q_stride_batch, q_stride_head, head_dim dense; out: dense; lse: [batch, heads] fp32 log
+ * of the sum of exponentials, or NULL.  q, caches and out have one dtype; scores, softmax and sums are fp32.  head_dim: a
+ * multiple of 16 up to 256 (KQ_EUNSUPPORTED otherwise); caches and their strides 16-byte aligned.
+ * scratch: kq_paged_attention_workspace_bytes(head_dim) bytes on the current device, 256-byte aligned, not initialised; calls
+ * that may overlap need one each. */
+size_t kq_paged_attention_workspace_bytes(int64_t head_dim);
+int kq_paged_attention(const void* q, int dtype, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                       int64_t q_stride_batch, int64_t q_stride_head, const void* k_cache, const int64_t* k_strides,
+                       const void* v_cache, const int64_t* v_strides, int64_t num_pages, int64_t page_size,
+                       const int32_t* block_table, int64_t table_stride, int64_t table_width, const int32_t* seq_lens,
+                       float scale, int64_t window, float softcap, void* out, float* lse, void* scratch,
+                       size_t scratch_bytes, void* stream);
+
+/* Page tables, slots and positions of a step.  Request r has seq_lens[r] tokens in the cache and new_lens[r] tokens to come
+ * (negative values count as 0).  It holds ceil(seq_lens[r] / page_size) pages, named by its row of block_table, and takes what it
+ * needs more from free_pages, in order: request 0's first page is free_pages[taken[0]].  Written:
+ *   block_table  the fresh entries, in place; -1 where the list has run out.  A row never takes more than table_width pages
+ *   total_lens   [requests]      seq_lens + new_lens
+ *   starts       [requests + 1]  where each request's new tokens start among all new tokens
+ *   positions, slots [num_tokens] of the new tokens, request by request; slot -1 (and position 0 behind the last token) for
+ *                padding, tokens beyond the row and tokens without a page
+ *   taken_out    [1]             taken + pages asked for: above num_free means that some were not there
+ * num_tokens must not be below the sum of new_lens: tokens that do not fit get neither a slot nor a table entry. */
+int kq_plan_pages(int32_t* block_table, int64_t table_stride, int64_t table_width, const int32_t* seq_lens,
+                  const int32_t* new_lens, int64_t requests, const int32_t* free_pages, int64_t num_free,
+                  const int32_t* taken, int64_t page_size, int64_t num_tokens, int32_t* total_lens, int32_t* starts,
+                  int32_t* positions, int64_t* slots, int32_t* taken_out, void* stream);
+
+/* Routing of tokens to experts: the topk_weights and topk_ids of the mixture-of-experts entry points.
+ *   logits [tokens, experts], row stride stride_t; p = softmax (sigmoid = 0) or sigmoid of them; c = p + bias (bias: float[experts],
+ *   or NULL: the order of the logits)
+ *   groups > 1: `groups` runs of experts / groups experts; a group counts its best c, with a bias the sum of its two best; only
+ *   the experts of the top_groups best groups stay
+ *   ids [tokens, top_k] int32: the best c, descending, ties (of groups too) to the lowest index; weights [tokens, top_k] fp32:
+ *   p of the chosen, divided by their sum if renormalize != 0 (zeros where that is 0), times scale
+ * NaN counts as -infinity and +infinity as the largest finite number; experts at -infinity come last, with weight 0 for softmax
+ * and sigmoid alike.  At most 1024 experts, top_k 32, 32 groups. */
+int kq_moe_route(const void* logits, int dtype, int64_t tokens, int64_t experts, int64_t stride_t, int64_t top_k,
+                 int sigmoid, const float* bias, int64_t groups, int64_t top_groups, int renormalize, float scale,
+                 float* weights, int32_t* ids, void* stream);
+
 /* Diagnostics: copies the device-side status word of a scratch buffer to the host (SYNCHRONISES with the
  * device; not for the serving path).  0 = every kernel that used the scratch finished normally; non-zero = a
  * bounded wait inside a kernel gave up and the kernel returned early (its outputs are then undefined).

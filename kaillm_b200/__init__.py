@@ -5,6 +5,7 @@ Layout:
   ops.py      the public op wrappers with the reference's names and argument meaning
               (vllm_gguf_plugin/ops.py:181-208)
   linear.py   regime dispatch and the linear method's apply (quantization/linear.py:40-63, 341-407)
+  attention.py  query/key norms and rotation, attention over a paged cache, page tables and slots
   sharded.py  row-sharded multi-GPU execution with an all-gather of the output slices
   synth.py    seeded synthetic wire tensors
 
@@ -12,4 +13,4 @@ There is no CPU or eager fallback: importing `capi` fails if libkq.so has not be
 (`python -m kaillm_b200._build`), and the ops raise if the `_C_gguf` extension is missing.
 """
 
-__all__ = ["capi", "ops", "linear", "sharded", "synth"]
+__all__ = ["capi", "ops", "linear", "attention", "sharded", "synth"]

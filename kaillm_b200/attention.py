@@ -1,0 +1,70 @@
+"""What a decode step runs between the q/k/v projection and the output projection, over a paged key-value cache.
+
+The reference leaves this part to vLLM, whose model code calls its linear method; here it is what `sharded.DecoderStack` calls
+between its projections:
+
+    total, starts, positions, slots, taken = plan_pages(block_table, seq_lens, new_lens, free_pages, taken, page_size, tokens)
+    q = qk_norm_rope_store(qkv, positions, inv_freq, heads, k_cache, v_cache, slots, q_weight=..., k_weight=...)   # every layer
+    out = paged_attention(q, k_cache, v_cache, block_table, total)                                                 # every layer
+
+A cache is a pair of tensors [pages, page size, kv heads, head dim] (any order of the first three in memory, so also
+`torch.empty(pages, kv_heads, page_size, head_dim).transpose(1, 2)`), dense and 16-byte aligned along the last dimension.  Lengths,
+tables, slots and positions stay on the GPU: no call synchronises, and a captured call reads their values at each replay.
+None of the operators has a derivative; they refuse inputs that require one.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import ops
+
+
+def qk_norm_rope(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, num_heads: int, num_kv_heads: int, *,
+                 q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 1e-6,
+                 interleaved: bool = False, factor: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rotated queries [tokens, num_heads, D] and keys [tokens, num_kv_heads, D] of a merged projection's output `qkv`
+    [tokens, (num_heads + 2 * num_kv_heads) * D].
+
+    positions: int32 or int64 [tokens].  inv_freq: float32 [R / 2], R <= D: pair i of a head turns by position * inv_freq[i] (formed
+    and reduced in 64 bits); pairs are (i, i + R / 2), or (2i, 2i + 1) if `interleaved`; values from R on are not turned.
+    `factor` multiplies the rotated values (the attention factor of scaled rotations).  With q_weight / k_weight [D] (float32 or
+    qkv's type) the head is first divided by sqrt(mean of squares + eps) and multiplied by the weight.  fp32 throughout, one
+    rounding at the end.  D: even, up to 512."""
+    return ops.qk_norm_rope(qkv, positions, inv_freq, num_heads, num_kv_heads, q_weight, k_weight, eps, interleaved, factor)
+
+
+def qk_norm_rope_store(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, num_heads: int, k_cache: torch.Tensor,
+                       v_cache: torch.Tensor, slots: torch.Tensor, *, q_weight: torch.Tensor | None = None,
+                       k_weight: torch.Tensor | None = None, eps: float = 1e-6, interleaved: bool = False,
+                       factor: float = 1.0) -> torch.Tensor:
+    """`qk_norm_rope` that returns the queries and writes the rotated keys and the values of token t into slot slots[t] of the caches
+    (slot = page * page size + place; int32 or int64; a slot outside the cache, -1 for instance, is skipped).  Slots should be
+    distinct: one that is named twice holds values of either token."""
+    return ops.qk_norm_rope_store(qkv, positions, inv_freq, num_heads, k_cache, v_cache, slots, q_weight, k_weight, eps, interleaved, factor)
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, *,
+                    scale: float | None = None, window: int = 0, softcap: float = 0.0, return_lse: bool = False):
+    """Attention of one token per sequence, q [batch, heads, D], over the first seq_lens[b] cached tokens (the last `window` of them
+    if window > 0): [batch, heads, D], and with return_lse the fp32 log of the sum of exponentials [batch, heads].
+
+    scale: 1 / sqrt(D) by default.  softcap > 0: scores become softcap * tanh(score / softcap).  block_table int32 [batch, pages]:
+    token j of sequence b is place j % page size of page block_table[b, j // page size]; entries outside the cache count as absent.
+    A sequence without visible tokens gives zeros (lse -inf).  The token's own key has to be in the cache
+    (`qk_norm_rope_store` first) and counted in seq_lens.  D: a multiple of 16 up to 256; float32, float16 or bfloat16."""
+    out, lse = ops.paged_attention(q, k_cache, v_cache, block_table, seq_lens, q.shape[-1] ** -0.5 if scale is None else scale, window,
+                                   softcap, return_lse)
+    return (out, lse) if return_lse else out
+
+
+def plan_pages(block_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: torch.Tensor, taken: torch.Tensor,
+               page_size: int, num_tokens: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Room in the cache for new_lens[r] more tokens of each request: (total_lens [R], starts [R + 1], positions [num_tokens], slots
+    [num_tokens] int64, taken [1]); everything else int32.
+
+    Request r holds ceil(seq_lens[r] / page_size) pages, named in its row of block_table [R, pages]; what it needs more is taken from
+    free_pages in the order of the requests, from index taken[0] on, and entered into block_table in place.  `taken` comes back
+    raised by the pages asked for; above len(free_pages) the list has run out and the tokens concerned have slot -1, as have
+    tokens beyond the table's width and the padding behind the last of the num_tokens entries.  num_tokens must be at least
+    the sum of new_lens."""
+    return ops.plan_pages(block_table, seq_lens, new_lens, free_pages, taken, page_size, num_tokens)

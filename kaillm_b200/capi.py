@@ -25,6 +25,7 @@ EXPORTS = (
     "kq_p2p_allgather", "kq_read_status_static", "kq_debug_copy_window", "kq_prepare_q8_rmsnorm", "kq_prepare_q8_swiglu",
     "kq_p2p_allgather_2d", "kq_mul_mat_prepared_gather", "kq_moe_a8_vec", "kq_moe_a8", "kq_moe_block_size", "kq_dequantize_rows", "kq_wait_arrival", "kq_arrival_status",
     "kq_dequant_mul_mat_supported", "kq_dequant_mul_mat_preferred", "kq_dequant_mul_mat", "kq_dequant_mul_mat_status", "kq_moe_project", "kq_moe_align", "kq_moe_combine",
+    "kq_qk_norm_rope", "kq_paged_attention_workspace_bytes", "kq_paged_attention", "kq_plan_pages", "kq_moe_route",
 )
 
 
@@ -75,6 +76,15 @@ def _load() -> ctypes.CDLL:
     lib.kq_dequant_mul_mat.argtypes = [vp, i32, i64, i64, vp, i32, i64, i64, vp, i64, vp]
     lib.kq_dequant_mul_mat_preferred.argtypes = [i64, i64]
     lib.kq_dequant_mul_mat_status.argtypes = [ctypes.POINTER(i32), i32]
+    f32, i64p = ctypes.c_float, ctypes.POINTER(i64)
+    lib.kq_qk_norm_rope.argtypes = [vp, i32, i64, i64, i64, i64, i64, vp, i32, vp, i64, i32, f32, vp, vp, i32, f32, vp, vp, i64p, vp, i64p,
+                                    vp, i32, i64, i64, vp]
+    lib.kq_paged_attention_workspace_bytes.restype = sz
+    lib.kq_paged_attention_workspace_bytes.argtypes = [i64]
+    lib.kq_paged_attention.argtypes = [vp, i32, i64, i64, i64, i64, i64, i64, vp, i64p, vp, i64p, i64, i64, vp, i64, i64, vp, f32, i64, f32,
+                                       vp, vp, vp, sz, vp]
+    lib.kq_plan_pages.argtypes = [vp, i64, i64, vp, vp, i64, vp, i64, vp, i64, i64, vp, vp, vp, vp, vp, vp]
+    lib.kq_moe_route.argtypes = [vp, i32, i64, i64, i64, i64, i32, vp, i64, i64, i32, f32, vp, vp, vp]
     lib.kq_set_option.argtypes = [ctypes.c_char_p, i32]
     lib.kq_get_option.argtypes = [ctypes.c_char_p, ctypes.POINTER(i32)]
     return lib
@@ -322,6 +332,46 @@ def dequantize_rows(W: torch.Tensor, qtype: int, k: int, row_ids: torch.Tensor, 
         _check(lib.kq_dequantize_rows(W.data_ptr(), qtype, W.shape[0], k, ids.data_ptr(), ids.numel(), out.data_ptr(),
                                       _DT[dtype], int(f32_math), _stream(W.device)))
     return out.view(*row_ids.shape, k)
+
+
+def _strides3(cache: torch.Tensor):
+    return (ctypes.c_int64 * 3)(*cache.stride()[:3])
+
+
+def qk_norm_rope(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, heads: int, kv_heads: int,
+                 q_out: torch.Tensor, k_out: torch.Tensor, *, q_weight: torch.Tensor | None = None,
+                 k_weight: torch.Tensor | None = None, eps: float = 1e-6, interleaved: bool = False, factor: float = 1.0,
+                 v_cache: torch.Tensor | None = None, slots: torch.Tensor | None = None) -> None:
+    """kq_qk_norm_rope: rotated queries into q_out [tokens, heads, head_dim]; keys into k_out [tokens, kv_heads, head_dim], or with
+    v_cache and slots keys and values into the paged caches k_out and v_cache [pages, page size, kv_heads, head_dim]."""
+    tokens, d = q_out.shape[0], q_out.shape[2]
+    store = v_cache is not None
+    w = q_weight if q_weight is not None else k_weight
+    with torch.cuda.device(qkv.device):
+        _check(lib.kq_qk_norm_rope(
+            qkv.data_ptr(), _DT[qkv.dtype], tokens, qkv.stride(0), heads, kv_heads, d, positions.data_ptr(), int(positions.dtype == torch.int64),
+            inv_freq.data_ptr(), 2 * inv_freq.numel(), int(interleaved), factor, q_weight.data_ptr() if q_weight is not None else None,
+            k_weight.data_ptr() if k_weight is not None else None, _DT[w.dtype] if w is not None else KQ_F32, eps, q_out.data_ptr(),
+            k_out.data_ptr(), _strides3(k_out) if store else None, v_cache.data_ptr() if store else None, _strides3(v_cache) if store else None,
+            slots.data_ptr() if store else None, int(store and slots.dtype == torch.int64), k_out.shape[0] if store else 0,
+            k_out.shape[1] if store else 0, _stream(qkv.device)))
+
+
+def paged_attention_workspace_bytes(head_dim: int) -> int:
+    return int(lib.kq_paged_attention_workspace_bytes(head_dim))
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                    seq_lens: torch.Tensor, out: torch.Tensor, scratch: torch.Tensor, *, scale: float, window: int = 0,
+                    softcap: float = 0.0, lse: torch.Tensor | None = None) -> None:
+    """kq_paged_attention: q [batch, heads, head_dim] over caches [pages, page size, kv_heads, head_dim] into out (dense)."""
+    b, h, d = q.shape
+    with torch.cuda.device(q.device):
+        _check(lib.kq_paged_attention(
+            q.data_ptr(), _DT[q.dtype], b, h, k_cache.shape[2], d, q.stride(0), q.stride(1), k_cache.data_ptr(), _strides3(k_cache),
+            v_cache.data_ptr(), _strides3(v_cache), k_cache.shape[0], k_cache.shape[1], block_table.data_ptr(), block_table.stride(0),
+            block_table.shape[1], seq_lens.data_ptr(), scale, window, softcap, out.data_ptr(), lse.data_ptr() if lse is not None else None,
+            scratch.data_ptr(), scratch.numel(), _stream(q.device)))
 
 
 def debug_group_dots(W: torch.Tensor, x: torch.Tensor, qtype: int):

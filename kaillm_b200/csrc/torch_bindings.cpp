@@ -8,12 +8,15 @@
 //   - an unsupported GGML type raises instead of silently returning zeros
 //     (reference: switch without default, csrc/gguf/gguf_kernel.cu:119-215);
 //   - ops of this library's own beside the reference's six: ggml_dequant_mul_mat, ggml_dequantize_rows,
-//     ggml_mul_mat_merged, fused_moe_swiglu (no derivative: kaillm_b200/linear.py calls them for plain tensors only).
+//     ggml_mul_mat_merged, fused_moe_swiglu (no derivative: kaillm_b200/linear.py calls them for plain tensors only);
+//   - the operators between the projections of a decode step (qk_norm_rope, qk_norm_rope_store, paged_attention, plan_pages,
+//     moe_route), which refuse inputs that require a gradient.
 #include <Python.h>
 
 #include <algorithm>
 
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/CUDAEvent.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -289,6 +292,172 @@ at::Tensor fused_moe_swiglu(const at::Tensor& X, const at::Tensor& W1, const at:
   return out;
 }
 
+void no_gradient(const char* fn, std::initializer_list<const at::Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const at::Tensor* t : ts) TORCH_CHECK(!t->defined() || !t->requires_grad(), fn, ": has no derivative, and an input requires one");
+}
+
+// defined, on `like`'s device and of one of the given types
+void check_on(const char* fn, const char* name, const at::Tensor& t, const at::Tensor& like, std::initializer_list<at::ScalarType> types) {
+  TORCH_CHECK(t.is_cuda() && t.get_device() == like.get_device(), fn, ": ", name, " must be on the device of the first argument");
+  bool ok = false;
+  for (at::ScalarType s : types) ok |= t.scalar_type() == s;
+  TORCH_CHECK(ok, fn, ": ", name, " has the wrong dtype ", t.scalar_type());
+}
+
+struct RopeCall { int64_t tokens, kv, d; int wdt; const void *qw, *kw; };
+
+RopeCall rope_checks(const char* fn, const at::Tensor& qkv, const at::Tensor& positions, const at::Tensor& inv_freq, int64_t heads, int64_t kv,
+                     const std::optional<at::Tensor>& q_weight, const std::optional<at::Tensor>& k_weight) {
+  TORCH_CHECK(qkv.is_cuda() && qkv.dim() == 2 && (qkv.size(1) == 1 || qkv.stride(1) == 1), fn, ": qkv must be a 2-D CUDA tensor, contiguous along its last dimension");
+  TORCH_CHECK(heads > 0 && kv > 0 && heads <= 65536 && kv <= 65536 && qkv.size(1) > 0 && qkv.size(1) % (heads + 2 * kv) == 0, fn,
+              ": qkv.size(1)=", qkv.size(1), " is not a whole number of values for ", heads, " query and ", kv, " key and value heads");
+  RopeCall c{qkv.size(0), kv, qkv.size(1) / (heads + 2 * kv), KQ_F32, nullptr, nullptr};
+  check_on(fn, "positions", positions, qkv, {at::kInt, at::kLong});
+  TORCH_CHECK(positions.dim() == 1 && positions.size(0) == c.tokens && positions.is_contiguous(), fn, ": positions must be contiguous, one per token");
+  check_on(fn, "inv_freq", inv_freq, qkv, {at::kFloat});
+  TORCH_CHECK(inv_freq.dim() == 1 && inv_freq.is_contiguous() && 2 * inv_freq.size(0) <= c.d, fn, ": inv_freq must be contiguous, one value per rotated pair, at most ", c.d / 2);
+  const at::Tensor none;
+  const at::Tensor &qw = q_weight.has_value() ? *q_weight : none, &kw = k_weight.has_value() ? *k_weight : none;
+  for (const at::Tensor* w : {&qw, &kw})
+    if (w->defined()) {
+      check_on(fn, "norm weight", *w, qkv, {at::kFloat, qkv.scalar_type()});
+      TORCH_CHECK(w->dim() == 1 && w->size(0) == c.d && w->is_contiguous(), fn, ": norm weights must be contiguous, ", c.d, " values");
+      c.wdt = kq_dtype_of(w->scalar_type(), fn);
+    }
+  TORCH_CHECK(!qw.defined() || !kw.defined() || qw.scalar_type() == kw.scalar_type(), fn, ": the norm weights must have one dtype");
+  c.qw = qw.defined() ? qw.data_ptr() : nullptr;
+  c.kw = kw.defined() ? kw.data_ptr() : nullptr;
+  no_gradient(fn, {&qkv, &inv_freq, &qw, &kw});
+  return c;
+}
+
+// caches [pages, page size, kv heads, head dim]; any order of the first three dimensions
+void cache_checks(const char* fn, const at::Tensor& k, const at::Tensor& v, const at::Tensor& like) {
+  for (const at::Tensor* t : {&k, &v}) {
+    check_on(fn, "cache", *t, like, {like.scalar_type()});
+    TORCH_CHECK(t->dim() == 4 && (t->size(3) == 1 || t->stride(3) == 1), fn, ": caches are [pages, page size, kv heads, head dim], dense along the last");
+  }
+  TORCH_CHECK(k.sizes() == v.sizes(), fn, ": the caches of keys and values differ in size");
+  no_gradient(fn, {&k, &v});
+}
+
+std::tuple<at::Tensor, at::Tensor> qk_norm_rope(const at::Tensor& qkv, const at::Tensor& positions, const at::Tensor& inv_freq, int64_t heads,
+                                                int64_t kv, const std::optional<at::Tensor>& q_weight, const std::optional<at::Tensor>& k_weight,
+                                                double eps, bool interleaved, double factor) {
+  const char* fn = "qk_norm_rope";
+  const RopeCall c = rope_checks(fn, qkv, positions, inv_freq, heads, kv, q_weight, k_weight);
+  const int dt = kq_dtype_of(qkv.scalar_type(), fn);
+  const c10::cuda::CUDAGuard guard(qkv.device());
+  at::Tensor q = at::empty({c.tokens, heads, c.d}, qkv.options()), k = at::empty({c.tokens, kv, c.d}, qkv.options());
+  TORCH_CHECK(kq_qk_norm_rope(qkv.data_ptr(), dt, c.tokens, qkv.stride(0), heads, kv, c.d, positions.data_ptr(), positions.scalar_type() == at::kLong,
+                              inv_freq.data_ptr<float>(), 2 * inv_freq.size(0), interleaved, (float)factor, c.qw, c.kw, c.wdt, (float)eps,
+                              q.data_ptr(), k.data_ptr(), nullptr, nullptr, nullptr, nullptr, 0, 0, 0,
+                              (void*)at::cuda::getCurrentCUDAStream(qkv.get_device()).stream()) == KQ_OK, fn, ": ", kq_last_error());
+  return {q, k};
+}
+
+at::Tensor qk_norm_rope_store(const at::Tensor& qkv, const at::Tensor& positions, const at::Tensor& inv_freq, int64_t heads,
+                              const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& slots,
+                              const std::optional<at::Tensor>& q_weight, const std::optional<at::Tensor>& k_weight, double eps,
+                              bool interleaved, double factor) {
+  const char* fn = "qk_norm_rope_store";
+  at::assert_no_internal_overlap(k_cache);
+  at::assert_no_internal_overlap(v_cache);
+  cache_checks(fn, k_cache, v_cache, qkv);
+  TORCH_CHECK(k_cache.size(0) > 0 && k_cache.size(1) > 0, fn, ": the caches have no pages");
+  const RopeCall c = rope_checks(fn, qkv, positions, inv_freq, heads, k_cache.size(2), q_weight, k_weight);
+  TORCH_CHECK(k_cache.size(3) == c.d, fn, ": the caches hold heads of ", k_cache.size(3), " values, qkv of ", c.d);
+  check_on(fn, "slots", slots, qkv, {at::kInt, at::kLong});
+  TORCH_CHECK(slots.dim() == 1 && slots.size(0) == c.tokens && slots.is_contiguous(), fn, ": slots must be contiguous, one per token");
+  const int dt = kq_dtype_of(qkv.scalar_type(), fn);
+  const c10::cuda::CUDAGuard guard(qkv.device());
+  at::Tensor q = at::empty({c.tokens, heads, c.d}, qkv.options());
+  TORCH_CHECK(kq_qk_norm_rope(qkv.data_ptr(), dt, c.tokens, qkv.stride(0), heads, c.kv, c.d, positions.data_ptr(), positions.scalar_type() == at::kLong,
+                              inv_freq.data_ptr<float>(), 2 * inv_freq.size(0), interleaved, (float)factor, c.qw, c.kw, c.wdt, (float)eps,
+                              q.data_ptr(), k_cache.data_ptr(), k_cache.strides().data(), v_cache.data_ptr(), v_cache.strides().data(),
+                              slots.data_ptr(), slots.scalar_type() == at::kLong, k_cache.size(0), k_cache.size(1),
+                              (void*)at::cuda::getCurrentCUDAStream(qkv.get_device()).stream()) == KQ_OK, fn, ": ", kq_last_error());
+  return q;
+}
+
+std::tuple<at::Tensor, at::Tensor> paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                                                   const at::Tensor& block_table, const at::Tensor& seq_lens, double scale, int64_t window,
+                                                   double softcap, bool lse) {
+  const char* fn = "paged_attention";
+  TORCH_CHECK(q.is_cuda() && q.dim() == 3 && (q.size(2) == 1 || q.stride(2) == 1), fn, ": q must be [batch, heads, head dim] on a GPU, dense along the last");
+  cache_checks(fn, k_cache, v_cache, q);
+  TORCH_CHECK(k_cache.size(3) == q.size(2), fn, ": the caches hold heads of ", k_cache.size(3), " values, q of ", q.size(2));
+  check_on(fn, "block_table", block_table, q, {at::kInt});
+  check_on(fn, "seq_lens", seq_lens, q, {at::kInt});
+  const int64_t b = q.size(0), h = q.size(1), d = q.size(2);
+  TORCH_CHECK(block_table.dim() == 2 && block_table.size(0) == b && (block_table.size(1) <= 1 || block_table.stride(1) == 1), fn, ": block_table must be [batch, pages], dense along the last");
+  TORCH_CHECK(seq_lens.dim() == 1 && seq_lens.size(0) == b && seq_lens.is_contiguous(), fn, ": seq_lens must be contiguous, one per sequence");
+  no_gradient(fn, {&q});
+  const int dt = kq_dtype_of(q.scalar_type(), fn);
+  const c10::cuda::CUDAGuard guard(q.device());
+  at::Tensor out = at::empty({b, h, d}, q.options()), norm = at::empty({lse ? b : 0, h}, q.options().dtype(at::kFloat));
+  const size_t ws = kq_paged_attention_workspace_bytes(d);
+  at::Tensor scratch = at::empty({(int64_t)ws}, q.options().dtype(at::kByte));
+  TORCH_CHECK(kq_paged_attention(q.data_ptr(), dt, b, h, k_cache.size(2), d, q.stride(0), q.stride(1), k_cache.data_ptr(), k_cache.strides().data(),
+                                 v_cache.data_ptr(), v_cache.strides().data(), k_cache.size(0), k_cache.size(1), block_table.data_ptr<int32_t>(),
+                                 block_table.stride(0), block_table.size(1), seq_lens.data_ptr<int32_t>(), (float)scale, window, (float)softcap,
+                                 out.data_ptr(), lse ? norm.data_ptr<float>() : nullptr, scratch.data_ptr(), ws,
+                                 (void*)at::cuda::getCurrentCUDAStream(q.get_device()).stream()) == KQ_OK, fn, ": ", kq_last_error());
+  return {out, norm};
+}
+
+// (total_lens, starts, positions, slots, taken); fresh pages are entered into block_table in place
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> plan_pages(const at::Tensor& block_table, const at::Tensor& seq_lens,
+                                                                                  const at::Tensor& new_lens, const at::Tensor& free_pages,
+                                                                                  const at::Tensor& taken, int64_t page_size, int64_t num_tokens) {
+  const char* fn = "plan_pages";
+  TORCH_CHECK(block_table.is_cuda() && block_table.dim() == 2 && block_table.scalar_type() == at::kInt && (block_table.size(1) <= 1 || block_table.stride(1) == 1), fn,
+              ": block_table must be an int32 CUDA tensor [requests, pages], dense along the last");
+  at::assert_no_internal_overlap(block_table);
+  const int64_t r = block_table.size(0);
+  for (const at::Tensor* t : {&seq_lens, &new_lens, &free_pages, &taken}) {
+    check_on(fn, "index tensor", *t, block_table, {at::kInt});
+    TORCH_CHECK(t->dim() == 1 && t->is_contiguous(), fn, ": seq_lens, new_lens, free_pages and taken must be contiguous and 1-D");
+  }
+  TORCH_CHECK(seq_lens.size(0) == r && new_lens.size(0) == r && taken.size(0) == 1, fn, ": one length per row of block_table, and one value in taken");
+  TORCH_CHECK(num_tokens >= 0 && page_size > 0, fn, ": page_size must be positive and num_tokens not negative");
+  const c10::cuda::CUDAGuard guard(block_table.device());
+  const auto opt = block_table.options();
+  // one allocation for the four int32 results, the 8-byte slots in front
+  at::Tensor slots = at::empty({num_tokens}, opt.dtype(at::kLong));
+  at::Tensor rest = at::empty({r + (r + 1) + num_tokens + 1}, opt);
+  at::Tensor total = rest.narrow(0, 0, r), starts = rest.narrow(0, r, r + 1), positions = rest.narrow(0, 2 * r + 1, num_tokens),
+             after = rest.narrow(0, 2 * r + 1 + num_tokens, 1);
+  TORCH_CHECK(kq_plan_pages(block_table.data_ptr<int32_t>(), block_table.stride(0), block_table.size(1), seq_lens.data_ptr<int32_t>(), new_lens.data_ptr<int32_t>(), r,
+                            free_pages.data_ptr<int32_t>(), free_pages.size(0), taken.data_ptr<int32_t>(), page_size, num_tokens,
+                            total.data_ptr<int32_t>(), starts.data_ptr<int32_t>(), positions.data_ptr<int32_t>(), slots.data_ptr<int64_t>(),
+                            after.data_ptr<int32_t>(), (void*)at::cuda::getCurrentCUDAStream(block_table.get_device()).stream()) == KQ_OK, fn, ": ", kq_last_error());
+  return {total, starts, positions, slots, after};
+}
+
+std::tuple<at::Tensor, at::Tensor> moe_route(const at::Tensor& logits, int64_t top_k, bool sigmoid, const std::optional<at::Tensor>& bias_, int64_t groups,
+                                             int64_t top_groups, bool renormalize, double scale) {
+  const char* fn = "moe_route";
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && (logits.size(1) <= 1 || logits.stride(1) == 1), fn, ": logits must be a 2-D CUDA tensor, contiguous along its last dimension");
+  const int dt = kq_dtype_of(logits.scalar_type(), fn);
+  const at::Tensor none;
+  const at::Tensor& bias = bias_.has_value() ? *bias_ : none;
+  const int64_t t = logits.size(0), e = logits.size(1);
+  if (bias.defined()) {
+    check_on(fn, "bias", bias, logits, {at::kFloat});
+    TORCH_CHECK(bias.dim() == 1 && bias.size(0) == e && bias.is_contiguous(), fn, ": bias must be contiguous, one value per expert");
+  }
+  no_gradient(fn, {&logits, &bias});
+  TORCH_CHECK(top_k > 0 && top_k <= e, fn, ": top_k=", top_k, " is not between 1 and ", e);
+  const c10::cuda::CUDAGuard guard(logits.device());
+  at::Tensor w = at::empty({t, top_k}, logits.options().dtype(at::kFloat)), ids = at::empty({t, top_k}, logits.options().dtype(at::kInt));
+  TORCH_CHECK(kq_moe_route(logits.data_ptr(), dt, t, e, logits.stride(0), top_k, sigmoid, bias.defined() ? bias.data_ptr<float>() : nullptr, groups, top_groups,
+                           renormalize, (float)scale, w.data_ptr<float>(), ids.data_ptr<int32_t>(),
+                           (void*)at::cuda::getCurrentCUDAStream(logits.get_device()).stream()) == KQ_OK, fn, ": ", kq_last_error());
+  return {w, ids};
+}
+
 int64_t ggml_moe_get_block_size(int64_t type) { return kq_moe_block_size((int)type); }
 
 }  // namespace
@@ -308,6 +477,21 @@ TORCH_LIBRARY(_C_gguf, ops) {
       "fused_moe_swiglu(Tensor X, Tensor W1, Tensor W2, Tensor topk_weights, Tensor topk_ids, int type1, int type2, bool block) "
       "-> Tensor");
   ops.def("ggml_moe_get_block_size(int type) -> int");
+  ops.def(
+      "qk_norm_rope(Tensor qkv, Tensor positions, Tensor inv_freq, int num_heads, int num_kv_heads, Tensor? q_weight, Tensor? k_weight, "
+      "float eps, bool interleaved, float factor) -> (Tensor, Tensor)");
+  ops.def(
+      "qk_norm_rope_store(Tensor qkv, Tensor positions, Tensor inv_freq, int num_heads, Tensor(a!) k_cache, Tensor(b!) v_cache, "
+      "Tensor slots, Tensor? q_weight, Tensor? k_weight, float eps, bool interleaved, float factor) -> Tensor");
+  ops.def(
+      "paged_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor seq_lens, float scale, int window, "
+      "float softcap, bool lse) -> (Tensor, Tensor)");
+  ops.def(
+      "plan_pages(Tensor(a!) block_table, Tensor seq_lens, Tensor new_lens, Tensor free_pages, Tensor taken, int page_size, "
+      "int num_tokens) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+  ops.def(
+      "moe_route(Tensor logits, int top_k, bool sigmoid, Tensor? bias, int groups, int top_groups, bool renormalize, float scale) "
+      "-> (Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(_C_gguf, CUDA, ops) {
@@ -320,6 +504,11 @@ TORCH_LIBRARY_IMPL(_C_gguf, CUDA, ops) {
   ops.impl("ggml_moe_a8", &ggml_moe_a8);
   ops.impl("ggml_moe_a8_vec", &ggml_moe_a8_vec);
   ops.impl("fused_moe_swiglu", &fused_moe_swiglu);
+  ops.impl("qk_norm_rope", &qk_norm_rope);
+  ops.impl("qk_norm_rope_store", &qk_norm_rope_store);
+  ops.impl("paged_attention", &paged_attention);
+  ops.impl("plan_pages", &plan_pages);
+  ops.impl("moe_route", &moe_route);
 }
 
 TORCH_LIBRARY_IMPL(_C_gguf, CompositeExplicitAutograd, ops) {

@@ -134,6 +134,20 @@ def apply_gguf_embedding(x: torch.Tensor, qweight: torch.Tensor, qweight_type: i
     raise NotImplementedError(f"Unsupported GGUF quantization type: {qweight_type}")
 
 
+def route_experts(router_logits: torch.Tensor, top_k: int, *, scoring: str = "softmax", bias: torch.Tensor | None = None, groups: int = 1,
+                  top_groups: int = 1, renormalize: bool = True, scale: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """The `topk_weights` (float32) and `topk_ids` (int32), both [tokens, top_k], that `fused_moe_gguf` takes, from the router's logits
+    [tokens, experts], in one launch (vLLM's fused_topk / grouped_topk stand here in the reference).
+
+    scoring "softmax" or "sigmoid" over the experts; bias (float32 [experts]): added for the choice only.  groups > 1: only the experts
+    of the top_groups best of `groups` equal runs of experts can be chosen; a run counts its best expert, with a bias the sum of its
+    two best.  Ids come best first, ties to the lowest index.  renormalize: the weights of a token sum to 1; then times scale.
+    NaN counts as -inf; masked experts (-inf) come last with weight 0.  At most 1024 experts, top_k 32, 32 groups; no gradient."""
+    if scoring not in ("softmax", "sigmoid"):
+        raise ValueError(f"scoring must be 'softmax' or 'sigmoid', got {scoring!r}")
+    return ops.moe_route(router_logits, top_k, scoring == "sigmoid", bias, groups, top_groups, renormalize, scale)
+
+
 def moe_align_block_size(topk_ids: torch.Tensor, block_size: int, num_experts: int):
     """What vLLM's moe_align_block_size returns (fused_moe.py, called at quantization/fused_moe.py:62-64): the flattened
     (token, k) slots sorted by expert, every expert's run padded to a multiple of `block_size` with the value
