@@ -12,12 +12,15 @@
 // captured call follows the lengths of each replay.  An item inside one CTA is finished there; one that crosses CTAs leaves
 // partial results (unnormalised values, maximum, sum) that attend_join_kernel adds in the order of the keys: no atomics, the
 // same bits every time.
+#include <type_traits>
+
 #include "kq_common.cuh"
 
 namespace kq {
 
 namespace {
 
+constexpr int AT_MAX_CTAS = 2;         // per multiprocessor
 constexpr int AT_WARPS = 4;            // warps of a CTA: each walks every fourth tile of keys of the CTA's share on its own
 constexpr float AT_LOG2E = 1.4426950408889634f;
 constexpr float AT_LN2 = 0.6931471805599453f;
@@ -104,9 +107,9 @@ __device__ __forceinline__ int cta_of(const Share& s, int64_t unit) {   // the C
   return c;
 }
 
-__device__ __forceinline__ void cp_async(uint32_t dst, const void* src, int bytes, int live) {
-  if (bytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live) : "memory");
-  else asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(live) : "memory");
+// 16 bytes, or with live = false 16 bytes of zeros and no read
+__device__ __forceinline__ void cp_async(uint32_t dst, const void* src, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -180,26 +183,20 @@ __device__ __forceinline__ bool find_key(const AttnParams& p, int b, int j, int 
   return *page >= 0 && *page < p.num_pages;
 }
 
-template <typename T> struct Vec4;
-template <> struct Vec4<float> { static __device__ __forceinline__ float4 load(uint32_t a) { float4 f; asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w) : "r"(a) : "memory"); return f; } };
-template <typename T> struct Vec4 {
-  static __device__ __forceinline__ float4 load(uint32_t a) {
-    uint32_t u, w;
-    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(u), "=r"(w) : "r"(a) : "memory");
-    const T* x = reinterpret_cast<const T*>(&u);
-    const T* y = reinterpret_cast<const T*>(&w);
-    return make_float4(to_f32<T>(x[0]), to_f32<T>(x[1]), to_f32<T>(y[0]), to_f32<T>(y[1]));
-  }
-};
+__device__ __forceinline__ float4 lds4(uint32_t a) {
+  float4 f;
+  asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w) : "r"(a) : "memory");
+  return f;
+}
 
-// Products on the fp32 pipes: a lane owns four neighbouring dimensions in every 128 (NI groups), so a key row is one dense read
+// fp32: products on the fp32 pipes (three tf32 products would be needed for as many bits): a lane owns four neighbouring dimensions in every 128 (NI groups), so a key row is one dense read
 // of the warp and q and the values stay in registers; R rows x 32 / R keys of partial dot products are summed over the lanes by
 // halving the rows and keys that a lane still holds (31 shuffles for 32 sums), after which lane = (row, key) holds one score.
 // Keys and values come through a ring of cp.async copies; a lane copies exactly the bytes that it reads back.
-template <typename T, int R, int NI, int STAGES>
+template <int R, int NI, int STAGES>
 __global__ void __launch_bounds__(AT_WARPS * 32) attend_fma_kernel(const AttnParams p) {
   constexpr int KB = 32 / R;                      // keys of a tile
-  constexpr int CH = 4 * (int)sizeof(T);          // bytes of a lane's piece of a row
+  constexpr int CH = 16;                          // bytes of a lane's piece of a row
   constexpr int ROW = NI * 32 * CH;
   constexpr int SLOT = 2 * KB * ROW;              // keys, then values
   extern __shared__ __align__(16) uint8_t smem[];
@@ -248,7 +245,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32) attend_fma_kernel(const AttnPar
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int d = i * 128 + lane * 4 + e;
-          q[r][i * 4 + e] = r < rows && d < p.dim ? to_f32<T>(reinterpret_cast<const T*>(p.q)[(int64_t)b * p.q_b + (int64_t)(head0 + r) * p.q_h + d]) : 0.f;
+          q[r][i * 4 + e] = r < rows && d < p.dim ? static_cast<const float*>(p.q)[(int64_t)b * p.q_b + (int64_t)(head0 + r) * p.q_h + d] : 0.f;
           o[r][i * 4 + e] = 0.f;
         }
     float m = -INFINITY, l = 0.f;                  // of row lane / KB; l: of the lane's own keys
@@ -264,14 +261,14 @@ __global__ void __launch_bounds__(AT_WARPS * 32) attend_fma_kernel(const AttnPar
         for (int kk = 0; kk < KB; ++kk) {
           const int64_t pg = __shfl_sync(0xffffffffu, page, kk), pl = __shfl_sync(0xffffffffu, place, kk);
           const bool on = live >> kk & 1;
-          const T* kr = reinterpret_cast<const T*>(p.k) + (on ? pg * p.k_page + pl * p.k_slot + h * p.k_head : 0);
-          const T* vr = reinterpret_cast<const T*>(p.v) + (on ? pg * p.v_page + pl * p.v_slot + h * p.v_head : 0);
+          const float* kr = static_cast<const float*>(p.k) + (on ? pg * p.k_page + pl * p.k_slot + h * p.k_head : 0);
+          const float* vr = static_cast<const float*>(p.v) + (on ? pg * p.v_page + pl * p.v_slot + h * p.v_head : 0);
 #pragma unroll
           for (int i = 0; i < NI; ++i) {
             const int d = i * 128 + lane * 4;
             const bool in = on && d < p.dim;       // otherwise zeros are written and nothing is read
-            cp_async(ring + slot * SLOT + kk * ROW + i * 32 * CH, kr + (in ? d : 0), CH, in ? CH : 0);
-            cp_async(ring + slot * SLOT + (KB + kk) * ROW + i * 32 * CH, vr + (in ? d : 0), CH, in ? CH : 0);
+            cp_async(ring + slot * SLOT + kk * ROW + i * 32 * CH, kr + (in ? d : 0), in);
+            cp_async(ring + slot * SLOT + (KB + kk) * ROW + i * 32 * CH, vr + (in ? d : 0), in);
           }
         }
       }
@@ -297,7 +294,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32) attend_fma_kernel(const AttnPar
         for (int r = 0; r < R; ++r) v[r * KB + kk] = 0.f;
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-          const float4 kx = Vec4<T>::load(at + kk * ROW + i * 32 * CH);
+          const float4 kx = lds4(at + kk * ROW + i * 32 * CH);
 #pragma unroll
           for (int r = 0; r < R; ++r) {
             float a = v[r * KB + kk];
@@ -342,7 +339,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32) attend_fma_kernel(const AttnPar
       for (int kk = 0; kk < KB; ++kk) {
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-          const float4 vx = Vec4<T>::load(at + (KB + kk) * ROW + i * 32 * CH);
+          const float4 vx = lds4(at + (KB + kk) * ROW + i * 32 * CH);
 #pragma unroll
           for (int r = 0; r < R; ++r) {
             const float wr = __shfl_sync(0xffffffffu, w, r * KB + kk);
@@ -366,6 +363,244 @@ __global__ void __launch_bounds__(AT_WARPS * 32) attend_fma_kernel(const AttnPar
       }
     __syncthreads();
     const bool whole = t0 == 0 && t1 == tiles;
+    store_tile<float>(p, s_o, s_ml, b, head0, rows, R, whole ? -1 : 2 * (int)blockIdx.x + (t0 == 0));
+    if (!p.split) break;
+    if (!whole && t0 == 0 && tid == 0)
+      p.meta[blockIdx.x] = make_int4(b * per + sub, cta_of(s, base + (int64_t)(sub + 1) * tiles - 1), 0, 0);
+    __syncthreads();
+    unit += t1 - t0;
+    if (unit == base + (int64_t)tiles * per) { base = unit; ++b; }
+  }
+}
+
+// ---- 16-bit types: products on the tensor cores ----
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <typename T> __device__ __forceinline__ uint32_t bits_of(T lo, T hi) {
+  return (uint32_t)*reinterpret_cast<const uint16_t*>(&lo) | (uint32_t)*reinterpret_cast<const uint16_t*>(&hi) << 16;
+}
+// two weights as two 16-bit parts each: hi = T(w), lo = T(w - hi)
+template <typename T> __device__ __forceinline__ void split_pair(float x, float y, uint32_t& hi, uint32_t& lo) {
+  const T a = from_f32<T>(x), b = from_f32<T>(y);
+  hi = bits_of<T>(a, b);
+  lo = bits_of<T>(from_f32<T>(x - to_f32<T>(a)), from_f32<T>(y - to_f32<T>(b)));
+}
+
+constexpr int MM_KEYS = 16;
+template <int DP> struct MmaShape {
+  static constexpr int ROW = ((DP / 8) | 1) * 16;                 // an odd number of 16-byte pieces: ldmatrix without bank conflicts
+  static constexpr int SLOT = 2 * MM_KEYS * ROW;                  // keys, then values
+  static constexpr int STAGES = DP == 64 ? 6 : 3;
+  static constexpr int CTAS = DP == 256 ? 1 : 2;                  // per multiprocessor
+  static constexpr int SMEM = AT_WARPS * STAGES * SLOT;
+};
+
+// m16n8k16 products: the query heads of a tile are the 16 rows, 16 cached keys a step.  Scores: A = q (registers), B = keys;
+// values: A = weights (the score accumulators are already in A's layout), B = values (transposed by ldmatrix).  The weights enter as
+// two 16-bit parts, so that they count with 16 bits and more; up to eight heads leave the upper eight rows free, and the low
+// parts ride there at no cost (TWO = false); above that they are a second product.
+template <typename T, int DP, bool TWO>
+__global__ void __launch_bounds__(AT_WARPS * 32, MmaShape<DP>::CTAS) attend_mma_kernel(const AttnParams p) {
+  using S = MmaShape<DP>;
+  constexpr int R = TWO ? 16 : 8;
+  constexpr int STAGES = S::STAGES;
+  constexpr int LPR = DP / 8 > 32 ? 32 : DP / 8;                  // lanes of a row of the copies
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ int64_t s_red[AT_WARPS];
+  __shared__ float2 s_ml[AT_WARPS * R];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * (STAGES * S::SLOT);
+  const uint32_t k_at = ring + ((lane >> 4) * 8 + (lane & 7)) * S::ROW + (lane >> 3 & 1) * 16;
+  const uint32_t v_at = ring + (MM_KEYS + (lane >> 3 & 1) * 8 + (lane & 7)) * S::ROW + (lane >> 4) * 16;
+  float* s_o = reinterpret_cast<float*>(smem);
+  const int nk = p.dim / 16;
+  pdl_trigger();
+  pdl_wait();
+
+  Share s;
+  int64_t unit, unit_end;
+  int b;
+  int64_t base;
+  const int per = p.kv_heads * p.row_tiles;
+  if (p.split) {
+    s = find_share<MM_KEYS>(p, s_red);
+    if (tid == 0) p.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    unit = s.u0; unit_end = s.u1; b = s.b; base = s.base;
+  } else {
+    b = blockIdx.x / per;
+    unit = 0; unit_end = 1; base = 0;
+  }
+  while (unit < unit_end) {
+    int first, end;
+    const int tiles = tiles_of<MM_KEYS>(p, b, &first, &end);
+    int sub, t0, t1;
+    if (p.split) {
+      sub = (int)((unit - base) / tiles);
+      t0 = (int)((unit - base) % tiles);
+      t1 = (int)min((int64_t)tiles, t0 + (unit_end - unit));
+    } else {
+      sub = blockIdx.x % per;
+      t0 = 0; t1 = tiles;
+    }
+    const int h = sub / p.row_tiles, x = sub % p.row_tiles;
+    const int head0 = h * p.group + x * p.rows, rows = min(p.rows, p.group - x * p.rows);
+    const int key0 = first / MM_KEYS * MM_KEYS;
+
+    uint32_t q[DP / 16][TWO ? 4 : 2];
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks)
+#pragma unroll
+      for (int i = 0; i < (TWO ? 4 : 2); ++i) {
+        const int r = TWO ? g + (i & 1) * 8 : g, d = ks * 16 + t4 * 2 + (TWO ? i >> 1 : i) * 8;
+        q[ks][i] = 0;
+        if (r < rows && ks < nk) {
+          const T* src = reinterpret_cast<const T*>(p.q) + (int64_t)b * p.q_b + (int64_t)(head0 + r) * p.q_h + d;
+          q[ks][i] = bits_of<T>(src[0], src[1]);
+        }
+      }
+    float o[DP / 8][4];
+#pragma unroll
+    for (int i = 0; i < DP / 8; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};       // rows g and g + 8; l: of the lane's own keys
+
+    // the page of lane's key is looked up a tile before the copies that need it
+    int page = 0, place = 0;
+    bool ok = false;
+    auto look = [&](int t) {
+      ok = t < t1 && find_key(p, b, key0 + t * MM_KEYS + (lane & 15), first, end, &page, &place);
+    };
+    auto fetch = [&](int slot) -> uint32_t {
+      const uint32_t live = __ballot_sync(0xffffffffu, ok) & 0xffffu;
+#pragma unroll
+      for (int i = 0; i < MM_KEYS * LPR / 32; ++i) {
+        const int row = i * (32 / LPR) + lane / LPR, piece = lane % LPR;
+        const int64_t pg = __shfl_sync(0xffffffffu, page, row), pl = __shfl_sync(0xffffffffu, place, row);
+        const bool on = live >> row & 1;
+        const int64_t ko = on ? pg * p.k_page + pl * p.k_slot + (int64_t)h * p.k_head + piece * 8 : 0;
+        const int64_t vo = on ? pg * p.v_page + pl * p.v_slot + (int64_t)h * p.v_head + piece * 8 : 0;
+        const uint32_t dst = ring + slot * S::SLOT + row * S::ROW + piece * 16;
+        if (piece * 8 < p.dim) {                                  // rows that are not live are filled with zeros
+          cp_async(dst, reinterpret_cast<const T*>(p.k) + ko, on);
+          cp_async(dst + MM_KEYS * S::ROW, reinterpret_cast<const T*>(p.v) + vo, on);
+        }
+      }
+      cp_commit();
+      return live;
+    };
+    const int mine = t0 + warp;
+    uint32_t live_ring[STAGES - 1];
+#pragma unroll
+    for (int st = 0; st < STAGES - 1; ++st) {
+      look(mine + st * AT_WARPS);
+      live_ring[st] = fetch(st);
+    }
+    look(mine + (STAGES - 1) * AT_WARPS);
+    int slot = 0;
+    for (int t = mine; t < t1; t += AT_WARPS) {
+      const uint32_t live = live_ring[0];
+#pragma unroll
+      for (int st = 0; st + 2 < STAGES; ++st) live_ring[st] = live_ring[st + 1];
+      __syncwarp();                                               // every lane has read the slot that is filled next
+      live_ring[STAGES - 2] = fetch(slot == 0 ? STAGES - 1 : slot - 1);
+      look(t + STAGES * AT_WARPS);
+      cp_wait<STAGES - 1>();
+      __syncwarp();
+      const uint32_t off = slot * S::SLOT;
+      slot = slot + 1 == STAGES ? 0 : slot + 1;
+
+      float c[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+      for (int ks = 0; ks < DP / 16; ++ks) {
+        if (ks < nk) {
+          uint32_t kb[4];
+          ldsm4(kb, k_at + off + ks * 32);
+#pragma unroll
+          for (int nt = 0; nt < 2; ++nt) {
+            if constexpr (TWO) mma16816<T>(c[nt], q[ks][0], q[ks][1], q[ks][2], q[ks][3], kb[2 * nt], kb[2 * nt + 1]);
+            else mma16816<T>(c[nt], q[ks][0], 0u, q[ks][1], 0u, kb[2 * nt], kb[2 * nt + 1]);
+          }
+        }
+      }
+      uint32_t hi[4], lo[4];                                      // weights: [key tile][row half]
+#pragma unroll
+      for (int half = 0; half < (TWO ? 2 : 1); ++half) {
+        float sc[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float v = c[i >> 1][half * 2 + (i & 1)] * p.scale;
+          if (p.cap > 0.f) v = p.cap * AT_LOG2E * tanhf(v / p.cap);
+          sc[i] = live >> ((i >> 1) * 8 + t4 * 2 + (i & 1)) & 1 ? v : -INFINITY;
+        }
+        float top = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float mn = fmaxf(m[half], top);
+        const float use = mn == -INFINITY ? 0.f : mn;
+        if (__any_sync(0xffffffffu, mn > m[half])) {              // a new maximum in some row: rescale what is there
+          const float f = exp2f(m[half] - use);
+          l[half] *= f;
+#pragma unroll
+          for (int i = 0; i < DP / 8; ++i) {
+            o[i][2 * half] *= f; o[i][2 * half + 1] *= f;
+            if constexpr (!TWO) { o[i][2] *= f; o[i][3] *= f; }
+          }
+        }
+        m[half] = mn;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { sc[i] = exp2f(sc[i] - use); l[half] += sc[i]; }
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) split_pair<T>(sc[2 * nt], sc[2 * nt + 1], hi[2 * nt + half], lo[2 * nt + half]);
+      }
+#pragma unroll
+      for (int cc = 0; cc < DP / 16; ++cc) {
+        if (cc < nk) {
+          uint32_t vb[4];
+          ldsm4_t(vb, v_at + off + cc * 32);
+#pragma unroll
+          for (int n2 = 0; n2 < 2; ++n2) {
+            if constexpr (TWO) {
+              mma16816<T>(o[2 * cc + n2], hi[0], hi[1], hi[2], hi[3], vb[2 * n2], vb[2 * n2 + 1]);
+              mma16816<T>(o[2 * cc + n2], lo[0], lo[1], lo[2], lo[3], vb[2 * n2], vb[2 * n2 + 1]);
+            } else {
+              mma16816<T>(o[2 * cc + n2], hi[0], lo[0], hi[2], lo[2], vb[2 * n2], vb[2 * n2 + 1]);
+            }
+          }
+        }
+      }
+    }
+    cp_wait<0>();
+    __syncthreads();                                              // the ring becomes the place where the warps' results meet
+#pragma unroll
+    for (int half = 0; half < (TWO ? 2 : 1); ++half) {
+      l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
+      l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
+      const int r = g + half * 8;
+      if (t4 == 0) s_ml[warp * R + r] = make_float2(m[half], l[half]);
+#pragma unroll
+      for (int i = 0; i < DP / 8; ++i) {
+        if (i < 2 * nk) {
+          const float a = TWO ? o[i][2 * half] : o[i][0] + o[i][2], e = TWO ? o[i][2 * half + 1] : o[i][1] + o[i][3];
+          *reinterpret_cast<float2*>(s_o + (warp * R + r) * p.dim + i * 8 + t4 * 2) = make_float2(a, e);
+        }
+      }
+    }
+    __syncthreads();
+    const bool whole = t0 == 0 && t1 == tiles;
     store_tile<T>(p, s_o, s_ml, b, head0, rows, R, whole ? -1 : 2 * (int)blockIdx.x + (t0 == 0));
     if (!p.split) break;
     if (!whole && t0 == 0 && tid == 0)
@@ -376,19 +611,10 @@ __global__ void __launch_bounds__(AT_WARPS * 32) attend_fma_kernel(const AttnPar
   }
 }
 
-template <typename T, int R, int NI>
-int run_fma(AttnParams& p, int64_t items, int64_t max_ctas, cudaStream_t st) {
-  constexpr int STAGES = R == 8 ? 3 : 2;
-  constexpr int ring = AT_WARPS * STAGES * 2 * (32 / R) * NI * 128 * (int)sizeof(T), join = AT_WARPS * R * NI * 128 * 4;
-  constexpr int smem = ring > join ? ring : join;
-  auto kern = attend_fma_kernel<T, R, NI, STAGES>;
-  static DeviceOnce attr_set;
-  if (attr_set.first_time()) {
-    KQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    attr_set.done();
-  }
+template <typename T>
+int launch_both(void (*kern)(const AttnParams), AttnParams& p, int smem, int ctas_per_sm, cudaStream_t st) {
   const bool pdl = options().pdl != 0;
-  const unsigned grid = (unsigned)(p.split ? max_ctas : items);
+  const unsigned grid = p.split ? (unsigned)(sm_count() * ctas_per_sm) : (unsigned)((int64_t)p.batch * p.kv_heads * p.row_tiles);
   KQ_CUDA_TRY(launch_pdl(kern, dim3(grid), dim3(AT_WARPS * 32), (size_t)smem, st, pdl, p));
   options().launches += 1;
   if (p.split) {
@@ -398,15 +624,55 @@ int run_fma(AttnParams& p, int64_t items, int64_t max_ctas, cudaStream_t st) {
   return KQ_OK;
 }
 
-template <typename T>
-int run_attention(AttnParams& p, int64_t items, int64_t max_ctas, cudaStream_t st) {
-  const bool wide = p.dim > 128;
-  if (p.rows <= 4) return wide ? run_fma<T, 4, 2>(p, items, max_ctas, st) : run_fma<T, 4, 1>(p, items, max_ctas, st);
-  return wide ? run_fma<T, 8, 2>(p, items, max_ctas, st) : run_fma<T, 8, 1>(p, items, max_ctas, st);
+template <int R, int NI>
+int run_fma(AttnParams& p, cudaStream_t st) {
+  constexpr int STAGES = R == 8 ? 3 : 2;
+  constexpr int ring = AT_WARPS * STAGES * 2 * (32 / R) * NI * 512, join = AT_WARPS * R * NI * 128 * 4;
+  constexpr int smem = ring > join ? ring : join;
+  auto kern = attend_fma_kernel<R, NI, STAGES>;
+  static DeviceOnce attr_set;
+  if (attr_set.first_time()) {
+    KQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    attr_set.done();
+  }
+  return launch_both<float>(kern, p, smem, AT_MAX_CTAS, st);
 }
 
-constexpr int AT_MAX_CTAS = 2;          // per multiprocessor
-constexpr int AT_MAX_ROWS = 8;
+template <typename T, int DP, bool TWO>
+int run_mma(AttnParams& p, cudaStream_t st) {
+  using S = MmaShape<DP>;
+  constexpr int join = AT_WARPS * (TWO ? 16 : 8) * DP * 4;
+  constexpr int smem = S::SMEM > join ? S::SMEM : join;
+  auto kern = attend_mma_kernel<T, DP, TWO>;
+  static DeviceOnce attr_set;
+  if (attr_set.first_time()) {
+    KQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    attr_set.done();
+  }
+  return launch_both<T>(kern, p, smem, S::CTAS, st);
+}
+
+// the query heads of a key head in tiles of at most `most` rows, of even sizes
+void set_rows(AttnParams& p, int most) {
+  p.row_tiles = (p.group + most - 1) / most;
+  p.rows = (p.group + p.row_tiles - 1) / p.row_tiles;
+  p.row_tiles = (p.group + p.rows - 1) / p.rows;
+}
+
+int run_f32(AttnParams& p, cudaStream_t st) {
+  set_rows(p, 8);
+  if (p.rows <= 4) return p.dim > 128 ? run_fma<4, 2>(p, st) : run_fma<4, 1>(p, st);
+  return p.dim > 128 ? run_fma<8, 2>(p, st) : run_fma<8, 1>(p, st);
+}
+
+template <typename T>
+int run_16bit(AttnParams& p, cudaStream_t st) {
+  set_rows(p, 16);
+  if (p.rows <= 8) return p.dim > 128 ? run_mma<T, 256, false>(p, st) : p.dim > 64 ? run_mma<T, 128, false>(p, st) : run_mma<T, 64, false>(p, st);
+  return p.dim > 128 ? run_mma<T, 256, true>(p, st) : p.dim > 64 ? run_mma<T, 128, true>(p, st) : run_mma<T, 64, true>(p, st);
+}
+
+constexpr int AT_MAX_ROWS = 16;
 
 struct Scratch { size_t o, ml, meta, total; };
 Scratch scratch_of(int64_t ctas, int64_t dim) {
@@ -475,22 +741,18 @@ int kq_paged_attention(const void* q, int dtype, int64_t batch, int64_t heads, i
   p.table = block_table; p.table_b = table_stride; p.width = (int)table_width; p.lens = seq_lens;
   p.batch = (int)batch; p.heads = (int)heads; p.kv_heads = (int)kv_heads; p.group = (int)(heads / kv_heads); p.dim = (int)head_dim;
   p.page_size = (int)page_size; p.num_pages = num_pages;
-  p.row_tiles = (p.group + AT_MAX_ROWS - 1) / AT_MAX_ROWS;
-  p.rows = (p.group + p.row_tiles - 1) / p.row_tiles;
-  p.row_tiles = (p.group + p.rows - 1) / p.rows;
   p.scale = softcap > 0.f ? scale : scale * AT_LOG2E; p.cap = softcap; p.window = (int)window;
   p.out = out; p.lse = lse;
   uint8_t* sb = (uint8_t*)scratch;
   p.part_o = (float*)(sb + L.o); p.part_ml = (float2*)(sb + L.ml); p.meta = (int4*)(sb + L.meta);
-  const int64_t items = batch * kv_heads * p.row_tiles;
   int64_t most = table_width * page_size;          // keys that a sequence can show
   if (window > 0 && window < most) most = window;
-  p.split = most > 256 || items > 0x7fffffff;      // short sequences: one launch, one CTA per item
+  p.split = most > 256;      // short sequences: one launch, one CTA per item
   cudaStream_t st = (cudaStream_t)stream;
   switch (dtype) {
-    case KQ_F32: return run_attention<float>(p, items, ctas, st);
-    case KQ_F16: return run_attention<__half>(p, items, ctas, st);
-    default: return run_attention<__nv_bfloat16>(p, items, ctas, st);
+    case KQ_F32: return run_f32(p, st);
+    case KQ_F16: return run_16bit<__half>(p, st);
+    default: return run_16bit<__nv_bfloat16>(p, st);
   }
 }
 
