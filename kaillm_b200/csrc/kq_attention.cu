@@ -7,8 +7,8 @@
 // share a key head (their rows are one tile) in registers, in fp32, and rescales them when a new maximum comes.
 //
 // The work is cut by cached keys, not by sequences: an item is (sequence, key head, row tile) and has one unit of work per
-// tile of keys; the units of all items, in order, are divided evenly over the CTAs of one wave.  A CTA finds its share from
-// the lengths themselves (a sum and a scan, the lengths stay on the GPU), so a batch of any mix of lengths is balanced and a
+// tile of keys, behind AT_START units for its beginning and end; the units of all items, in order, are divided evenly over the
+// CTAs of one wave.  A CTA finds its share from the lengths themselves (a sum and a scan, the lengths stay on the GPU), so a batch of any mix of lengths is balanced and a
 // captured call follows the lengths of each replay.  An item inside one CTA is finished there; one that crosses CTAs leaves
 // partial results (unnormalised values, maximum, sum) that attend_join_kernel adds in the order of the keys: no atomics, the
 // same bits every time.
@@ -22,6 +22,10 @@ namespace {
 
 constexpr int AT_MAX_CTAS = 2;         // per multiprocessor
 constexpr int AT_WARPS = 4;            // warps of a CTA: each walks every fourth tile of keys of the CTA's share on its own
+// An item costs as much as so many tiles beside its own (loading q, filling the ring, joining the warps).  Without it the CTAs
+// that get the short sequences of a mixed batch end last: 64 sequences of 0..4k tokens, busy cycles of the slowest SM 290k
+// against 197k of the fastest.
+constexpr int AT_START = 8;
 constexpr float AT_LOG2E = 1.4426950408889634f;
 constexpr float AT_LN2 = 0.6931471805599453f;
 
@@ -61,7 +65,7 @@ __device__ Share find_share(const AttnParams& p, int64_t* s_red) {
   const int per = p.kv_heads * p.row_tiles;
   int64_t sum = 0;
   int f, e;
-  for (int b = tid; b < p.batch; b += AT_WARPS * 32) sum += tiles_of<TK>(p, b, &f, &e);
+  for (int b = tid; b < p.batch; b += AT_WARPS * 32) sum += AT_START + tiles_of<TK>(p, b, &f, &e);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
   if (lane == 0) s_red[warp] = sum;
@@ -71,8 +75,8 @@ __device__ Share find_share(const AttnParams& p, int64_t* s_red) {
 #pragma unroll
   for (int w = 0; w < AT_WARPS; ++w) s.total += s_red[w];
   s.total *= per;
-  // a CTA without a tile for each of its warps would only add partial results
-  s.ctas = (int)min((int64_t)gridDim.x, (s.total + AT_WARPS - 1) / AT_WARPS);
+  // a share that is hardly more than a beginning would only add partial results
+  s.ctas = (int)min((int64_t)gridDim.x, (s.total + AT_START + AT_WARPS - 1) / (AT_START + AT_WARPS));
   s.u0 = s.total * blockIdx.x / s.ctas;
   s.u1 = s.total * (blockIdx.x + 1) / s.ctas;
   s.b = 0;
@@ -81,7 +85,7 @@ __device__ Share find_share(const AttnParams& p, int64_t* s_red) {
   // every warp scans the sequences 32 at a time until it reaches the one that holds u0
   int64_t run = 0;
   for (int b0 = 0; b0 < p.batch; b0 += 32) {
-    int64_t v = b0 + lane < p.batch ? (int64_t)tiles_of<TK>(p, b0 + lane, &f, &e) * per : 0;
+    int64_t v = b0 + lane < p.batch ? (int64_t)(AT_START + tiles_of<TK>(p, b0 + lane, &f, &e)) * per : 0;
     const int64_t own = v;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -224,11 +228,17 @@ __global__ void __launch_bounds__(AT_WARPS * 32) attend_fma_kernel(const AttnPar
   while (unit < unit_end) {
     int first, end;
     const int tiles = tiles_of<KB>(p, b, &first, &end);
-    int sub, t0, t1;                               // (key head, row tile), first and last + 1 tile of this segment
+    int64_t next_base = base;
+    int next_b = b, sub, t0, t1;                   // (key head, row tile), first and last + 1 tile of this segment
     if (p.split) {
-      sub = (int)((unit - base) / tiles);
-      t0 = (int)((unit - base) % tiles);
-      t1 = (int)min((int64_t)tiles, t0 + (unit_end - unit));
+      const int cost = AT_START + tiles;
+      sub = (int)((unit - base) / cost);
+      const int at = (int)((unit - base) % cost);
+      const int upto = (int)min((int64_t)cost, at + (unit_end - unit));
+      t0 = max(at - AT_START, 0); t1 = upto - AT_START;
+      unit += upto - at;
+      if (unit == base + (int64_t)cost * per) { next_base = unit; next_b = b + 1; }
+      if (t1 <= 0) { base = next_base; b = next_b; continue; }    // the next CTA begins this item
     } else {
       sub = blockIdx.x % per;
       t0 = 0; t1 = tiles;
@@ -366,10 +376,10 @@ __global__ void __launch_bounds__(AT_WARPS * 32) attend_fma_kernel(const AttnPar
     store_tile<float>(p, s_o, s_ml, b, head0, rows, R, whole ? -1 : 2 * (int)blockIdx.x + (t0 == 0));
     if (!p.split) break;
     if (!whole && t0 == 0 && tid == 0)
-      p.meta[blockIdx.x] = make_int4(b * per + sub, cta_of(s, base + (int64_t)(sub + 1) * tiles - 1), 0, 0);
+      p.meta[blockIdx.x] = make_int4(b * per + sub, cta_of(s, base + (int64_t)(sub + 1) * (AT_START + tiles) - 1), 0, 0);
     __syncthreads();
-    unit += t1 - t0;
-    if (unit == base + (int64_t)tiles * per) { base = unit; ++b; }
+    base = next_base;
+    b = next_b;
   }
 }
 
@@ -417,7 +427,8 @@ __global__ void __launch_bounds__(AT_WARPS * 32, MmaShape<DP>::CTAS) attend_mma_
   using S = MmaShape<DP>;
   constexpr int R = TWO ? 16 : 8;
   constexpr int STAGES = S::STAGES;
-  constexpr int LPR = DP / 8 > 32 ? 32 : DP / 8;                  // lanes of a row of the copies
+  constexpr int LPR = DP / 8;                                     // lanes of a row of the copies
+  constexpr int COPIES = MM_KEYS * LPR / 32;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int64_t s_red[AT_WARPS];
   __shared__ float2 s_ml[AT_WARPS * R];
@@ -427,6 +438,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, MmaShape<DP>::CTAS) attend_mma_
   const uint32_t v_at = ring + (MM_KEYS + (lane >> 3 & 1) * 8 + (lane & 7)) * S::ROW + (lane >> 4) * 16;
   float* s_o = reinterpret_cast<float*>(smem);
   const int nk = p.dim / 16;
+  const bool one_page = p.page_size % MM_KEYS == 0;               // tiles start at multiples of 16
   pdl_trigger();
   pdl_wait();
 
@@ -446,11 +458,17 @@ __global__ void __launch_bounds__(AT_WARPS * 32, MmaShape<DP>::CTAS) attend_mma_
   while (unit < unit_end) {
     int first, end;
     const int tiles = tiles_of<MM_KEYS>(p, b, &first, &end);
-    int sub, t0, t1;
+    int64_t next_base = base;
+    int next_b = b, sub, t0, t1;
     if (p.split) {
-      sub = (int)((unit - base) / tiles);
-      t0 = (int)((unit - base) % tiles);
-      t1 = (int)min((int64_t)tiles, t0 + (unit_end - unit));
+      const int cost = AT_START + tiles;
+      sub = (int)((unit - base) / cost);
+      const int at = (int)((unit - base) % cost);
+      const int upto = (int)min((int64_t)cost, at + (unit_end - unit));
+      t0 = max(at - AT_START, 0); t1 = upto - AT_START;
+      unit += upto - at;
+      if (unit == base + (int64_t)cost * per) { next_base = unit; next_b = b + 1; }
+      if (t1 <= 0) { base = next_base; b = next_b; continue; }    // the next CTA begins this item
     } else {
       sub = blockIdx.x % per;
       t0 = 0; t1 = tiles;
@@ -478,25 +496,44 @@ __global__ void __launch_bounds__(AT_WARPS * 32, MmaShape<DP>::CTAS) attend_mma_
       for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};       // rows g and g + 8; l: of the lane's own keys
 
-    // the page of lane's key is looked up a tile before the copies that need it
-    int page = 0, place = 0;
+    // the page of the lane's key is looked up a tile before the copies that need it; k_lane, v_lane: the lane's piece of its first
+    // row, in the first page
+    int page32 = 0, place = 0;
+    int64_t page = 0, place0 = 0;                                 // place0: of the tile's first key, seen from the lane's
     bool ok = false;
     auto look = [&](int t) {
-      ok = t < t1 && find_key(p, b, key0 + t * MM_KEYS + (lane & 15), first, end, &page, &place);
+      ok = t < t1 && find_key(p, b, key0 + t * MM_KEYS + (lane & 15), first, end, &page32, &place);
+      page = page32;
+      place0 = place - (lane & 15);
     };
+    const int piece = lane % LPR;
+    const T* k_lane = static_cast<const T*>(p.k) + ((int64_t)h * p.k_head + (lane / LPR) * p.k_slot + piece * 8);
+    const T* v_lane = static_cast<const T*>(p.v) + ((int64_t)h * p.v_head + (lane / LPR) * p.v_slot + piece * 8);
     auto fetch = [&](int slot) -> uint32_t {
       const uint32_t live = __ballot_sync(0xffffffffu, ok) & 0xffffu;
+      const uint32_t dst = ring + slot * S::SLOT + (lane / LPR) * S::ROW + piece * 16;
+      if (live == 0xffffu && one_page) {                          // 16 tokens of one page: one address and a fixed step
+        if (piece * 8 < p.dim) {
+          const T* kp = k_lane + (page * p.k_page + place0 * p.k_slot);
+          const T* vp = v_lane + (page * p.v_page + place0 * p.v_slot);
 #pragma unroll
-      for (int i = 0; i < MM_KEYS * LPR / 32; ++i) {
-        const int row = i * (32 / LPR) + lane / LPR, piece = lane % LPR;
-        const int64_t pg = __shfl_sync(0xffffffffu, page, row), pl = __shfl_sync(0xffffffffu, place, row);
-        const bool on = live >> row & 1;
-        const int64_t ko = on ? pg * p.k_page + pl * p.k_slot + (int64_t)h * p.k_head + piece * 8 : 0;
-        const int64_t vo = on ? pg * p.v_page + pl * p.v_slot + (int64_t)h * p.v_head + piece * 8 : 0;
-        const uint32_t dst = ring + slot * S::SLOT + row * S::ROW + piece * 16;
-        if (piece * 8 < p.dim) {                                  // rows that are not live are filled with zeros
-          cp_async(dst, reinterpret_cast<const T*>(p.k) + ko, on);
-          cp_async(dst + MM_KEYS * S::ROW, reinterpret_cast<const T*>(p.v) + vo, on);
+          for (int i = 0; i < COPIES; ++i) {
+            cp_async(dst + i * (32 / LPR) * S::ROW, kp, true);
+            cp_async(dst + (MM_KEYS + i * (32 / LPR)) * S::ROW, vp, true);
+            kp += (32 / LPR) * p.k_slot;
+            vp += (32 / LPR) * p.v_slot;
+          }
+        }
+      } else {
+#pragma unroll 1
+        for (int i = 0; i < COPIES; ++i) {
+          const int row = i * (32 / LPR) + lane / LPR;
+          const int64_t pg = __shfl_sync(0xffffffffu, page, row), pl = __shfl_sync(0xffffffffu, place0 + (lane & 15), row) - lane / LPR;
+          const bool on = live >> row & 1;
+          if (piece * 8 < p.dim) {                                // rows that are not live are filled with zeros
+            cp_async(dst + i * (32 / LPR) * S::ROW, on ? k_lane + (pg * p.k_page + pl * p.k_slot) : k_lane, on);
+            cp_async(dst + (MM_KEYS + i * (32 / LPR)) * S::ROW, on ? v_lane + (pg * p.v_page + pl * p.v_slot) : v_lane, on);
+          }
         }
       }
       cp_commit();
@@ -604,10 +641,10 @@ __global__ void __launch_bounds__(AT_WARPS * 32, MmaShape<DP>::CTAS) attend_mma_
     store_tile<T>(p, s_o, s_ml, b, head0, rows, R, whole ? -1 : 2 * (int)blockIdx.x + (t0 == 0));
     if (!p.split) break;
     if (!whole && t0 == 0 && tid == 0)
-      p.meta[blockIdx.x] = make_int4(b * per + sub, cta_of(s, base + (int64_t)(sub + 1) * tiles - 1), 0, 0);
+      p.meta[blockIdx.x] = make_int4(b * per + sub, cta_of(s, base + (int64_t)(sub + 1) * (AT_START + tiles) - 1), 0, 0);
     __syncthreads();
-    unit += t1 - t0;
-    if (unit == base + (int64_t)tiles * per) { base = unit; ++b; }
+    base = next_base;
+    b = next_b;
   }
 }
 
