@@ -362,6 +362,10 @@ int kq_paged_attention(const void* q, int dtype, int64_t batch, int64_t heads, i
                        float scale, int64_t window, float softcap, void* out, float* lse, void* scratch,
                        size_t scratch_bytes, void* stream);
 
+/* A bounded wait inside a kernel of kq_paged_attention that ran out leaves a non-zero word (its outputs are then undefined), which
+ * this call copies to *status (SYNCHRONISES; may be NULL) and, with clear != 0, zeroes. */
+int kq_paged_attention_status(int* status, int clear);
+
 /* Page tables, slots and positions of a step.  Request r has seq_lens[r] tokens in the cache and new_lens[r] tokens to come
  * (negative values count as 0).  It holds ceil(seq_lens[r] / page_size) pages, named by its row of block_table, and takes what it
  * needs more from free_pages, in order: request 0's first page is free_pages[taken[0]].  Written:

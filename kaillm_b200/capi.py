@@ -25,7 +25,7 @@ EXPORTS = (
     "kq_p2p_allgather", "kq_read_status_static", "kq_debug_copy_window", "kq_prepare_q8_rmsnorm", "kq_prepare_q8_swiglu",
     "kq_p2p_allgather_2d", "kq_mul_mat_prepared_gather", "kq_moe_a8_vec", "kq_moe_a8", "kq_moe_block_size", "kq_dequantize_rows", "kq_wait_arrival", "kq_arrival_status",
     "kq_dequant_mul_mat_supported", "kq_dequant_mul_mat_preferred", "kq_dequant_mul_mat", "kq_dequant_mul_mat_status", "kq_moe_project", "kq_moe_align", "kq_moe_combine",
-    "kq_qk_norm_rope", "kq_paged_attention_workspace_bytes", "kq_paged_attention", "kq_plan_pages", "kq_moe_route",
+    "kq_qk_norm_rope", "kq_paged_attention_workspace_bytes", "kq_paged_attention", "kq_paged_attention_status", "kq_plan_pages", "kq_moe_route",
 )
 
 
@@ -372,6 +372,13 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
             v_cache.data_ptr(), _strides3(v_cache), k_cache.shape[0], k_cache.shape[1], block_table.data_ptr(), block_table.stride(0),
             block_table.shape[1], seq_lens.data_ptr(), scale, window, softcap, out.data_ptr(), lse.data_ptr() if lse is not None else None,
             scratch.data_ptr(), scratch.numel(), _stream(q.device)))
+
+
+def paged_attention_status(clear: bool = False) -> int:
+    """kq_paged_attention_status on the current device (synchronises): non-zero when a wait inside the kernel has run out."""
+    v = ctypes.c_int()
+    _check(lib.kq_paged_attention_status(ctypes.byref(v), int(clear)))
+    return v.value
 
 
 def debug_group_dots(W: torch.Tensor, x: torch.Tensor, qtype: int):

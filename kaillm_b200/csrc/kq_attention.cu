@@ -7,7 +7,7 @@
 // share a key head (their rows are one tile) in registers, in fp32, and rescales them when a new maximum comes.
 //
 // The work is cut by cached keys, not by sequences: an item is (sequence, key head, row tile) and has one unit of work per
-// tile of keys, behind AT_START units for its beginning and end; the units of all items, in order, are divided evenly over the
+// tile of keys, behind a few units for its beginning and end; the units of all items, in order, are divided evenly over the
 // CTAs of one wave.  A CTA finds its share from the lengths themselves (a sum and a scan, the lengths stay on the GPU), so a batch of any mix of lengths is balanced and a
 // captured call follows the lengths of each replay.  An item inside one CTA is finished there; one that crosses CTAs leaves
 // partial results (unnormalised values, maximum, sum) that attend_join_kernel adds in the order of the keys: no atomics, the
@@ -20,14 +20,12 @@ namespace kq {
 
 namespace {
 
-constexpr int AT_MAX_CTAS = 2;         // per multiprocessor
-constexpr int AT_WARPS = 4;            // warps of a CTA: each walks every fourth tile of keys of the CTA's share on its own
-// An item costs as much as so many tiles beside its own (loading q, filling the ring, joining the warps).  Without it the CTAs
-// that get the short sequences of a mixed batch end last: 64 sequences of 0..4k tokens, busy cycles of the slowest SM 290k
-// against 197k of the fastest.
-constexpr int AT_START = 8;
+#include "kq_tile_common.cuh"
+
 constexpr float AT_LOG2E = 1.4426950408889634f;
 constexpr float AT_LN2 = 0.6931471805599453f;
+
+__device__ int g_attend_status = 0;
 
 struct AttnParams {
   const void* q; int64_t q_b, q_h;                     // strides in elements; the head dimension is dense everywhere
@@ -42,11 +40,11 @@ struct AttnParams {
   int window;
   void* out;                                           // [batch][heads][dim]
   float* lse;                                          // [batch][heads] or null
-  float* part_o; float2* part_ml; int4* meta;          // two partial results per CTA, and which items start here but end elsewhere
+  float* part_o; float2* part_ml; int2* meta;          // two partial results per CTA; which item starts in a CTA and ends in which other
   int split;                                           // 0: one CTA per item
 };
 
-// tiles of keys of sequence b (at least one, so that an empty row is visited too); *first..*end: its visible keys
+// tiles of TK keys of sequence b (at least one, so that an empty row is visited too); *first..*end: its visible keys
 template <int TK>
 __device__ __forceinline__ int tiles_of(const AttnParams& p, int b, int* first, int* end) {
   const int len = max(p.lens[b], 0);
@@ -56,59 +54,103 @@ __device__ __forceinline__ int tiles_of(const AttnParams& p, int b, int* first, 
   return max(1, (*end + TK - 1) / TK - *first / TK);
 }
 
-// The share of this CTA: units [u0, u1), and the sequence and offset of u0.
-struct Share { int64_t u0, u1, base; int b; int64_t total; int ctas; };
+// A stretch of an item's tiles that one CTA works on.
+struct Segment {
+  int b, sub;            // sequence, (key head, row tile)
+  int first, end;        // visible keys
+  int t0, t1, tiles;     // tiles [t0, t1) of `tiles`; tile 0 starts at the last multiple of TK not above `first`
+  int last;              // the CTA that works on the item's last tile
+};
 
-template <int TK>
-__device__ Share find_share(const AttnParams& p, int64_t* s_red) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int per = p.kv_heads * p.row_tiles;
-  int64_t sum = 0;
-  int f, e;
-  for (int b = tid; b < p.batch; b += AT_WARPS * 32) sum += AT_START + tiles_of<TK>(p, b, &f, &e);
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-  if (lane == 0) s_red[warp] = sum;
-  __syncthreads();
-  Share s;
-  s.total = 0;
-#pragma unroll
-  for (int w = 0; w < AT_WARPS; ++w) s.total += s_red[w];
-  s.total *= per;
-  // a share that is hardly more than a beginning would only add partial results
-  s.ctas = (int)min((int64_t)gridDim.x, (s.total + AT_START + AT_WARPS - 1) / (AT_START + AT_WARPS));
-  s.u0 = s.total * blockIdx.x / s.ctas;
-  s.u1 = s.total * (blockIdx.x + 1) / s.ctas;
-  s.b = 0;
-  s.base = 0;
-  if ((int)blockIdx.x >= s.ctas) { s.u0 = s.u1 = 0; return s; }
-  // every warp scans the sequences 32 at a time until it reaches the one that holds u0
-  int64_t run = 0;
-  for (int b0 = 0; b0 < p.batch; b0 += 32) {
-    int64_t v = b0 + lane < p.batch ? (int64_t)(AT_START + tiles_of<TK>(p, b0 + lane, &f, &e)) * per : 0;
-    const int64_t own = v;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int64_t u = __shfl_up_sync(0xffffffffu, v, d);
-      if (lane >= d) v += u;
-    }
-    const unsigned past = __ballot_sync(0xffffffffu, run + v > s.u0);
-    if (past) {
-      const int at = __ffs(past) - 1;
-      s.b = b0 + at;
-      s.base = run + __shfl_sync(0xffffffffu, v - own, at);
-      break;
-    }
-    run += __shfl_sync(0xffffffffu, v, 31);
+// The segments of one CTA, in order.  START: what an item costs beside its tiles, in tiles (loading q, joining the warps; without
+// it the CTAs that get the short sequences of a mixed batch end last).
+template <int TK, int START>
+struct Walk {
+  int64_t left, pos, total;       // units left, unit index, units of all items
+  int ctas;
+  int b, sub, at, first, end, tiles;
+
+  __device__ void load(const AttnParams& p) { if (b < p.batch) tiles = tiles_of<TK>(p, b, &first, &end); }
+
+  __device__ void begin_item(const AttnParams& p, int item) {
+    const int per = p.kv_heads * p.row_tiles;
+    b = item / per; sub = item - b * per; at = START; left = 0x7fffffff; pos = 0; total = 1; ctas = 1;
+    load(p);
+    left = tiles;
   }
-  return s;
-}
 
-__device__ __forceinline__ int cta_of(const Share& s, int64_t unit) {   // the CTA whose share holds `unit`
-  int c = (int)(unit * s.ctas / s.total);
-  while (c + 1 < s.ctas && s.total * (c + 1) / s.ctas <= unit) ++c;
-  while (c > 0 && s.total * c / s.ctas > unit) --c;
-  return c;
+  // called by `threads` threads at once; s_red: one int64 per warp
+  __device__ void begin_share(const AttnParams& p, int64_t* s_red, int threads) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int per = p.kv_heads * p.row_tiles;
+    int64_t sum = 0;
+    int f, e;
+    for (int i = tid; i < p.batch; i += threads) sum += START + tiles_of<TK>(p, i, &f, &e);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    if (lane == 0) s_red[warp] = sum;
+    __syncthreads();
+    total = 0;
+    for (int w = 0; w < threads / 32; ++w) total += s_red[w];
+    total *= per;
+    // a share that is hardly more than a beginning would only add partial results
+    ctas = (int)min((int64_t)gridDim.x, (total + START + 3) / (START + 4));
+    pos = total * blockIdx.x / ctas;
+    left = total * (blockIdx.x + 1) / ctas - pos;
+    b = sub = at = 0;
+    if ((int)blockIdx.x >= ctas) { left = 0; return; }
+    // every warp scans the sequences 32 at a time until it reaches the one that holds `pos`
+    int64_t run = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += 32) {
+      int64_t v = b0 + lane < p.batch ? (int64_t)(START + tiles_of<TK>(p, b0 + lane, &f, &e)) * per : 0;
+      const int64_t own = v;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int64_t u = __shfl_up_sync(0xffffffffu, v, d);
+        if (lane >= d) v += u;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, run + v > pos);
+      if (past) {
+        const int i = __ffs(past) - 1;
+        b = b0 + i;
+        const int64_t in = pos - run - __shfl_sync(0xffffffffu, v - own, i);
+        load(p);
+        sub = (int)(in / (START + tiles));
+        at = (int)(in - (int64_t)sub * (START + tiles));
+        break;
+      }
+      run += __shfl_sync(0xffffffffu, v, 31);
+    }
+  }
+
+  __device__ int cta_of(int64_t unit) const {     // the CTA whose share holds `unit`
+    int c = (int)(unit * ctas / total);
+    while (c + 1 < ctas && total * (c + 1) / ctas <= unit) ++c;
+    while (c > 0 && total * c / ctas > unit) --c;
+    return c;
+  }
+
+  __device__ bool next(const AttnParams& p, Segment* s) {
+    while (left > 0) {
+      const int cost = START + tiles, take = (int)min((int64_t)(cost - at), left);
+      s->b = b; s->sub = sub; s->first = first; s->end = end; s->tiles = tiles;
+      s->t0 = max(at - START, 0); s->t1 = at + take - START;
+      s->last = -1;
+      if (s->t0 == 0 && s->t1 > 0 && s->t1 < tiles) s->last = cta_of(pos + cost - at - 1);
+      left -= take; pos += take; at += take;
+      if (at == cost) {
+        at = 0;
+        if (++sub == p.kv_heads * p.row_tiles) { sub = 0; ++b; load(p); }
+      }
+      if (s->t1 > 0) return true;                 // otherwise the next CTA begins this item
+    }
+    return false;
+  }
+};
+
+// index of a segment's partial result, -1 if it is the whole item
+__device__ __forceinline__ int part_of(const Segment& s) {
+  return s.t0 == 0 && s.t1 == s.tiles ? -1 : 2 * (int)blockIdx.x + (s.t0 == 0);
 }
 
 // 16 bytes, or with live = false 16 bytes of zeros and no read
@@ -117,65 +159,62 @@ __device__ __forceinline__ void cp_async(uint32_t dst, const void* src, bool liv
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ float ex2(float x) {      // 2^x, relative error 2^-22; results below 2^-126 become 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
-// Writes the tile's results: s_o [AT_WARPS][rows][dim] unnormalised values of the warps, s_ml their maxima and sums.
-// `slot` < 0: the item is complete; otherwise the index of its partial result.
+// One value of a finished row, or of a partial one: o relative to 2^m, l the row's sum.
 template <typename T>
-__device__ void store_tile(const AttnParams& p, const float* s_o, const float2* s_ml, int b, int head0, int rows, int R, int slot) {
-  const int n = rows * p.dim;
-  for (int i = threadIdx.x; i < n; i += AT_WARPS * 32) {
-    const int r = i / p.dim, d = i - r * p.dim;
-    float m = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < AT_WARPS; ++w) m = fmaxf(m, s_ml[w * R + r].x);
-    const float mm = m == -INFINITY ? 0.f : m;
-    float l = 0.f, o = 0.f;
-#pragma unroll
-    for (int w = 0; w < AT_WARPS; ++w) {
-      const float f = exp2f(s_ml[w * R + r].x - mm);
-      l += s_ml[w * R + r].y * f;
-      o += s_o[(w * R + r) * p.dim + d] * f;
-    }
-    if (slot < 0) {
-      reinterpret_cast<T*>(p.out)[((int64_t)b * p.heads + head0 + r) * p.dim + d] = from_f32<T>(l == 0.f ? 0.f : o / l);
-      if (d == 0 && p.lse) p.lse[(int64_t)b * p.heads + head0 + r] = l == 0.f ? -INFINITY : m * AT_LN2 + logf(l);
-    } else {
-      p.part_o[((int64_t)slot * p.rows + r) * p.dim + d] = o;
-      if (d == 0) p.part_ml[(int64_t)slot * p.rows + r] = make_float2(m, l);
-    }
+__device__ __forceinline__ void put(const AttnParams& p, int part, int b, int head0, int r, int d, float o, float m, float l) {
+  if (part < 0) {
+    static_cast<T*>(p.out)[((int64_t)b * p.heads + head0 + r) * p.dim + d] = from_f32<T>(l == 0.f ? 0.f : o / l);
+    if (d == 0 && p.lse) p.lse[(int64_t)b * p.heads + head0 + r] = l == 0.f ? -INFINITY : m * AT_LN2 + logf(l);
+  } else {
+    p.part_o[((int64_t)part * p.rows + r) * p.dim + d] = o;
+    if (d == 0) p.part_ml[(int64_t)part * p.rows + r] = make_float2(m, l);
   }
 }
 
-// Adds the partial results of the item that starts in share c and ends in share meta.y, in the order of the keys.
+// Adds the partial results of the item that starts in share c and ends in share meta.y: a warp takes every fourth of them, the four
+// sums are added in order.
 template <typename T>
 __global__ void __launch_bounds__(128) attend_join_kernel(const AttnParams p) {
+  __shared__ float s_o[4][256];
+  __shared__ float s_l[4];
   pdl_trigger();
   pdl_wait();
-  const int c = blockIdx.x;
-  const int4 m4 = p.meta[c];
-  const int item = m4.x, last = m4.y;
-  if (item < 0) return;
+  const int c = blockIdx.x, r = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int2 it = p.meta[c];
+  if (it.x < 0) return;
   const int per = p.kv_heads * p.row_tiles;
-  const int b = item / per, h = item % per / p.row_tiles, x = item % p.row_tiles;
-  const int head0 = h * p.group + x * p.rows, rows = min(p.rows, p.group - x * p.rows);
-  const int r = blockIdx.y;
-  if (r >= rows) return;
+  const int b = it.x / per, sub = it.x - b * per, h = sub / p.row_tiles, x = sub - h * p.row_tiles;
+  const int head0 = h * p.group + x * p.rows;
+  if (r >= min(p.rows, p.group - x * p.rows)) return;
+  auto at = [&](int i) { return (int64_t)(2 * i + (i == c)) * p.rows + r; };
   float m = -INFINITY;
-  for (int i = c; i <= last; ++i) m = fmaxf(m, p.part_ml[(int64_t)(2 * i + (i == c)) * p.rows + r].x);
-  const float mm = m == -INFINITY ? 0.f : m;
-  for (int d = threadIdx.x; d < p.dim; d += 128) {
-    float l = 0.f, o = 0.f;
+  for (int i = c + lane; i <= it.y; i += 32) m = fmaxf(m, p.part_ml[at(i)].x);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+  const float use = m == -INFINITY ? 0.f : m;
+  float l = 0.f, o[8] = {};
 #pragma unroll 4
-    for (int i = c; i <= last; ++i) {
-      const int64_t at = (int64_t)(2 * i + (i == c)) * p.rows + r;
-      const float2 ml = p.part_ml[at];
-      const float f = exp2f(ml.x - mm);
-      l += ml.y * f;
-      o += p.part_o[at * p.dim + d] * f;
-    }
-    reinterpret_cast<T*>(p.out)[((int64_t)b * p.heads + head0 + r) * p.dim + d] = from_f32<T>(l == 0.f ? 0.f : o / l);
-    if (d == 0 && p.lse) p.lse[(int64_t)b * p.heads + head0 + r] = l == 0.f ? -INFINITY : m * AT_LN2 + logf(l);
+  for (int i = c + warp; i <= it.y; i += 4) {
+    const float2 ml = p.part_ml[at(i)];
+    const float f = ex2(ml.x - use);
+    const float* src = p.part_o + at(i) * p.dim;
+    l += ml.y * f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e * 32 + lane < p.dim) o[e] += src[e * 32 + lane] * f;
   }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) s_o[warp][e * 32 + lane] = o[e];
+  if (lane == 0) s_l[warp] = l;
+  __syncthreads();
+  l = s_l[0] + s_l[1] + s_l[2] + s_l[3];
+  for (int d = threadIdx.x; d < p.dim; d += 128) put<T>(p, -1, b, head0, r, d, s_o[0][d] + s_o[1][d] + s_o[2][d] + s_o[3][d], m, l);
 }
 
 // Where key j of sequence b lies: page name and place inside the page; false where there is no such page.
@@ -193,57 +232,40 @@ __device__ __forceinline__ float4 lds4(uint32_t a) {
   return f;
 }
 
+constexpr int FM_WARPS = 4;            // each walks every fourth tile of keys of the CTA's share on its own
+constexpr int FM_START = 8;
+constexpr int FM_CTAS = 2;             // per multiprocessor
+
 // fp32: products on the fp32 pipes (three tf32 products would be needed for as many bits): a lane owns four neighbouring dimensions in every 128 (NI groups), so a key row is one dense read
 // of the warp and q and the values stay in registers; R rows x 32 / R keys of partial dot products are summed over the lanes by
 // halving the rows and keys that a lane still holds (31 shuffles for 32 sums), after which lane = (row, key) holds one score.
 // Keys and values come through a ring of cp.async copies; a lane copies exactly the bytes that it reads back.
 template <int R, int NI, int STAGES>
-__global__ void __launch_bounds__(AT_WARPS * 32) attend_fma_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(FM_WARPS * 32) attend_fma_kernel(const AttnParams p) {
   constexpr int KB = 32 / R;                      // keys of a tile
   constexpr int CH = 16;                          // bytes of a lane's piece of a row
   constexpr int ROW = NI * 32 * CH;
   constexpr int SLOT = 2 * KB * ROW;              // keys, then values
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ int64_t s_red[AT_WARPS];
-  __shared__ float2 s_ml[AT_WARPS * R];
+  __shared__ int64_t s_red[FM_WARPS];
+  __shared__ float2 s_ml[FM_WARPS * R];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * (STAGES * SLOT) + lane * CH;
   float* s_o = reinterpret_cast<float*>(smem);
   pdl_trigger();
   pdl_wait();
 
-  Share s;
-  int64_t unit, unit_end;
-  int b;
-  int64_t base;
-  const int per = p.kv_heads * p.row_tiles;
+  Walk<KB, FM_START> walk;
   if (p.split) {
-    s = find_share<KB>(p, s_red);
-    if (tid == 0) p.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
-    unit = s.u0; unit_end = s.u1; b = s.b; base = s.base;
+    walk.begin_share(p, s_red, FM_WARPS * 32);
+    if (tid == 0) p.meta[blockIdx.x] = make_int2(-1, 0);
   } else {
-    b = blockIdx.x / per;
-    unit = 0; unit_end = 1; base = 0;              // one item, whatever its tiles
+    walk.begin_item(p, blockIdx.x);
   }
-  while (unit < unit_end) {
-    int first, end;
-    const int tiles = tiles_of<KB>(p, b, &first, &end);
-    int64_t next_base = base;
-    int next_b = b, sub, t0, t1;                   // (key head, row tile), first and last + 1 tile of this segment
-    if (p.split) {
-      const int cost = AT_START + tiles;
-      sub = (int)((unit - base) / cost);
-      const int at = (int)((unit - base) % cost);
-      const int upto = (int)min((int64_t)cost, at + (unit_end - unit));
-      t0 = max(at - AT_START, 0); t1 = upto - AT_START;
-      unit += upto - at;
-      if (unit == base + (int64_t)cost * per) { next_base = unit; next_b = b + 1; }
-      if (t1 <= 0) { base = next_base; b = next_b; continue; }    // the next CTA begins this item
-    } else {
-      sub = blockIdx.x % per;
-      t0 = 0; t1 = tiles;
-    }
-    const int h = sub / p.row_tiles, x = sub % p.row_tiles;
+  Segment s;
+  while (walk.next(p, &s)) {
+    const int b = s.b, first = s.first, end = s.end, t0 = s.t0, t1 = s.t1;
+    const int h = s.sub / p.row_tiles, x = s.sub - h * p.row_tiles;
     const int head0 = h * p.group + x * p.rows, rows = min(p.rows, p.group - x * p.rows);
     const int key0 = first / KB * KB;              // tiles start at multiples of KB
 
@@ -287,13 +309,13 @@ __global__ void __launch_bounds__(AT_WARPS * 32) attend_fma_kernel(const AttnPar
     };
     const int mine = t0 + warp;
 #pragma unroll
-    for (int st = 0; st < STAGES - 1; ++st) live_ring[st] = fetch(mine + st * AT_WARPS, st);
+    for (int st = 0; st < STAGES - 1; ++st) live_ring[st] = fetch(mine + st * FM_WARPS, st);
     int slot = 0;
-    for (int t = mine; t < t1; t += AT_WARPS) {
+    for (int t = mine; t < t1; t += FM_WARPS) {
       const uint32_t got = live_ring[0];
 #pragma unroll
       for (int st = 0; st + 2 < STAGES; ++st) live_ring[st] = live_ring[st + 1];
-      live_ring[STAGES - 2] = fetch(t + (STAGES - 1) * AT_WARPS, (slot + STAGES - 1) % STAGES);
+      live_ring[STAGES - 2] = fetch(t + (STAGES - 1) * FM_WARPS, (slot + STAGES - 1) % STAGES);
       cp_wait<STAGES - 1>();
       const uint32_t at = ring + slot * SLOT;
       slot = slot + 1 == STAGES ? 0 : slot + 1;
@@ -372,14 +394,23 @@ __global__ void __launch_bounds__(AT_WARPS * 32) attend_fma_kernel(const AttnPar
         if (d < p.dim) *reinterpret_cast<float4*>(s_o + (warp * R + r) * p.dim + d) = make_float4(o[r][i * 4], o[r][i * 4 + 1], o[r][i * 4 + 2], o[r][i * 4 + 3]);
       }
     __syncthreads();
-    const bool whole = t0 == 0 && t1 == tiles;
-    store_tile<float>(p, s_o, s_ml, b, head0, rows, R, whole ? -1 : 2 * (int)blockIdx.x + (t0 == 0));
-    if (!p.split) break;
-    if (!whole && t0 == 0 && tid == 0)
-      p.meta[blockIdx.x] = make_int4(b * per + sub, cta_of(s, base + (int64_t)(sub + 1) * (AT_START + tiles) - 1), 0, 0);
+    const int part = part_of(s);
+    for (int i = tid; i < rows * p.dim; i += FM_WARPS * 32) {
+      const int r = i / p.dim, d = i - r * p.dim;
+      float top = -INFINITY, sum = 0.f, val = 0.f;
+#pragma unroll
+      for (int w = 0; w < FM_WARPS; ++w) top = fmaxf(top, s_ml[w * R + r].x);
+      const float use = top == -INFINITY ? 0.f : top;
+#pragma unroll
+      for (int w = 0; w < FM_WARPS; ++w) {
+        const float fw = exp2f(s_ml[w * R + r].x - use);
+        sum += s_ml[w * R + r].y * fw;
+        val += s_o[(w * R + r) * p.dim + d] * fw;
+      }
+      put<float>(p, part, b, head0, r, d, val, top, sum);
+    }
+    if (s.last >= 0 && tid == 0) p.meta[blockIdx.x] = make_int2(b * p.kv_heads * p.row_tiles + s.sub, s.last);
     __syncthreads();
-    base = next_base;
-    b = next_b;
   }
 }
 
@@ -409,75 +440,157 @@ template <typename T> __device__ __forceinline__ void split_pair(float x, float 
   lo = bits_of<T>(from_f32<T>(x - to_f32<T>(a)), from_f32<T>(y - to_f32<T>(b)));
 }
 
-constexpr int MM_KEYS = 16;
-template <int DP> struct MmaShape {
-  static constexpr int ROW = ((DP / 8) | 1) * 16;                 // an odd number of 16-byte pieces: ldmatrix without bank conflicts
-  static constexpr int SLOT = 2 * MM_KEYS * ROW;                  // keys, then values
-  static constexpr int STAGES = DP == 64 ? 6 : 3;
-  static constexpr int CTAS = DP == 256 ? 1 : 2;                  // per multiprocessor
-  static constexpr int SMEM = AT_WARPS * STAGES * SLOT;
+constexpr int MM_COPIERS = 4;                                      // warps that fill the ring
+
+template <int DP, bool TWO> struct MmaShape {
+  static constexpr int R = TWO ? 16 : 8;                           // rows: query heads of a tile
+  static constexpr int NC = 4;                                     // warps that compute
+  static constexpr int THREADS = (NC + MM_COPIERS) * 32;
+  static constexpr int KEYS = DP == 256 ? 16 : 32;                 // of a tile
+  static constexpr int START = DP == 256 ? 4 : 3;
+  static constexpr int ROW = ((DP / 8) | 1) * 16;                  // an odd number of 16-byte pieces: ldmatrix without bank conflicts
+  static constexpr int SLOT = 2 * KEYS * ROW;                      // keys, then values
+  static constexpr int JROW = 40;                                  // floats of a row of 32 values in the join buffers: no bank conflicts
+  static constexpr int JOIN = 2 * NC * R * JROW * 4;
+  static constexpr int FIXED = JOIN + NC * R * 8 + R * 8 + 64 * 24 + 256;
+  // a multiple of the warps: each computing warp shares its slots with one copier, so that no barrier is ever a phase ahead of a waiter
+  static constexpr int SLOTS = (232448 - FIXED) / SLOT < 24 ? (232448 - FIXED) / SLOT / 4 * 4 : 24;
+  static constexpr int SMEM = SLOTS * SLOT + JOIN + NC * R * 8 + R * 8;
 };
 
-// m16n8k16 products: the query heads of a tile are the 16 rows, 16 cached keys a step.  Scores: A = q (registers), B = keys;
-// values: A = weights (the score accumulators are already in A's layout), B = values (transposed by ldmatrix).  The weights enter as
-// two 16-bit parts, so that they count with 16 bits and more; up to eight heads leave the upper eight rows free, and the low
-// parts ride there at no cost (TWO = false); above that they are a second product.
-template <typename T, int DP, bool TWO>
-__global__ void __launch_bounds__(AT_WARPS * 32, MmaShape<DP>::CTAS) attend_mma_kernel(const AttnParams p) {
-  using S = MmaShape<DP>;
-  constexpr int R = TWO ? 16 : 8;
-  constexpr int STAGES = S::STAGES;
-  constexpr int LPR = DP / 8;                                     // lanes of a row of the copies
-  constexpr int COPIES = MM_KEYS * LPR / 32;
-  extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ int64_t s_red[AT_WARPS];
-  __shared__ float2 s_ml[AT_WARPS * R];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
-  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * (STAGES * S::SLOT);
-  const uint32_t k_at = ring + ((lane >> 4) * 8 + (lane & 7)) * S::ROW + (lane >> 3 & 1) * 16;
-  const uint32_t v_at = ring + (MM_KEYS + (lane >> 3 & 1) * 8 + (lane & 7)) * S::ROW + (lane >> 4) * 16;
-  float* s_o = reinterpret_cast<float*>(smem);
-  const int nk = p.dim / 16;
-  const bool one_page = p.page_size % MM_KEYS == 0;               // tiles start at multiples of 16
-  pdl_trigger();
-  pdl_wait();
-
-  Share s;
-  int64_t unit, unit_end;
-  int b;
-  int64_t base;
-  const int per = p.kv_heads * p.row_tiles;
-  if (p.split) {
-    s = find_share<MM_KEYS>(p, s_red);
-    if (tid == 0) p.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
-    unit = s.u0; unit_end = s.u1; b = s.b; base = s.base;
-  } else {
-    b = blockIdx.x / per;
-    unit = 0; unit_end = 1; base = 0;
+// Waits for a barrier's phase; when that takes a second the whole CTA stops waiting, runs through its remaining steps (every access
+// stays where it would have been) and reports it.
+__device__ __forceinline__ void ring_wait(uint32_t bar, uint32_t parity, volatile int* gave_up) {
+  if (bar_try(bar, parity) || *gave_up) return;
+  const long long t0 = clock64();
+  while (!bar_try(bar, parity)) {
+    if (*gave_up) return;
+    if (clock64() - t0 > 2000000000ll) { *gave_up = 1; return; }
   }
-  while (unit < unit_end) {
-    int first, end;
-    const int tiles = tiles_of<MM_KEYS>(p, b, &first, &end);
-    int64_t next_base = base;
-    int next_b = b, sub, t0, t1;
-    if (p.split) {
-      const int cost = AT_START + tiles;
-      sub = (int)((unit - base) / cost);
-      const int at = (int)((unit - base) % cost);
-      const int upto = (int)min((int64_t)cost, at + (unit_end - unit));
-      t0 = max(at - AT_START, 0); t1 = upto - AT_START;
-      unit += upto - at;
-      if (unit == base + (int64_t)cost * per) { next_base = unit; next_b = b + 1; }
-      if (t1 <= 0) { base = next_base; b = next_b; continue; }    // the next CTA begins this item
-    } else {
-      sub = blockIdx.x % per;
-      t0 = 0; t1 = tiles;
-    }
-    const int h = sub / p.row_tiles, x = sub % p.row_tiles;
-    const int head0 = h * p.group + x * p.rows, rows = min(p.rows, p.group - x * p.rows);
-    const int key0 = first / MM_KEYS * MM_KEYS;
+}
 
-    uint32_t q[DP / 16][TWO ? 4 : 2];
+// 16-bit types: m16n8k16 products.  The query heads of a tile are the 16 rows, a step is 16 or 32 cached keys.  Scores: A = q (registers), B =
+// keys; values: A = weights (the score accumulators are already in A's layout), B = values (transposed by ldmatrix).  The weights
+// enter as two 16-bit parts, so that they count with 16 bits and more; up to eight heads leave the upper eight rows free, and the
+// low parts ride there at no cost (TWO = false); above that they are a second product.
+//
+// Four warps copy, the others compute.  The copiers walk the tiles of all segments of the CTA into one ring without a stop (cp.async,
+// whose arrival the slot's barrier counts), so the loads of the next segment are under way while this one's warps join; tile n goes to
+// computing warp n % NC, from copier n % NC.  The warps' results of a segment are added through shared memory, 32 columns at a time.
+template <typename T, int DP, bool TWO>
+__global__ void __launch_bounds__(MmaShape<DP, TWO>::THREADS, 1) attend_mma_kernel(const AttnParams p) {
+  using S = MmaShape<DP, TWO>;
+  constexpr int R = S::R, NC = S::NC, NS = S::SLOTS, KEYS = S::KEYS, NT = KEYS / 8;
+  static_assert(NS % NC == 0 && NC == MM_COPIERS, "private rings");
+  constexpr uint32_t ALL = KEYS == 32 ? 0xffffffffu : 0xffffu;
+  constexpr float LIFT = std::is_same<T, __half>::value ? 12.f : 0.f;   // weights up to 2^12: fp16's small numbers begin at 2^-24
+  extern __shared__ __align__(128) uint8_t tl_smem[];
+  float* s_join = reinterpret_cast<float*>(tl_smem + NS * S::SLOT);
+  float2* s_ml = reinterpret_cast<float2*>(tl_smem + NS * S::SLOT + S::JOIN);          // [NC][R] maximum and sum of a warp
+  float2* s_row = s_ml + NC * R;                                                        // [R] of the segment
+  __shared__ __align__(8) uint64_t s_full[NS], s_empty[NS];
+  __shared__ uint32_t s_live[NS];
+  __shared__ int64_t s_red[S::THREADS / 32];
+  __shared__ int s_gave_up;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t ring = s_u32(tl_smem), full = s_u32(s_full), empty = s_u32(s_empty);
+  const int nk = p.dim / 16;
+  pdl_trigger();
+  if (tid < NS) {
+    bar_init(full + tid * 8, 33);        // the copies of 32 lanes, and the word of live keys
+    bar_init(empty + tid * 8, 1);
+  }
+  if (tid == 0) s_gave_up = 0;
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  pdl_wait();
+  Walk<KEYS, S::START> walk;
+  if (p.split) {
+    walk.begin_share(p, s_red, S::THREADS);
+    if (tid == 0) p.meta[blockIdx.x] = make_int2(-1, 0);
+  } else {
+    walk.begin_item(p, blockIdx.x);
+  }
+  __syncthreads();
+  Segment s;
+
+  if (warp >= NC) {
+    // ------------------------------------------------------------ copiers
+    constexpr int LPR = DP / 8;                                   // lanes of a row
+    constexpr int STEP = 32 / LPR;                                // rows of an instruction
+    const int piece = lane % LPR;
+    const bool in_dim = piece * 8 < p.dim;
+    const bool one_page = p.page_size % 16 == 0;                  // 16 keys from a multiple of 16 on lie in one page
+    int n = warp - NC, n0 = 0;                                    // this warp's next tile; tiles before the segment
+    int slot = n, use = 0;                                        // n % NS, n / NS
+    while (walk.next(p, &s)) {
+      const int h = s.sub / p.row_tiles;
+      const T* k_lane = static_cast<const T*>(p.k) + ((int64_t)h * p.k_head + (lane / LPR) * p.k_slot + piece * 8);
+      const T* v_lane = static_cast<const T*>(p.v) + ((int64_t)h * p.v_head + (lane / LPR) * p.v_slot + piece * 8);
+      const int key0 = s.first / KEYS * KEYS + lane, count = s.t1 - s.t0;
+      int page = 0, place = 0;
+      bool ok = n - n0 < count && lane < KEYS && find_key(p, s.b, key0 + (s.t0 + n - n0) * KEYS, s.first, s.end, &page, &place);
+      for (; n - n0 < count; n += MM_COPIERS) {
+        const uint32_t live = __ballot_sync(0xffffffffu, ok);
+        if (use > 0) ring_wait(empty + slot * 8, (use - 1) & 1, &s_gave_up);
+        const int page_now = page, place_now = place;
+        ok = n + MM_COPIERS - n0 < count && lane < KEYS && find_key(p, s.b, key0 + (s.t0 + n + MM_COPIERS - n0) * KEYS, s.first, s.end, &page, &place);
+#pragma unroll
+        for (int half = 0; half < KEYS / 16; ++half) {
+          const uint32_t dst = ring + slot * S::SLOT + (half * 16 + lane / LPR) * S::ROW + piece * 16;
+          if (one_page && (live >> (half * 16) & 0xffffu) == 0xffffu) {   // one address and a fixed step
+            const int64_t pg = __shfl_sync(0xffffffffu, page_now, half * 16), pl = __shfl_sync(0xffffffffu, place_now, half * 16);
+            const T* kp = k_lane + (pg * p.k_page + pl * p.k_slot);
+            const T* vp = v_lane + (pg * p.v_page + pl * p.v_slot);
+            if (in_dim) {
+#pragma unroll
+              for (int i = 0; i < 16 / STEP; ++i) {
+                cp_async(dst + i * STEP * S::ROW, kp, true);
+                kp += STEP * p.k_slot;
+              }
+#pragma unroll
+              for (int i = 0; i < 16 / STEP; ++i) {
+                cp_async(dst + (KEYS + i * STEP) * S::ROW, vp, true);
+                vp += STEP * p.v_slot;
+              }
+            }
+          } else {
+#pragma unroll 4
+            for (int i = 0; i < 16 / STEP; ++i) {
+              const int row = half * 16 + i * STEP + lane / LPR;
+              const int64_t pg = __shfl_sync(0xffffffffu, page_now, row), pl = __shfl_sync(0xffffffffu, place_now, row) - lane / LPR;
+              const bool on = live >> row & 1;
+              if (in_dim) {                                       // rows that are not live are filled with zeros
+                cp_async(dst + i * STEP * S::ROW, on ? k_lane + (pg * p.k_page + pl * p.k_slot) : k_lane, on);
+                cp_async(dst + (KEYS + i * STEP) * S::ROW, on ? v_lane + (pg * p.v_page + pl * p.v_slot) : v_lane, on);
+              }
+            }
+          }
+        }
+        if (lane == 0) {
+          s_live[slot] = live;
+          bar_arrive(full + slot * 8);
+        }
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(full + slot * 8) : "memory");
+        slot += MM_COPIERS;
+        if (slot >= NS) { slot -= NS; ++use; }
+      }
+      n0 += count;
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (lane == 0 && *(volatile int*)&s_gave_up) atomicExch(&g_attend_status, 1);
+    return;
+  }
+
+  // -------------------------------------------------------------- computing warps
+  const int g = lane >> 2, t4 = lane & 3;
+  const uint32_t k_at = ring + ((lane >> 4) * 8 + (lane & 7)) * S::ROW + (lane >> 3 & 1) * 16;
+  const uint32_t v_at = ring + (KEYS + (lane >> 3 & 1) * 8 + (lane & 7)) * S::ROW + (lane >> 4) * 16;
+  uint32_t q[DP / 16][TWO ? 4 : 2];
+  int n0 = 0, n = warp, slot = warp % NS, use = warp / NS;
+  bool more = walk.next(p, &s);
+  auto load_q = [&]() {
+    const int h = s.sub / p.row_tiles, x = s.sub - h * p.row_tiles;
+    const int head0 = h * p.group + x * p.rows, rows = min(p.rows, p.group - x * p.rows);
 #pragma unroll
     for (int ks = 0; ks < DP / 16; ++ks)
 #pragma unroll
@@ -485,111 +598,70 @@ __global__ void __launch_bounds__(AT_WARPS * 32, MmaShape<DP>::CTAS) attend_mma_
         const int r = TWO ? g + (i & 1) * 8 : g, d = ks * 16 + t4 * 2 + (TWO ? i >> 1 : i) * 8;
         q[ks][i] = 0;
         if (r < rows && ks < nk) {
-          const T* src = reinterpret_cast<const T*>(p.q) + (int64_t)b * p.q_b + (int64_t)(head0 + r) * p.q_h + d;
+          const T* src = static_cast<const T*>(p.q) + ((int64_t)s.b * p.q_b + (int64_t)(head0 + r) * p.q_h + d);
           q[ks][i] = bits_of<T>(src[0], src[1]);
         }
       }
+  };
+  if (more) load_q();
+  while (more) {
+    const Segment now = s;
+    const int count = now.t1 - now.t0;
     float o[DP / 8][4];
 #pragma unroll
     for (int i = 0; i < DP / 8; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};       // rows g and g + 8; l: of the lane's own keys
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};       // rows g and g + 8, m less LIFT; l: of the lane's own keys
 
-    // the page of the lane's key is looked up a tile before the copies that need it; k_lane, v_lane: the lane's piece of its first
-    // row, in the first page
-    int page32 = 0, place = 0;
-    int64_t page = 0, place0 = 0;                                 // place0: of the tile's first key, seen from the lane's
-    bool ok = false;
-    auto look = [&](int t) {
-      ok = t < t1 && find_key(p, b, key0 + t * MM_KEYS + (lane & 15), first, end, &page32, &place);
-      page = page32;
-      place0 = place - (lane & 15);
-    };
-    const int piece = lane % LPR;
-    const T* k_lane = static_cast<const T*>(p.k) + ((int64_t)h * p.k_head + (lane / LPR) * p.k_slot + piece * 8);
-    const T* v_lane = static_cast<const T*>(p.v) + ((int64_t)h * p.v_head + (lane / LPR) * p.v_slot + piece * 8);
-    auto fetch = [&](int slot) -> uint32_t {
-      const uint32_t live = __ballot_sync(0xffffffffu, ok) & 0xffffu;
-      const uint32_t dst = ring + slot * S::SLOT + (lane / LPR) * S::ROW + piece * 16;
-      if (live == 0xffffu && one_page) {                          // 16 tokens of one page: one address and a fixed step
-        if (piece * 8 < p.dim) {
-          const T* kp = k_lane + (page * p.k_page + place0 * p.k_slot);
-          const T* vp = v_lane + (page * p.v_page + place0 * p.v_slot);
-#pragma unroll
-          for (int i = 0; i < COPIES; ++i) {
-            cp_async(dst + i * (32 / LPR) * S::ROW, kp, true);
-            cp_async(dst + (MM_KEYS + i * (32 / LPR)) * S::ROW, vp, true);
-            kp += (32 / LPR) * p.k_slot;
-            vp += (32 / LPR) * p.v_slot;
-          }
-        }
-      } else {
-#pragma unroll 1
-        for (int i = 0; i < COPIES; ++i) {
-          const int row = i * (32 / LPR) + lane / LPR;
-          const int64_t pg = __shfl_sync(0xffffffffu, page, row), pl = __shfl_sync(0xffffffffu, place0 + (lane & 15), row) - lane / LPR;
-          const bool on = live >> row & 1;
-          if (piece * 8 < p.dim) {                                // rows that are not live are filled with zeros
-            cp_async(dst + i * (32 / LPR) * S::ROW, on ? k_lane + (pg * p.k_page + pl * p.k_slot) : k_lane, on);
-            cp_async(dst + (MM_KEYS + i * (32 / LPR)) * S::ROW, on ? v_lane + (pg * p.v_page + pl * p.v_slot) : v_lane, on);
-          }
-        }
-      }
-      cp_commit();
-      return live;
-    };
-    const int mine = t0 + warp;
-    uint32_t live_ring[STAGES - 1];
-#pragma unroll
-    for (int st = 0; st < STAGES - 1; ++st) {
-      look(mine + st * AT_WARPS);
-      live_ring[st] = fetch(st);
-    }
-    look(mine + (STAGES - 1) * AT_WARPS);
-    int slot = 0;
-    for (int t = mine; t < t1; t += AT_WARPS) {
-      const uint32_t live = live_ring[0];
-#pragma unroll
-      for (int st = 0; st + 2 < STAGES; ++st) live_ring[st] = live_ring[st + 1];
-      __syncwarp();                                               // every lane has read the slot that is filled next
-      live_ring[STAGES - 2] = fetch(slot == 0 ? STAGES - 1 : slot - 1);
-      look(t + STAGES * AT_WARPS);
-      cp_wait<STAGES - 1>();
-      __syncwarp();
+    for (; n - n0 < count; n += NC) {
+      ring_wait(full + slot * 8, use & 1, &s_gave_up);
+      const uint32_t live = s_live[slot];
       const uint32_t off = slot * S::SLOT;
-      slot = slot + 1 == STAGES ? 0 : slot + 1;
-
-      float c[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      float c[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c[nt][e] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < DP / 16; ++ks) {
         if (ks < nk) {
-          uint32_t kb[4];
-          ldsm4(kb, k_at + off + ks * 32);
+          uint32_t kb[KEYS / 16][4];
 #pragma unroll
-          for (int nt = 0; nt < 2; ++nt) {
-            if constexpr (TWO) mma16816<T>(c[nt], q[ks][0], q[ks][1], q[ks][2], q[ks][3], kb[2 * nt], kb[2 * nt + 1]);
-            else mma16816<T>(c[nt], q[ks][0], 0u, q[ks][1], 0u, kb[2 * nt], kb[2 * nt + 1]);
+          for (int j = 0; j < KEYS / 16; ++j) ldsm4(kb[j], k_at + off + ks * 32 + j * 16 * S::ROW);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const uint32_t b0 = kb[nt >> 1][2 * (nt & 1)], b1 = kb[nt >> 1][2 * (nt & 1) + 1];
+            if constexpr (TWO) mma16816<T>(c[nt], q[ks][0], q[ks][1], q[ks][2], q[ks][3], b0, b1);
+            else mma16816<T>(c[nt], q[ks][0], 0u, q[ks][1], 0u, b0, b1);
           }
         }
       }
-      uint32_t hi[4], lo[4];                                      // weights: [key tile][row half]
+      uint32_t hi[KEYS / 16][4], lo[KEYS / 16][4];                              // weights as A: [16 keys][register]
 #pragma unroll
       for (int half = 0; half < (TWO ? 2 : 1); ++half) {
-        float sc[4];
+        float sc[2 * NT];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float v = c[i >> 1][half * 2 + (i & 1)] * p.scale;
-          if (p.cap > 0.f) v = p.cap * AT_LOG2E * tanhf(v / p.cap);
-          sc[i] = live >> ((i >> 1) * 8 + t4 * 2 + (i & 1)) & 1 ? v : -INFINITY;
+        for (int i = 0; i < 2 * NT; ++i) {
+          sc[i] = c[i >> 1][half * 2 + (i & 1)] * p.scale;
+          if (p.cap > 0.f) sc[i] = p.cap * AT_LOG2E * tanhf(sc[i] / p.cap);
         }
-        float top = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
+        if (live != ALL) {
+#pragma unroll
+          for (int i = 0; i < 2 * NT; ++i)
+            if (!(live >> ((i >> 1) * 8 + t4 * 2 + (i & 1)) & 1)) sc[i] = -INFINITY;
+        }
+        float tops[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) tops[nt] = fmaxf(sc[2 * nt], sc[2 * nt + 1]);
+        float top = fmaxf(tops[0], tops[1]);
+        if constexpr (NT == 4) top = fmaxf(top, fmaxf(tops[2], tops[3]));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const float mn = fmaxf(m[half], top);
-        const float use = mn == -INFINITY ? 0.f : mn;
+        const float mn = fmaxf(m[half], top - LIFT);
+        const float base = mn == -INFINITY ? 0.f : mn;
         if (__any_sync(0xffffffffu, mn > m[half])) {              // a new maximum in some row: rescale what is there
-          const float f = exp2f(m[half] - use);
+          const float f = ex2(m[half] - base);
           l[half] *= f;
 #pragma unroll
           for (int i = 0; i < DP / 8; ++i) {
@@ -599,60 +671,100 @@ __global__ void __launch_bounds__(AT_WARPS * 32, MmaShape<DP>::CTAS) attend_mma_
         }
         m[half] = mn;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { sc[i] = exp2f(sc[i] - use); l[half] += sc[i]; }
+        for (int i = 0; i < 2 * NT; ++i) sc[i] = ex2(sc[i] - base);
+        l[half] += (sc[0] + sc[1]) + (sc[2] + sc[3]);
+        if constexpr (NT == 4) l[half] += (sc[4] + sc[5]) + (sc[6] + sc[7]);
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt) split_pair<T>(sc[2 * nt], sc[2 * nt + 1], hi[2 * nt + half], lo[2 * nt + half]);
+        for (int nt = 0; nt < NT; ++nt) split_pair<T>(sc[2 * nt], sc[2 * nt + 1], hi[nt >> 1][2 * (nt & 1) + half], lo[nt >> 1][2 * (nt & 1) + half]);
       }
 #pragma unroll
       for (int cc = 0; cc < DP / 16; ++cc) {
         if (cc < nk) {
-          uint32_t vb[4];
-          ldsm4_t(vb, v_at + off + cc * 32);
 #pragma unroll
-          for (int n2 = 0; n2 < 2; ++n2) {
-            if constexpr (TWO) {
-              mma16816<T>(o[2 * cc + n2], hi[0], hi[1], hi[2], hi[3], vb[2 * n2], vb[2 * n2 + 1]);
-              mma16816<T>(o[2 * cc + n2], lo[0], lo[1], lo[2], lo[3], vb[2 * n2], vb[2 * n2 + 1]);
-            } else {
-              mma16816<T>(o[2 * cc + n2], hi[0], lo[0], hi[2], lo[2], vb[2 * n2], vb[2 * n2 + 1]);
+          for (int j = 0; j < KEYS / 16; ++j) {
+            uint32_t vb[4];
+            ldsm4_t(vb, v_at + off + cc * 32 + j * 16 * S::ROW);
+#pragma unroll
+            for (int n2 = 0; n2 < 2; ++n2) {
+              if constexpr (TWO) {
+                mma16816<T>(o[2 * cc + n2], hi[j][0], hi[j][1], hi[j][2], hi[j][3], vb[2 * n2], vb[2 * n2 + 1]);
+                mma16816<T>(o[2 * cc + n2], lo[j][0], lo[j][1], lo[j][2], lo[j][3], vb[2 * n2], vb[2 * n2 + 1]);
+              } else {
+                mma16816<T>(o[2 * cc + n2], hi[j][0], lo[j][0], hi[j][2], lo[j][2], vb[2 * n2], vb[2 * n2 + 1]);
+              }
             }
           }
         }
       }
+      __syncwarp();
+      if (lane == 0) bar_arrive(empty + slot * 8);
+      slot += NC;
+      if (slot >= NS) { slot -= NS; ++use; }
     }
-    cp_wait<0>();
-    __syncthreads();                                              // the ring becomes the place where the warps' results meet
+    n0 += count;
+    more = walk.next(p, &s);
+    if (more) load_q();                                           // arrives while the warps join
+
 #pragma unroll
     for (int half = 0; half < (TWO ? 2 : 1); ++half) {
       l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
       l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
-      const int r = g + half * 8;
-      if (t4 == 0) s_ml[warp * R + r] = make_float2(m[half], l[half]);
+      if (t4 == 0) s_ml[warp * R + g + half * 8] = make_float2(m[half], l[half]);
+    }
+    auto meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(NC * 32) : "memory"); };
+    meet();
+    float f[2] = {0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < DP / 8; ++i) {
-        if (i < 2 * nk) {
-          const float a = TWO ? o[i][2 * half] : o[i][0] + o[i][2], e = TWO ? o[i][2 * half + 1] : o[i][1] + o[i][3];
-          *reinterpret_cast<float2*>(s_o + (warp * R + r) * p.dim + i * 8 + t4 * 2) = make_float2(a, e);
+    for (int half = 0; half < (TWO ? 2 : 1); ++half) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < NC; ++w) top = fmaxf(top, s_ml[w * R + g + half * 8].x);
+      f[half] = ex2(m[half] - (top == -INFINITY ? 0.f : top));
+    }
+    if (tid < R) {
+      float top = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < NC; ++w) top = fmaxf(top, s_ml[w * R + tid].x);
+#pragma unroll
+      for (int w = 0; w < NC; ++w) sum += s_ml[w * R + tid].y * ex2(s_ml[w * R + tid].x - (top == -INFINITY ? 0.f : top));
+      s_row[tid] = make_float2(top, sum);
+    }
+    const int h = now.sub / p.row_tiles, x = now.sub - h * p.row_tiles;
+    const int head0 = h * p.group + x * p.rows, rows = min(p.rows, p.group - x * p.rows);
+    const int part = part_of(now);
+#pragma unroll
+    for (int sl = 0; sl < DP / 32; ++sl) {
+      if (sl * 32 < p.dim) {
+        float* buf = s_join + (sl & 1) * (NC * R * S::JROW);
+#pragma unroll
+        for (int half = 0; half < (TWO ? 2 : 1); ++half)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int nt = sl * 4 + i;
+            const float a = TWO ? o[nt][2 * half] : o[nt][0] + o[nt][2], e = TWO ? o[nt][2 * half + 1] : o[nt][1] + o[nt][3];
+            *reinterpret_cast<float2*>(buf + (warp * R + g + half * 8) * S::JROW + i * 8 + t4 * 2) = make_float2(a * f[half], e * f[half]);
+          }
+        meet();
+#pragma unroll
+        for (int e = 0; e < R / NC; ++e) {
+          const int r = e * NC + warp, d = sl * 32 + lane;
+          float sum = 0.f;
+#pragma unroll
+          for (int w = 0; w < NC; ++w) sum += buf[(w * R + r) * S::JROW + lane];
+          const float2 ml = s_row[r];
+          if (r < rows && d < p.dim) put<T>(p, part, now.b, head0, r, d, sum, ml.x, ml.y);
         }
       }
     }
-    __syncthreads();
-    const bool whole = t0 == 0 && t1 == tiles;
-    store_tile<T>(p, s_o, s_ml, b, head0, rows, R, whole ? -1 : 2 * (int)blockIdx.x + (t0 == 0));
-    if (!p.split) break;
-    if (!whole && t0 == 0 && tid == 0)
-      p.meta[blockIdx.x] = make_int4(b * per + sub, cta_of(s, base + (int64_t)(sub + 1) * (AT_START + tiles) - 1), 0, 0);
-    __syncthreads();
-    base = next_base;
-    b = next_b;
+    if (now.last >= 0 && tid == 0) p.meta[blockIdx.x] = make_int2(now.b * p.kv_heads * p.row_tiles + now.sub, now.last);
   }
 }
 
 template <typename T>
-int launch_both(void (*kern)(const AttnParams), AttnParams& p, int smem, int ctas_per_sm, cudaStream_t st) {
+int launch_both(void (*kern)(const AttnParams), AttnParams& p, int threads, int smem, int ctas_per_sm, cudaStream_t st) {
   const bool pdl = options().pdl != 0;
   const unsigned grid = p.split ? (unsigned)(sm_count() * ctas_per_sm) : (unsigned)((int64_t)p.batch * p.kv_heads * p.row_tiles);
-  KQ_CUDA_TRY(launch_pdl(kern, dim3(grid), dim3(AT_WARPS * 32), (size_t)smem, st, pdl, p));
+  KQ_CUDA_TRY(launch_pdl(kern, dim3(grid), dim3(threads), (size_t)smem, st, pdl, p));
   options().launches += 1;
   if (p.split) {
     KQ_CUDA_TRY(launch_pdl(attend_join_kernel<T>, dim3(grid, (unsigned)p.rows), dim3(128), (size_t)0, st, pdl, p));
@@ -664,7 +776,7 @@ int launch_both(void (*kern)(const AttnParams), AttnParams& p, int smem, int cta
 template <int R, int NI>
 int run_fma(AttnParams& p, cudaStream_t st) {
   constexpr int STAGES = R == 8 ? 3 : 2;
-  constexpr int ring = AT_WARPS * STAGES * 2 * (32 / R) * NI * 512, join = AT_WARPS * R * NI * 128 * 4;
+  constexpr int ring = FM_WARPS * STAGES * 2 * (32 / R) * NI * 512, join = FM_WARPS * R * NI * 128 * 4;
   constexpr int smem = ring > join ? ring : join;
   auto kern = attend_fma_kernel<R, NI, STAGES>;
   static DeviceOnce attr_set;
@@ -672,21 +784,19 @@ int run_fma(AttnParams& p, cudaStream_t st) {
     KQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     attr_set.done();
   }
-  return launch_both<float>(kern, p, smem, AT_MAX_CTAS, st);
+  return launch_both<float>(kern, p, FM_WARPS * 32, smem, FM_CTAS, st);
 }
 
 template <typename T, int DP, bool TWO>
 int run_mma(AttnParams& p, cudaStream_t st) {
-  using S = MmaShape<DP>;
-  constexpr int join = AT_WARPS * (TWO ? 16 : 8) * DP * 4;
-  constexpr int smem = S::SMEM > join ? S::SMEM : join;
+  using S = MmaShape<DP, TWO>;
   auto kern = attend_mma_kernel<T, DP, TWO>;
   static DeviceOnce attr_set;
   if (attr_set.first_time()) {
-    KQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    KQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
     attr_set.done();
   }
-  return launch_both<T>(kern, p, smem, S::CTAS, st);
+  return launch_both<T>(kern, p, S::THREADS, S::SMEM, 1, st);
 }
 
 // the query heads of a key head in tiles of at most `most` rows, of even sizes
@@ -709,7 +819,7 @@ int run_16bit(AttnParams& p, cudaStream_t st) {
   return p.dim > 128 ? run_mma<T, 256, true>(p, st) : p.dim > 64 ? run_mma<T, 128, true>(p, st) : run_mma<T, 64, true>(p, st);
 }
 
-constexpr int AT_MAX_ROWS = 16;
+constexpr int AT_MAX_ROWS = 16;         // rows of a partial result at most
 
 struct Scratch { size_t o, ml, meta, total; };
 Scratch scratch_of(int64_t ctas, int64_t dim) {
@@ -717,7 +827,7 @@ Scratch scratch_of(int64_t ctas, int64_t dim) {
   s.o = 0;
   s.ml = s.o + (size_t)(2 * ctas * AT_MAX_ROWS * dim * 4 + 255) / 256 * 256;
   s.meta = s.ml + (size_t)(2 * ctas * AT_MAX_ROWS * 8 + 255) / 256 * 256;
-  s.total = s.meta + (size_t)(ctas * 16 + 255) / 256 * 256;
+  s.total = s.meta + (size_t)(ctas * 8 + 255) / 256 * 256;
   return s;
 }
 
@@ -731,7 +841,7 @@ extern "C" {
 
 size_t kq_paged_attention_workspace_bytes(int64_t head_dim) {
   if (head_dim <= 0 || head_dim > 256) return 0;
-  return scratch_of((int64_t)sm_count() * AT_MAX_CTAS, head_dim).total;
+  return scratch_of((int64_t)sm_count() * FM_CTAS, head_dim).total;
 }
 
 int kq_paged_attention(const void* q, int dtype, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t q_stride_batch,
@@ -766,7 +876,7 @@ int kq_paged_attention(const void* q, int dtype, int64_t batch, int64_t heads, i
       return KQ_EINVAL;
     }
   if ((uintptr_t)k_cache % 16 || (uintptr_t)v_cache % 16 || (uintptr_t)q % size || (uintptr_t)out % 16) { set_error("%s: misaligned pointer", fn); return KQ_EINVAL; }
-  const int64_t ctas = (int64_t)sm_count() * AT_MAX_CTAS;
+  const int64_t ctas = (int64_t)sm_count() * FM_CTAS;
   const Scratch L = scratch_of(ctas, head_dim);
   if (!scratch || (uintptr_t)scratch % 256) { set_error("%s: scratch must be non-null and 256-byte aligned", fn); return KQ_ESCRATCH; }
   if (scratch_bytes < L.total) { set_error("%s: scratch too small (%zu < %zu)", fn, scratch_bytes, L.total); return KQ_ESCRATCH; }
@@ -781,7 +891,7 @@ int kq_paged_attention(const void* q, int dtype, int64_t batch, int64_t heads, i
   p.scale = softcap > 0.f ? scale : scale * AT_LOG2E; p.cap = softcap; p.window = (int)window;
   p.out = out; p.lse = lse;
   uint8_t* sb = (uint8_t*)scratch;
-  p.part_o = (float*)(sb + L.o); p.part_ml = (float2*)(sb + L.ml); p.meta = (int4*)(sb + L.meta);
+  p.part_o = (float*)(sb + L.o); p.part_ml = (float2*)(sb + L.ml); p.meta = (int2*)(sb + L.meta);
   int64_t most = table_width * page_size;          // keys that a sequence can show
   if (window > 0 && window < most) most = window;
   p.split = most > 256;      // short sequences: one launch, one CTA per item
@@ -791,6 +901,16 @@ int kq_paged_attention(const void* q, int dtype, int64_t batch, int64_t heads, i
     case KQ_F16: return run_16bit<__half>(p, st);
     default: return run_16bit<__nv_bfloat16>(p, st);
   }
+}
+
+int kq_paged_attention_status(int* status, int clear) {
+  set_error("%s", "");
+  KQ_CUDA_TRY(cudaDeviceSynchronize());   // the copy does not wait for non-blocking streams
+  int v = 0;
+  KQ_CUDA_TRY(cudaMemcpyFromSymbol(&v, g_attend_status, sizeof(int)));
+  if (status) *status = v;
+  if (clear && v) { const int z = 0; KQ_CUDA_TRY(cudaMemcpyToSymbol(g_attend_status, &z, sizeof(int))); }
+  return KQ_OK;
 }
 
 }  // extern "C"

@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from kaillm_b200 import attention
+from kaillm_b200 import attention, capi
 from tests.attention_util import DT, attend, check_attention, paged_cache
 from tests.gpu_util import dev
 
@@ -171,6 +171,11 @@ def test_side_stream():
         got = attention.paged_attention(late, k, v, table, n)
     torch.cuda.current_stream().wait_stream(s)
     assert torch.equal(got, want)
+
+
+def test_no_wait_has_run_out():
+    run([5000, 0, 77], 8, 2, 128, 16, "bf16")
+    assert capi.paged_attention_status() == 0
 
 
 def test_refusals():
