@@ -28,7 +28,7 @@ constexpr float AT_LN2 = 0.6931471805599453f;
 __device__ int g_attend_status = 0;
 
 struct AttnParams {
-  const void* q; int64_t q_b, q_h;                     // strides in elements; the head dimension is dense everywhere
+  const void* q; int64_t q_b, q_h; int q_words;        // strides in elements; the head dimension is dense everywhere; q_words: pairs are aligned
   const void* k; int64_t k_page, k_slot, k_head;
   const void* v; int64_t v_page, v_slot, v_head;
   const int32_t* table; int64_t table_b; int width;    // page names [batch][width]
@@ -66,68 +66,81 @@ struct Segment {
 // it the CTAs that get the short sequences of a mixed batch end last).
 template <int TK, int START>
 struct Walk {
-  int64_t left, pos, total;       // units left, unit index, units of all items
+  int64_t left, pos;              // units left, unit index
+  int64_t share, more;            // of `ctas` CTAs the first `more` have share + 1 units, the others `share`
   int ctas;
   int b, sub, at, first, end, tiles;
+  int first2, end2, tiles2;       // of the next sequence, loaded ahead
 
-  __device__ void load(const AttnParams& p) { if (b < p.batch) tiles = tiles_of<TK>(p, b, &first, &end); }
+  __device__ void load(const AttnParams& p) { tiles2 = b + 1 < p.batch ? tiles_of<TK>(p, b + 1, &first2, &end2) : 0; }
 
   __device__ void begin_item(const AttnParams& p, int item) {
     const int per = p.kv_heads * p.row_tiles;
-    b = item / per; sub = item - b * per; at = START; left = 0x7fffffff; pos = 0; total = 1; ctas = 1;
-    load(p);
-    left = tiles;
+    b = item / per; sub = item - b * per; at = START;
+    tiles = tiles2 = tiles_of<TK>(p, b, &first, &end);
+    first2 = first; end2 = end;
+    pos = 0; share = left = tiles; more = 0; ctas = 1;
+  }
+
+  __device__ int64_t begin_of(int c) const { return share * c + min((int64_t)c, more); }
+  __device__ int cta_of(int64_t unit) const {     // the CTA whose share holds `unit`
+    return (int)(unit < more * (share + 1) ? div(unit, share + 1) : more + div(unit - more * (share + 1), share));
+  }
+  static __device__ int64_t div(int64_t x, int64_t y) {
+    return (x | y) >> 32 ? x / y : (int64_t)((uint32_t)x / (uint32_t)y);
   }
 
   // called by `threads` threads at once; s_red: one int64 per warp
   __device__ void begin_share(const AttnParams& p, int64_t* s_red, int threads) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int per = p.kv_heads * p.row_tiles;
-    int64_t sum = 0;
     int f, e;
-    for (int i = tid; i < p.batch; i += threads) sum += START + tiles_of<TK>(p, i, &f, &e);
+    int64_t total = 0;
+    if (p.batch > 32) {
+      for (int i = tid; i < p.batch; i += threads) total += START + tiles_of<TK>(p, i, &f, &e);
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    if (lane == 0) s_red[warp] = sum;
-    __syncthreads();
-    total = 0;
-    for (int w = 0; w < threads / 32; ++w) total += s_red[w];
-    total *= per;
-    // a share that is hardly more than a beginning would only add partial results
-    ctas = (int)min((int64_t)gridDim.x, (total + START + 3) / (START + 4));
-    pos = total * blockIdx.x / ctas;
-    left = total * (blockIdx.x + 1) / ctas - pos;
-    b = sub = at = 0;
-    if ((int)blockIdx.x >= ctas) { left = 0; return; }
-    // every warp scans the sequences 32 at a time until it reaches the one that holds `pos`
+      for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+      if (lane == 0) s_red[warp] = total;
+      __syncthreads();
+      total = 0;
+      for (int w = 0; w < threads / 32; ++w) total += s_red[w];
+    }
+    // every warp scans the sequences 32 at a time until it reaches the one that holds `pos` (up to 32: the scan is the sum as well)
     int64_t run = 0;
     for (int b0 = 0; b0 < p.batch; b0 += 32) {
-      int64_t v = b0 + lane < p.batch ? (int64_t)(START + tiles_of<TK>(p, b0 + lane, &f, &e)) * per : 0;
+      int64_t v = b0 + lane < p.batch ? START + tiles_of<TK>(p, b0 + lane, &f, &e) : 0;
       const int64_t own = v;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
         const int64_t u = __shfl_up_sync(0xffffffffu, v, d);
         if (lane >= d) v += u;
       }
-      const unsigned past = __ballot_sync(0xffffffffu, run + v > pos);
+      const int64_t sum = __shfl_sync(0xffffffffu, v, 31);
+      if (b0 == 0) {
+        if (p.batch <= 32) total = sum;
+        total *= per;
+        // a share that is hardly more than a beginning would only add partial results
+        ctas = (int)min((int64_t)gridDim.x, div(total + START, START + 2) + 1);
+        share = div(total, ctas);
+        more = total - share * ctas;
+        pos = begin_of(blockIdx.x);
+        left = begin_of(blockIdx.x + 1) - pos;
+        b = sub = at = 0;
+        if ((int)blockIdx.x >= ctas) { left = 0; return; }
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, (run + v) * per > pos);
       if (past) {
         const int i = __ffs(past) - 1;
         b = b0 + i;
-        const int64_t in = pos - run - __shfl_sync(0xffffffffu, v - own, i);
+        const int64_t in = pos - (run + __shfl_sync(0xffffffffu, v - own, i)) * per;
+        tiles = tiles_of<TK>(p, b, &first, &end);
         load(p);
-        sub = (int)(in / (START + tiles));
+        sub = (int)div(in, START + tiles);
         at = (int)(in - (int64_t)sub * (START + tiles));
         break;
       }
-      run += __shfl_sync(0xffffffffu, v, 31);
+      run += sum;
     }
-  }
-
-  __device__ int cta_of(int64_t unit) const {     // the CTA whose share holds `unit`
-    int c = (int)(unit * ctas / total);
-    while (c + 1 < ctas && total * (c + 1) / ctas <= unit) ++c;
-    while (c > 0 && total * c / ctas > unit) --c;
-    return c;
   }
 
   __device__ bool next(const AttnParams& p, Segment* s) {
@@ -140,7 +153,11 @@ struct Walk {
       left -= take; pos += take; at += take;
       if (at == cost) {
         at = 0;
-        if (++sub == p.kv_heads * p.row_tiles) { sub = 0; ++b; load(p); }
+        if (++sub == p.kv_heads * p.row_tiles) {
+          sub = 0; ++b;
+          first = first2; end = end2; tiles = tiles2;
+          load(p);
+        }
       }
       if (s->t1 > 0) return true;                 // otherwise the next CTA begins this item
     }
@@ -165,17 +182,24 @@ __device__ __forceinline__ float ex2(float x) {      // 2^x, relative error 2^-2
   return y;
 }
 
-// One value of a finished row, or of a partial one: o relative to 2^m, l the row's sum.
-template <typename T>
-__device__ __forceinline__ void put(const AttnParams& p, int part, int b, int head0, int r, int d, float o, float m, float l) {
-  if (part < 0) {
-    static_cast<T*>(p.out)[((int64_t)b * p.heads + head0 + r) * p.dim + d] = from_f32<T>(l == 0.f ? 0.f : o / l);
-    if (d == 0 && p.lse) p.lse[(int64_t)b * p.heads + head0 + r] = l == 0.f ? -INFINITY : m * AT_LN2 + logf(l);
-  } else {
-    p.part_o[((int64_t)part * p.rows + r) * p.dim + d] = o;
-    if (d == 0) p.part_ml[(int64_t)part * p.rows + r] = make_float2(m, l);
+// Where row r (of the tile's rows) of a finished item goes, or of a partial one; `scale`: what its values are multiplied by.
+template <typename T> struct RowOut {
+  T* out; float* part; float scale;
+  RowOut() = default;
+  __device__ RowOut(const AttnParams& p, int part_index, int b, int head, int r, float m, float l, bool writes_norm) {
+    const int64_t row = (int64_t)b * p.heads + head;
+    out = static_cast<T*>(p.out) + row * p.dim;
+    part = part_index < 0 ? nullptr : p.part_o + ((int64_t)part_index * p.rows + r) * p.dim;
+    scale = part_index >= 0 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+    if (writes_norm) {
+      if (part_index >= 0) p.part_ml[(int64_t)part_index * p.rows + r] = make_float2(m, l);
+      else if (p.lse) p.lse[row] = l == 0.f ? -INFINITY : m * AT_LN2 + logf(l);
+    }
   }
-}
+  __device__ __forceinline__ void put(int d, float o) const {
+    if (part) part[d] = o; else out[d] = from_f32<T>(o * scale);
+  }
+};
 
 // Adds the partial results of the item that starts in share c and ends in share meta.y: a warp takes every fourth of them, the four
 // sums are added in order.
@@ -214,7 +238,8 @@ __global__ void __launch_bounds__(128) attend_join_kernel(const AttnParams p) {
   if (lane == 0) s_l[warp] = l;
   __syncthreads();
   l = s_l[0] + s_l[1] + s_l[2] + s_l[3];
-  for (int d = threadIdx.x; d < p.dim; d += 128) put<T>(p, -1, b, head0, r, d, s_o[0][d] + s_o[1][d] + s_o[2][d] + s_o[3][d], m, l);
+  const RowOut<T> out(p, -1, b, head0 + r, r, m, l, threadIdx.x == 0);
+  for (int d = threadIdx.x; d < p.dim; d += 128) out.put(d, s_o[0][d] + s_o[1][d] + s_o[2][d] + s_o[3][d]);
 }
 
 // Where key j of sequence b lies: page name and place inside the page; false where there is no such page.
@@ -407,7 +432,7 @@ __global__ void __launch_bounds__(FM_WARPS * 32) attend_fma_kernel(const AttnPar
         sum += s_ml[w * R + r].y * fw;
         val += s_o[(w * R + r) * p.dim + d] * fw;
       }
-      put<float>(p, part, b, head0, r, d, val, top, sum);
+      RowOut<float>(p, part, b, head0 + r, r, top, sum, d == 0).put(d, val);
     }
     if (s.last >= 0 && tid == 0) p.meta[blockIdx.x] = make_int2(b * p.kv_heads * p.row_tiles + s.sub, s.last);
     __syncthreads();
@@ -446,8 +471,9 @@ template <int DP, bool TWO> struct MmaShape {
   static constexpr int R = TWO ? 16 : 8;                           // rows: query heads of a tile
   static constexpr int NC = 4;                                     // warps that compute
   static constexpr int THREADS = (NC + MM_COPIERS) * 32;
-  static constexpr int KEYS = DP == 256 ? 16 : 32;                 // of a tile
-  static constexpr int START = DP == 256 ? 4 : 3;
+  static constexpr int KEYS = DP > 128 ? 16 : 32;                  // of a tile
+  static constexpr int START = DP > 128 ? 4 : 3;
+  static constexpr int LPR = DP <= 64 ? 8 : DP <= 128 ? 16 : 32;   // lanes of a row of the copies
   static constexpr int ROW = ((DP / 8) | 1) * 16;                  // an odd number of 16-byte pieces: ldmatrix without bank conflicts
   static constexpr int SLOT = 2 * KEYS * ROW;                      // keys, then values
   static constexpr int JROW = 40;                                  // floats of a row of 32 values in the join buffers: no bank conflicts
@@ -494,7 +520,6 @@ __global__ void __launch_bounds__(MmaShape<DP, TWO>::THREADS, 1) attend_mma_kern
   __shared__ int s_gave_up;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t ring = s_u32(tl_smem), full = s_u32(s_full), empty = s_u32(s_empty);
-  const int nk = p.dim / 16;
   pdl_trigger();
   if (tid < NS) {
     bar_init(full + tid * 8, 33);        // the copies of 32 lanes, and the word of live keys
@@ -515,10 +540,10 @@ __global__ void __launch_bounds__(MmaShape<DP, TWO>::THREADS, 1) attend_mma_kern
 
   if (warp >= NC) {
     // ------------------------------------------------------------ copiers
-    constexpr int LPR = DP / 8;                                   // lanes of a row
+    constexpr int LPR = S::LPR;
     constexpr int STEP = 32 / LPR;                                // rows of an instruction
     const int piece = lane % LPR;
-    const bool in_dim = piece * 8 < p.dim;
+    const bool in_row = piece * 8 < DP, in_dim = piece * 8 < p.dim;   // pieces from dim on are filled with zeros
     const bool one_page = p.page_size % 16 == 0;                  // 16 keys from a multiple of 16 on lie in one page
     int n = warp - NC, n0 = 0;                                    // this warp's next tile; tiles before the segment
     int slot = n, use = 0;                                        // n % NS, n / NS
@@ -541,15 +566,16 @@ __global__ void __launch_bounds__(MmaShape<DP, TWO>::THREADS, 1) attend_mma_kern
             const int64_t pg = __shfl_sync(0xffffffffu, page_now, half * 16), pl = __shfl_sync(0xffffffffu, place_now, half * 16);
             const T* kp = k_lane + (pg * p.k_page + pl * p.k_slot);
             const T* vp = v_lane + (pg * p.v_page + pl * p.v_slot);
-            if (in_dim) {
+            if (!in_dim) { kp = k_lane; vp = v_lane; }
+            if (in_row) {
 #pragma unroll
               for (int i = 0; i < 16 / STEP; ++i) {
-                cp_async(dst + i * STEP * S::ROW, kp, true);
+                cp_async(dst + i * STEP * S::ROW, kp, in_dim);
                 kp += STEP * p.k_slot;
               }
 #pragma unroll
               for (int i = 0; i < 16 / STEP; ++i) {
-                cp_async(dst + (KEYS + i * STEP) * S::ROW, vp, true);
+                cp_async(dst + (KEYS + i * STEP) * S::ROW, vp, in_dim);
                 vp += STEP * p.v_slot;
               }
             }
@@ -558,8 +584,8 @@ __global__ void __launch_bounds__(MmaShape<DP, TWO>::THREADS, 1) attend_mma_kern
             for (int i = 0; i < 16 / STEP; ++i) {
               const int row = half * 16 + i * STEP + lane / LPR;
               const int64_t pg = __shfl_sync(0xffffffffu, page_now, row), pl = __shfl_sync(0xffffffffu, place_now, row) - lane / LPR;
-              const bool on = live >> row & 1;
-              if (in_dim) {                                       // rows that are not live are filled with zeros
+              const bool on = in_dim && (live >> row & 1);
+              if (in_row) {                                       // rows that are not live are filled with zeros
                 cp_async(dst + i * STEP * S::ROW, on ? k_lane + (pg * p.k_page + pl * p.k_slot) : k_lane, on);
                 cp_async(dst + (KEYS + i * STEP) * S::ROW, on ? v_lane + (pg * p.v_page + pl * p.v_slot) : v_lane, on);
               }
@@ -597,9 +623,9 @@ __global__ void __launch_bounds__(MmaShape<DP, TWO>::THREADS, 1) attend_mma_kern
       for (int i = 0; i < (TWO ? 4 : 2); ++i) {
         const int r = TWO ? g + (i & 1) * 8 : g, d = ks * 16 + t4 * 2 + (TWO ? i >> 1 : i) * 8;
         q[ks][i] = 0;
-        if (r < rows && ks < nk) {
+        if (r < rows && d < p.dim) {
           const T* src = static_cast<const T*>(p.q) + ((int64_t)s.b * p.q_b + (int64_t)(head0 + r) * p.q_h + d);
-          q[ks][i] = bits_of<T>(src[0], src[1]);
+          q[ks][i] = p.q_words ? *reinterpret_cast<const uint32_t*>(src) : bits_of<T>(src[0], src[1]);
         }
       }
   };
@@ -625,7 +651,7 @@ __global__ void __launch_bounds__(MmaShape<DP, TWO>::THREADS, 1) attend_mma_kern
         for (int e = 0; e < 4; ++e) c[nt][e] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < DP / 16; ++ks) {
-        if (ks < nk) {
+        {
           uint32_t kb[KEYS / 16][4];
 #pragma unroll
           for (int j = 0; j < KEYS / 16; ++j) ldsm4(kb[j], k_at + off + ks * 32 + j * 16 * S::ROW);
@@ -679,7 +705,7 @@ __global__ void __launch_bounds__(MmaShape<DP, TWO>::THREADS, 1) attend_mma_kern
       }
 #pragma unroll
       for (int cc = 0; cc < DP / 16; ++cc) {
-        if (cc < nk) {
+        {
 #pragma unroll
           for (int j = 0; j < KEYS / 16; ++j) {
             uint32_t vb[4];
@@ -732,29 +758,39 @@ __global__ void __launch_bounds__(MmaShape<DP, TWO>::THREADS, 1) attend_mma_kern
     const int h = now.sub / p.row_tiles, x = now.sub - h * p.row_tiles;
     const int head0 = h * p.group + x * p.rows, rows = min(p.rows, p.group - x * p.rows);
     const int part = part_of(now);
+    auto lay_down = [&](int sl) {
+      float* buf = s_join + (sl & 1) * (NC * R * S::JROW) + (warp * R + g) * S::JROW + t4 * 2;
+#pragma unroll
+      for (int half = 0; half < (TWO ? 2 : 1); ++half)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int nt = sl * 4 + i;
+          const float a = TWO ? o[nt][2 * half] : o[nt][0] + o[nt][2], e = TWO ? o[nt][2 * half + 1] : o[nt][1] + o[nt][3];
+          *reinterpret_cast<float2*>(buf + half * 8 * S::JROW + i * 8) = make_float2(a * f[half], e * f[half]);
+        }
+    };
+    lay_down(0);
+    meet();
+    RowOut<T> out[R / NC] = {};
+#pragma unroll
+    for (int e = 0; e < R / NC; ++e) {
+      const int r = e * NC + warp;
+      const float2 ml = s_row[r];
+      if (r < rows) out[e] = RowOut<T>(p, part, now.b, head0 + r, r, ml.x, ml.y, lane == 0);
+    }
 #pragma unroll
     for (int sl = 0; sl < DP / 32; ++sl) {
-      if (sl * 32 < p.dim) {
-        float* buf = s_join + (sl & 1) * (NC * R * S::JROW);
+      if (sl > 0) meet();
+      const float* buf = s_join + (sl & 1) * (NC * R * S::JROW);
 #pragma unroll
-        for (int half = 0; half < (TWO ? 2 : 1); ++half)
+      for (int e = 0; e < R / NC; ++e) {
+        const int r = e * NC + warp, d = sl * 32 + lane;
+        float sum = 0.f;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int nt = sl * 4 + i;
-            const float a = TWO ? o[nt][2 * half] : o[nt][0] + o[nt][2], e = TWO ? o[nt][2 * half + 1] : o[nt][1] + o[nt][3];
-            *reinterpret_cast<float2*>(buf + (warp * R + g + half * 8) * S::JROW + i * 8 + t4 * 2) = make_float2(a * f[half], e * f[half]);
-          }
-        meet();
-#pragma unroll
-        for (int e = 0; e < R / NC; ++e) {
-          const int r = e * NC + warp, d = sl * 32 + lane;
-          float sum = 0.f;
-#pragma unroll
-          for (int w = 0; w < NC; ++w) sum += buf[(w * R + r) * S::JROW + lane];
-          const float2 ml = s_row[r];
-          if (r < rows && d < p.dim) put<T>(p, part, now.b, head0, r, d, sum, ml.x, ml.y);
-        }
+        for (int w = 0; w < NC; ++w) sum += buf[(w * R + r) * S::JROW + lane];
+        if (r < rows && d < p.dim) out[e].put(d, sum);
       }
+      if (sl + 1 < DP / 32) lay_down(sl + 1);
     }
     if (now.last >= 0 && tid == 0) p.meta[blockIdx.x] = make_int2(now.b * p.kv_heads * p.row_tiles + now.sub, now.last);
   }
@@ -815,8 +851,11 @@ int run_f32(AttnParams& p, cudaStream_t st) {
 template <typename T>
 int run_16bit(AttnParams& p, cudaStream_t st) {
   set_rows(p, 16);
-  if (p.rows <= 8) return p.dim > 128 ? run_mma<T, 256, false>(p, st) : p.dim > 64 ? run_mma<T, 128, false>(p, st) : run_mma<T, 64, false>(p, st);
-  return p.dim > 128 ? run_mma<T, 256, true>(p, st) : p.dim > 64 ? run_mma<T, 128, true>(p, st) : run_mma<T, 64, true>(p, st);
+  if (p.rows <= 8)
+    return p.dim <= 64 ? run_mma<T, 64, false>(p, st) : p.dim <= 96 ? run_mma<T, 96, false>(p, st) : p.dim <= 128 ? run_mma<T, 128, false>(p, st)
+         : p.dim <= 192 ? run_mma<T, 192, false>(p, st) : run_mma<T, 256, false>(p, st);
+  return p.dim <= 64 ? run_mma<T, 64, true>(p, st) : p.dim <= 96 ? run_mma<T, 96, true>(p, st) : p.dim <= 128 ? run_mma<T, 128, true>(p, st)
+       : p.dim <= 192 ? run_mma<T, 192, true>(p, st) : run_mma<T, 256, true>(p, st);
 }
 
 constexpr int AT_MAX_ROWS = 16;         // rows of a partial result at most
@@ -882,7 +921,7 @@ int kq_paged_attention(const void* q, int dtype, int64_t batch, int64_t heads, i
   if (scratch_bytes < L.total) { set_error("%s: scratch too small (%zu < %zu)", fn, scratch_bytes, L.total); return KQ_ESCRATCH; }
 
   AttnParams p;
-  p.q = q; p.q_b = q_stride_batch; p.q_h = q_stride_head;
+  p.q = q; p.q_b = q_stride_batch; p.q_h = q_stride_head; p.q_words = !((uintptr_t)q % 4 || q_stride_batch % 2 || q_stride_head % 2);
   p.k = k_cache; p.k_page = k_strides[0]; p.k_slot = k_strides[1]; p.k_head = k_strides[2];
   p.v = v_cache; p.v_page = v_strides[0]; p.v_slot = v_strides[1]; p.v_head = v_strides[2];
   p.table = block_table; p.table_b = table_stride; p.width = (int)table_width; p.lens = seq_lens;
