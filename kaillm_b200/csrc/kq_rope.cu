@@ -7,6 +7,8 @@
 //
 // All of it in fp32 with one rounding at the end; the angle is the exact product, reduced to one turn in fp64 (position 10^6
 // times a frequency near 1 would be off by 0.06 rad in fp32), and its cosine and sine are formed once per token.
+#include <type_traits>
+
 #include "kq_common.cuh"
 
 namespace kq {
@@ -21,7 +23,7 @@ struct RopeParams {
   const void* positions; int pos64;
   const float* inv_freq;
   const void* qw; const void* kw; int w_f32;
-  float eps, factor;
+  float eps, factor, inv_dim;
   int64_t tokens;
   int heads, kv_heads, dim, half, interleaved;
   void* q;                                           // [tokens][heads][dim]
@@ -63,7 +65,181 @@ __device__ __forceinline__ T* target_of(const RopeParams& p, int64_t t, int head
              : static_cast<T*>(p.v) + page * p.v_page + place * p.v_slot + h * p.v_head;
 }
 
-// One CTA per token: the angles once into shared memory, then a warp per head; any even width, any alignment.
+// Rows of 16-byte pieces.  A lane owns two pieces A and B of a head whose values turn into one another: a pair of pieces half the rotated
+// width apart, or (interleaved, and behind the rotated part, where nothing turns) two neighbouring ones; D / 2V lanes share a
+// head (V values per piece), rounded up to a power of two for the sum of squares, and the other lanes take further heads.  So nothing but
+// that sum crosses lanes, and out_A = A * c0 + A' * c1, out_B = B * c2 + B' * c3 (A', B': the partners) with factors made of the norm's
+// weight and the token's cosine and sine, which a lane forms once for all heads of a kind and token and keeps in registers.
+// A CTA forms its token's angles while the first rows of queries, keys and values are on their way; its warps share the token's steps
+// (a step: as many heads as a warp holds).  SPREAD: queries, keys and values in CTAs of their own (blockIdx.z).
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack2(float x, float y) { f32x2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y)); return r; }
+__device__ __forceinline__ float2 unpack2(f32x2 v) { float2 r; asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v)); return r; }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) { f32x2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) { f32x2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ f32x2 swap2(f32x2 v) { const float2 u = unpack2(v); return pack2(u.y, u.x); }
+
+template <typename T> __device__ __forceinline__ f32x2 widen(const uint4& v, int i) {   // values 2i, 2i + 1 of a piece
+  const T* e = reinterpret_cast<const T*>(&v);
+  return pack2(to_f32<T>(e[2 * i]), to_f32<T>(e[2 * i + 1]));
+}
+template <typename T> __device__ __forceinline__ void narrow(uint4& v, int i, f32x2 x) {
+  const float2 u = unpack2(x);
+  if constexpr (sizeof(T) == 4) {
+    reinterpret_cast<float2*>(&v)[i] = u;
+  } else if constexpr (std::is_same<T, __half>::value) {
+    reinterpret_cast<__half2*>(&v)[i] = __floats2half2_rn(u.x, u.y);
+  } else {
+    reinterpret_cast<__nv_bfloat162*>(&v)[i] = __floats2bfloat162_rn(u.x, u.y);
+  }
+}
+
+// V values of a norm weight from d on (without a weight: ones)
+template <typename T, int V>
+__device__ __forceinline__ void weights_of(const RopeParams& p, const void* w, int d, float (&out)[V]) {
+  if (!w) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) out[e] = 1.f;
+  } else if (p.w_f32) {
+#pragma unroll
+    for (int e = 0; e < V; e += 4) {
+      const float4 f = *reinterpret_cast<const float4*>(static_cast<const float*>(w) + d + e);
+      out[e] = f.x; out[e + 1] = f.y; out[e + 2] = f.z; out[e + 3] = f.w;
+    }
+  } else {
+    const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const T*>(w) + d);
+#pragma unroll
+    for (int e = 0; e < V; ++e) out[e] = to_f32<T>(reinterpret_cast<const T*>(&u)[e]);
+  }
+}
+
+// HALVES: pairs half a head apart and nothing unturned, so that no lane has to choose its partners.
+template <typename T, int WARPS, int AHEAD, bool HALVES, bool SPREAD>
+__global__ void __launch_bounds__(WARPS * 32, SPREAD ? 4 : 16 / WARPS) rope_rows_kernel(const RopeParams p, int lanes_log2) {
+  constexpr int V = 16 / (int)sizeof(T), P = V / 2;                               // values, pairs of them in a piece
+  __shared__ float2 s_turn[RP_MAX_DIM / 2];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t t = blockIdx.x;
+  const bool q_here = !SPREAD || blockIdx.z == 0, k_here = !SPREAD || blockIdx.z == 1, v_here = p.store && (!SPREAD || blockIdx.z == 2);
+  const int unit = lane & ((1 << lanes_log2) - 1);                               // this lane's pieces
+  const bool active = unit * 2 * V < p.dim;
+  const bool turned = HALVES || unit * 2 * V < 2 * p.half, apart = HALVES || (turned && !p.interleaved);
+  const int da = apart ? unit * V : unit * 2 * V, db = apart ? p.half + unit * V : unit * 2 * V + V;
+  const int per = 32 >> lanes_log2, step = gridDim.y * WARPS * per;               // heads of a step, from step to step of this warp
+  const int h0 = (blockIdx.y * WARPS + warp) * per + (lane >> lanes_log2);
+  pdl_trigger();
+  pdl_wait();
+  const T* src = static_cast<const T*>(p.qkv) + t * p.qkv_t + h0 * p.dim;
+  auto load = [&](const T* from, bool on, uint4& va, uint4& vb) {
+    va = vb = make_uint4(0, 0, 0, 0);
+    if (on) { va = *reinterpret_cast<const uint4*>(from + da); vb = *reinterpret_cast<const uint4*>(from + db); }
+  };
+  // the first steps of all three kinds are on their way before the angles are formed
+  uint4 a[AHEAD], b[AHEAD], ka, kb, va, vb;
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) load(src + i * step * p.dim, q_here && active && h0 + i * step < p.heads, a[i], b[i]);
+  const T* k_src = src + p.heads * p.dim;
+  const T* v_src = k_src + p.kv_heads * p.dim;
+  load(k_src, k_here && active && h0 < p.kv_heads, ka, kb);
+  load(v_src, v_here && active && h0 < p.kv_heads, va, vb);
+
+  const int64_t pos = index_at(p.positions, p.pos64, t);
+  for (int i = threadIdx.x; i < p.half; i += WARPS * 32) s_turn[i] = angle_of(p, pos, i);
+  T* k_dst = static_cast<T*>(p.k) + (t * p.kv_heads + h0) * p.dim;
+  T* v_dst = nullptr;
+  int64_t k_head = p.dim;
+  bool kept = active;
+  if (p.store && active) {
+    const int64_t slot = index_at(p.slots, p.slot64, t);
+    kept = slot >= 0 && slot < p.num_slots;
+    if (kept) {
+      const int64_t page = slot >> 31 ? slot / p.page_size : (int64_t)((uint32_t)slot / (uint32_t)p.page_size), place = slot - page * p.page_size;
+      k_dst = static_cast<T*>(p.k) + page * p.k_page + place * p.k_slot + h0 * p.k_head;
+      v_dst = static_cast<T*>(p.v) + page * p.v_page + place * p.v_slot + h0 * p.v_head;
+    }
+    k_head = p.k_head;
+  }
+  __syncthreads();
+
+  f32x2 c0[P], c1[P], c2[P], c3[P];
+  const float2* turn = s_turn + unit * V;
+  auto factors = [&](const void* w) {
+    float wa[V], wb[V];
+    weights_of<T, V>(p, active ? w : nullptr, da, wa);
+    weights_of<T, V>(p, active ? w : nullptr, db, wb);
+#pragma unroll
+    for (int e = 0; e < V; e += 2) {
+      if (HALVES || apart || !turned) {
+        const float2 u = turned && active ? turn[e] : make_float2(1.f, 0.f), v = turned && active ? turn[e + 1] : make_float2(1.f, 0.f);
+        c0[e / 2] = pack2(wa[e] * u.x, wa[e + 1] * v.x); c1[e / 2] = pack2(-wb[e] * u.y, -wb[e + 1] * v.y);
+        c2[e / 2] = pack2(wb[e] * u.x, wb[e + 1] * v.x); c3[e / 2] = pack2(wa[e] * u.y, wa[e + 1] * v.y);
+      } else {
+        const float2 u = turn[e / 2], v = turn[P + e / 2];
+        c0[e / 2] = pack2(wa[e] * u.x, wa[e + 1] * u.x); c1[e / 2] = pack2(-wa[e + 1] * u.y, wa[e] * u.y);
+        c2[e / 2] = pack2(wb[e] * v.x, wb[e + 1] * v.x); c3[e / 2] = pack2(-wb[e + 1] * v.y, wb[e] * v.y);
+      }
+    }
+  };
+  auto turn_and_put = [&](uint4 ra, uint4 rb, bool normed, T* dst, bool on) {
+    f32x2 x[P], y[P];
+#pragma unroll
+    for (int e = 0; e < P; ++e) { x[e] = widen<T>(ra, e); y[e] = widen<T>(rb, e); }
+    f32x2 inv = 0;
+    if (normed) {
+      f32x2 sq = mul2(x[0], x[0]);
+#pragma unroll
+      for (int e = 0; e < P; ++e) sq = fma2(y[e], y[e], e ? fma2(x[e], x[e], sq) : sq);
+      float sum = unpack2(sq).x + unpack2(sq).y;
+      for (int m = 1 << lanes_log2 >> 1; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+      const float f = rsqrtf(fmaf(sum, p.inv_dim, p.eps));
+      inv = pack2(f, f);
+    }
+#pragma unroll
+    for (int e = 0; e < P; ++e) {
+      // behind the rotated part the partner counts with 0, also where it is no number
+      const f32x2 px = apart ? y[e] : turned ? swap2(x[e]) : 0, py = apart ? x[e] : turned ? swap2(y[e]) : 0;
+      f32x2 u = fma2(px, c1[e], mul2(x[e], c0[e])), v = fma2(py, c3[e], mul2(y[e], c2[e]));
+      if (normed) { u = mul2(u, inv); v = mul2(v, inv); }
+      narrow<T>(ra, e, u);
+      narrow<T>(rb, e, v);
+    }
+    if (on) { *reinterpret_cast<uint4*>(dst + da) = ra; *reinterpret_cast<uint4*>(dst + db) = rb; }
+  };
+  if (v_here) {                                                   // values go as they came
+    for (int h = h0; h - (lane >> lanes_log2) < p.kv_heads; h += step) {
+      if (kept && active && h < p.kv_heads) { *reinterpret_cast<uint4*>(v_dst + da) = va; *reinterpret_cast<uint4*>(v_dst + db) = vb; }
+      v_src += step * p.dim;
+      v_dst += step * p.v_head;
+      load(v_src, active && h + step < p.kv_heads, va, vb);
+    }
+  }
+  factors(q_here ? p.qw : p.kw);
+  T* dst = static_cast<T*>(p.q) + (t * p.heads + h0) * p.dim;
+  src += AHEAD * step * p.dim;
+  for (int h = h0; q_here && h - (lane >> lanes_log2) < p.heads; h += AHEAD * step) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int hi = h + i * step;
+      if (hi - (lane >> lanes_log2) >= p.heads) break;
+      const uint4 ra = a[i], rb = b[i];
+      load(src, active && hi + AHEAD * step < p.heads, a[i], b[i]);
+      src += step * p.dim;
+      turn_and_put(ra, rb, p.qw != nullptr, dst, active && hi < p.heads);
+      dst += step * p.dim;
+    }
+  }
+  if (!k_here || h0 - (lane >> lanes_log2) >= p.kv_heads) return;
+  if (!SPREAD && p.kw != p.qw) factors(p.kw);
+  for (int h = h0; h - (lane >> lanes_log2) < p.kv_heads; h += step) {
+    const uint4 ra = ka, rb = kb;
+    k_src += step * p.dim;
+    load(k_src, active && h + step < p.kv_heads, ka, kb);
+    turn_and_put(ra, rb, p.kw != nullptr, k_dst, kept && active && h < p.kv_heads);
+    k_dst += step * k_head;
+  }
+}
+
+// Any even width, any alignment: one CTA per token (or part of its heads), a warp per head, the angles once into shared memory.
 template <typename T>
 __global__ void __launch_bounds__(RP_THREADS) rope_any_kernel(const RopeParams p) {
   __shared__ float2 s_turn[RP_MAX_DIM / 2];
@@ -108,13 +284,39 @@ __global__ void __launch_bounds__(RP_THREADS) rope_any_kernel(const RopeParams p
   }
 }
 
+// rope_rows_kernel's case: every row, piece pair and target made of 16-byte pieces at 16-byte addresses
+template <typename T>
+bool in_pieces(const RopeParams& p) {
+  constexpr int V = 16 / (int)sizeof(T);
+  const int64_t strides = p.qkv_t | p.k_page | p.k_slot | p.k_head | p.v_page | p.v_slot | p.v_head;   // zeros where there is no cache
+  const uintptr_t at = (uintptr_t)p.qkv | (uintptr_t)p.q | (uintptr_t)p.k | (uintptr_t)p.v | (uintptr_t)p.qw | (uintptr_t)p.kw;
+  return p.dim % (2 * V) == 0 && p.half % V == 0 && p.dim <= 64 * V && strides % V == 0 && at % 16 == 0;
+}
+
 template <typename T>
 int run_rope(const RopeParams& p, cudaStream_t st) {
   const int all = p.heads + (p.store ? 2 : 1) * p.kv_heads;
+  const bool pdl = options().pdl != 0;
+  if (in_pieces<T>(p)) {
+    int log2 = 0;
+    while ((1 << log2) * (32 / (int)sizeof(T)) < p.dim) ++log2;
+    const bool halves = !p.interleaved && 2 * p.half == p.dim;
+    if (p.tokens >= 4 * sm_count()) {
+      // many tokens: two warps walk a token's heads
+      KQ_CUDA_TRY(launch_pdl(halves ? rope_rows_kernel<T, 2, 2, true, false> : rope_rows_kernel<T, 2, 2, false, false>, dim3((unsigned)p.tokens), dim3(64), (size_t)0, st, pdl, p, log2));
+    } else {
+      // few: a step per warp, queries, keys and values apart, spread over the multiprocessors
+      const int steps = ((p.heads > p.kv_heads ? p.heads : p.kv_heads) + (32 >> log2) - 1) >> (5 - log2);
+      const dim3 grid((unsigned)p.tokens, (unsigned)((steps + 3) / 4), p.store ? 3 : 2);
+      KQ_CUDA_TRY(launch_pdl(halves ? rope_rows_kernel<T, 4, 1, true, true> : rope_rows_kernel<T, 4, 1, false, true>, grid, dim3(128), (size_t)0, st, pdl, p, log2));
+    }
+    options().launches += 1;
+    return KQ_OK;
+  }
   // few tokens: the heads of one token over several CTAs
   int64_t split = 1;
   while (p.tokens * split < 2 * sm_count() && split * (RP_THREADS / 32) < all) split *= 2;
-  KQ_CUDA_TRY(launch_pdl(rope_any_kernel<T>, dim3((unsigned)p.tokens, (unsigned)split), dim3(RP_THREADS), (size_t)0, st, options().pdl != 0, p));
+  KQ_CUDA_TRY(launch_pdl(rope_any_kernel<T>, dim3((unsigned)p.tokens, (unsigned)split), dim3(RP_THREADS), (size_t)0, st, pdl, p));
   options().launches += 1;
   return KQ_OK;
 }
@@ -147,7 +349,7 @@ extern "C" int kq_qk_norm_rope(const void* qkv, int dtype, int64_t tokens, int64
   if ((uintptr_t)qkv % size || (uintptr_t)q_out % size || (uintptr_t)k_out % size || (uintptr_t)v_cache % size || (uintptr_t)inv_freq % 4) { set_error("%s: misaligned pointer", fn); return KQ_EINVAL; }
   RopeParams p;
   p.qkv = qkv; p.qkv_t = stride_t; p.positions = positions; p.pos64 = positions64; p.inv_freq = inv_freq;
-  p.qw = q_weight; p.kw = k_weight; p.w_f32 = w_dtype == KQ_F32; p.eps = eps; p.factor = factor; p.tokens = tokens;
+  p.qw = q_weight; p.kw = k_weight; p.w_f32 = w_dtype == KQ_F32; p.eps = eps; p.factor = factor; p.inv_dim = 1.f / (float)head_dim; p.tokens = tokens;
   p.heads = (int)heads; p.kv_heads = (int)kv_heads; p.dim = (int)head_dim; p.half = (int)(rotated / 2); p.interleaved = interleaved != 0;
   p.q = q_out; p.k = k_out; p.v = v_cache; p.slots = slots; p.slot64 = slots64; p.store = store;
   p.num_slots = store ? num_pages * page_size : 0; p.page_size = store ? (int)page_size : 1;

@@ -4,9 +4,13 @@
 //   groups: a group counts its best expert (no bias) or the sum of its two best c (bias); only the top groups stay
 //   ids = the top_k experts by c, descending, ties to the lowest index;  w = p[ids] (/ sum) * scale
 //
-// A warp per token; the experts' values sit in registers, expert i * 32 + lane in slot i of a lane.  Without a bias the choice
-// compares the logits themselves and is exact.  With a bias it is made in fp64: two of a few hundred scores lie closer than fp32
-// tells apart once in some thousand tokens, and a router's choice should not depend on the last bit of an exponential.
+// A warp per token, NV experts next to each other per lane.  Without a bias the choice compares the logits themselves.  With one, two of
+// a few hundred scores lie closer than fp32 tells apart once in some thousand tokens, and a router's choice should not depend on the
+// last bit of an exponential: a token whose chosen scores (or group scores) come within RT_CLOSE of one another, or of the first one
+// left out, is routed again in fp64 (route_wide).
+//
+// Bound by instructions, about 500 per token (17 MB and 2.7 us of memory for 16384 x 256 fp32 logits): the best of 32 lanes is one
+// redux.sync on order-preserving integers, and where whole lanes make up a group all groups are scored at once.
 #include "kq_common.cuh"
 
 namespace kq {
@@ -22,24 +26,134 @@ struct RouteParams {
   int experts, top_k, sigmoid, groups, top_groups, group_size, renormalize;
   const float* bias;
   float scale;
+  int aligned, bias_aligned;  // rows, the bias start at 16-byte addresses
   float* weights; int32_t* ids;
 };
 
-constexpr double RT_OUT = -1e301;   // below every score: experts outside the chosen groups, or already taken
-constexpr double RT_LOW = -1e300;   // a score of -infinity (a masked expert): after every finite one, before RT_OUT
-
-__device__ __forceinline__ double warp_max(double v) {
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) v = fmax(v, __shfl_xor_sync(0xffffffffu, v, d));
-  return v;
-}
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
   return v;
 }
 // NaN counts as -infinity and +infinity as the largest finite value, so that the probabilities of a row stay numbers
-__device__ __forceinline__ float sane(float x) { return x != x ? -INFINITY : fminf(x, 3.4028234663852886e38f); }
+__device__ __forceinline__ float sane(float x) { return fminf(fmaxf(x, -INFINITY), 3.4028234663852886e38f); }   // the larger of NaN and y is y
+
+// fp64 scores as integers that compare as they do (both zeros alike); RT_TAKEN below all of them
+constexpr unsigned long long RT_TAKEN = 0, RT_OUTSIDE = 1;      // taken; outside the chosen groups (no score maps to either)
+__device__ __forceinline__ unsigned long long ordered64(double v) {
+  const unsigned long long u = __double_as_longlong(v + 0.);
+  return u ^ (u >> 63 ? 0xffffffffffffffffull : 0x8000000000000000ull);
+}
+__device__ __forceinline__ double unordered64(unsigned long long k) {
+  return __longlong_as_double(k ^ (k >> 63 ? 0x8000000000000000ull : 0xffffffffffffffffull));
+}
+__device__ __forceinline__ unsigned long long warp_max64(unsigned long long v) {
+  const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(v >> 32));
+  const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(v >> 32) == hi ? (uint32_t)v : 0u);
+  return (unsigned long long)hi << 32 | lo;
+}
+
+// A token whose choice fp32 cannot make, with a bias: scores, groups and choice in fp64; NV experts next to each other per lane.
+template <typename T, int NV>
+__device__ __noinline__ void route_wide(const RouteParams& p, int64_t t) {
+  const int lane = threadIdx.x & 31, e0 = lane * NV;
+  const T* row = static_cast<const T*>(p.logits) + t * p.stride_t;
+  float x[NV];
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    x[i] = e0 + i < p.experts ? sane(to_f32<T>(row[e0 + i])) : -INFINITY;
+    top = fmaxf(top, x[i]);
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+  top = fmaxf(top, -3.4028234663852886e38f);
+  double sum = 0.;
+  double c[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    c[i] = exp(p.sigmoid ? -(double)x[i] : (double)x[i] - (double)top);
+    sum += c[i];
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  sum = fmax(sum, 1e-300);
+  unsigned long long key[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    key[i] = e0 + i < p.experts ? ordered64((p.sigmoid ? 1. / (1. + c[i]) : c[i] / sum) + (double)sane(p.bias[e0 + i])) : RT_TAKEN;
+  if (p.groups > 1) {
+    unsigned long long mine = RT_TAKEN;          // score of group `lane`
+    for (int g = 0; g < p.groups; ++g) {
+      const int lo = g * p.group_size, hi = lo + p.group_size;
+      unsigned long long a = RT_TAKEN, b = RT_TAKEN;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const unsigned long long k = e0 + i >= lo && e0 + i < hi ? key[i] : RT_TAKEN;
+        if (k > a) { b = a; a = k; } else if (k > b) b = k;
+      }
+      const unsigned long long best = warp_max64(a);
+      unsigned long long score = best;
+      if (p.group_size > 1) {
+        const int owner = __ffs(__ballot_sync(0xffffffffu, a == best)) - 1;
+        score = ordered64(unordered64(best) + unordered64(warp_max64(lane == owner ? b : a)));
+      }
+      if (lane == g) mine = score;
+    }
+    unsigned kept = 0;
+    for (int n = 0; n < p.top_groups; ++n) {
+      const unsigned long long best = warp_max64(mine);
+      const int g = __ffs(__ballot_sync(0xffffffffu, mine == best)) - 1;
+      kept |= 1u << g;
+      if (lane == g) mine = RT_TAKEN;
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (e0 + i < p.experts && !(kept >> ((e0 + i) / p.group_size) & 1)) key[i] = RT_OUTSIDE;
+  }
+  int id = 0;                                    // of rank `lane`
+  float w = 0.f;
+  for (int n = 0; n < p.top_k; ++n) {
+    unsigned long long a = key[0];
+    int at = 0;
+    float xv = x[0];
+#pragma unroll
+    for (int i = 1; i < NV; ++i)
+      if (key[i] > a) { a = key[i]; at = i; xv = x[i]; }
+    const unsigned long long best = warp_max64(a);
+    const int owner = __ffs(__ballot_sync(0xffffffffu, a == best)) - 1;
+    const int e = __shfl_sync(0xffffffffu, e0 + at, owner);
+    const float xe = __shfl_sync(0xffffffffu, xv, owner);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (e0 + i == e) key[i] = RT_TAKEN;
+    if (lane == n) {
+      id = e;
+      w = (float)(p.sigmoid ? 1. / (1. + exp(-(double)xe)) : exp((double)xe - (double)top) / sum);
+    }
+  }
+  if (p.renormalize) w /= fmaxf(warp_sum(w), 1.1754943508222875e-38f);
+  if (lane < p.top_k) {
+    p.weights[t * p.top_k + lane] = w * p.scale;
+    p.ids[t * p.top_k + lane] = id;
+  }
+}
+
+__device__ __forceinline__ uint32_t ordered(float v) {      // compares as v does (both zeros alike)
+  const uint32_t u = __float_as_uint(v + 0.f);
+  return u ^ (u >> 31 ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ float unordered(uint32_t k) { return __uint_as_float(k ^ (k >> 31 ? 0x80000000u : 0xffffffffu)); }
+// fp32 scores nearer than this (times the larger of 1 and their size) may be in the wrong order.  With u = 2^-24 an exponential is off by
+// (4 + |x|) u of itself; a sigmoid by p (1 - p) (4 + |x|) u + 4 p u < 5.5 u; a softmax by 30 p u (its sum of up to 1024 terms
+// included), so two of them, or the four of two groups, by 30 u together; the sum with the bias by another u of itself.  64 u are asked for.
+constexpr float RT_CLOSE = 1.f / (1 << 18);
+__device__ __forceinline__ bool close(float hi, float lo) { return !(hi - lo > RT_CLOSE * fmaxf(1.f, fabsf(hi))); }
+__device__ __forceinline__ float fast_exp(float x) {        // relative error 2^-22 + |x| 2^-24
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+  return y;
+}
 
 template <typename T, int NV>
 __global__ void __launch_bounds__(RT_WARPS * 32) route_kernel(const RouteParams p) {
@@ -49,98 +163,198 @@ __global__ void __launch_bounds__(RT_WARPS * 32) route_kernel(const RouteParams 
   pdl_wait();
   if (t >= p.tokens) return;
   const T* row = static_cast<const T*>(p.logits) + t * p.stride_t;
+  const int e0 = lane * NV;
+  __shared__ uint2 s_list[RT_WARPS][32];
   float x[NV];
-  float top = -INFINITY;
+  constexpr int VEC = NV * (int)sizeof(T) >= 16 ? 16 / (int)sizeof(T) : NV;      // values of one load
+  if (p.aligned && (p.experts % NV == 0)) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int e = i * 32 + lane;
-    x[i] = e < p.experts ? sane(to_f32<T>(row[e])) : -INFINITY;
-    top = fmaxf(top, x[i]);
+    for (int i = 0; i < NV; i += VEC) {
+      alignas(16) T v[VEC];
+      if (e0 < p.experts) {
+        if constexpr (VEC * sizeof(T) == 16) *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(row + e0 + i);
+        else if constexpr (VEC * sizeof(T) == 8) *reinterpret_cast<uint2*>(v) = *reinterpret_cast<const uint2*>(row + e0 + i);
+        else if constexpr (VEC * sizeof(T) == 4) *reinterpret_cast<uint32_t*>(v) = *reinterpret_cast<const uint32_t*>(row + e0 + i);
+        else v[0] = row[e0];
+      }
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) x[i + j] = e0 < p.experts ? sane(to_f32<T>(v[j])) : -INFINITY;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) x[i] = e0 + i < p.experts ? sane(to_f32<T>(row[e0 + i])) : -INFINITY;
   }
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-  top = fmaxf(top, -3.4028234663852886e38f);     // a row of masked experts only: probabilities of zero instead of NaN
-  float sum = 0.f;
+  float top = 0.f, sum = 1.f;
   if (!p.sigmoid) {
+    top = x[0];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) sum += expf(x[i] - top);
+    for (int i = 1; i < NV; ++i) top = fmaxf(top, x[i]);
+    top = unordered(__reduce_max_sync(0xffffffffu, ordered(top)));
+    top = fmaxf(top, -3.4028234663852886e38f);   // a row of masked experts only: probabilities of zero instead of NaN
+    sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) sum += fast_exp(x[i] - top);
     sum = fmaxf(warp_sum(sum), 1.1754943508222875e-38f);
   }
-  double c[NV];
-  double wide = 0.;
-  if (p.bias && !p.sigmoid) {
+  // order-preserving keys of the scores; 0: no expert, or taken
+  uint32_t key[NV];
+  if (p.bias) {
+    const float inv = p.sigmoid ? 1.f : 1.f / sum;
+    float bias[NV];
+    if (NV % 4 == 0 && p.bias_aligned && p.experts % NV == 0) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) wide += exp((double)x[i] - (double)top);
+      for (int i = 0; i < NV; i += 4)
+        if (e0 < p.experts) *reinterpret_cast<float4*>(bias + i) = *reinterpret_cast<const float4*>(p.bias + e0 + i);
+    } else {
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) wide += __shfl_xor_sync(0xffffffffu, wide, d);
-    wide = fmax(wide, 1e-300);
-  }
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int e = i * 32 + lane;
-    if (e >= p.experts) { c[i] = RT_OUT; continue; }
-    double v = x[i];
-    if (p.bias) v = (p.sigmoid ? 1. / (1. + exp(-(double)x[i])) : exp((double)x[i] - (double)top) / wide) + (double)sane(p.bias[e]);
-    c[i] = v < RT_LOW ? RT_LOW : v;
-  }
-  if (p.groups > 1) {
-    // lane g ends with the value of group g
-    double value = RT_OUT;
-    for (int g = 0; g < p.groups; ++g) {
-      const int lo = g * p.group_size, hi = lo + p.group_size;
-      double a = RT_OUT, b = RT_OUT;             // the two best of the lane's experts in this group
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int e = i * 32 + lane;
-        if (e >= lo && e < hi) {
-          if (c[i] > a) { b = a; a = c[i]; } else if (c[i] > b) b = c[i];
-        }
-      }
-      const double best = warp_max(a);
-      double s = best;
-      if (p.bias && p.group_size > 1) {
-        const int owner = __ffs(__ballot_sync(0xffffffffu, a == best)) - 1;
-        s += warp_max(lane == owner ? b : a);
-      }
-      if (lane == g) value = s < RT_LOW ? RT_LOW : s;
-    }
-    unsigned keep = 0;
-    for (int n = 0; n < p.top_groups; ++n) {
-      const double best = warp_max(value);
-      const int g = __ffs(__ballot_sync(0xffffffffu, value == best)) - 1;
-      keep |= 1u << g;
-      if (lane == g) value = 2 * RT_OUT;
+      for (int i = 0; i < NV; ++i) bias[i] = e0 + i < p.experts ? p.bias[e0 + i] : 0.f;
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int e = i * 32 + lane;
-      if (e < p.experts && !(keep >> (e / p.group_size) & 1)) c[i] = RT_OUT;
+      const float pr = p.sigmoid ? __fdividef(1.f, 1.f + fast_exp(-x[i])) : fast_exp(x[i] - top) * inv;
+      key[i] = e0 + i < p.experts ? ordered(pr + sane(bias[i])) : 0u;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) key[i] = e0 + i < p.experts ? ordered(x[i]) : 0u;
+  }
+  bool wide = false;                             // too close to call
+  if (p.groups > 1) {
+    uint32_t mine = 0;                           // lane's group's score, or in the general form that of group `lane`
+    bool whole = p.group_size % NV == 0;         // whole lanes make up a group, a power of two of them
+    const int lanes = p.group_size / NV;
+    whole = whole && (lanes & (lanes - 1)) == 0;
+    if (whole) {
+      uint32_t a = 0, b = 0;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) { b = max(b, min(a, key[i])); a = max(a, key[i]); }
+      for (int d = 1; d < lanes; d <<= 1) {
+        const uint32_t oa = __shfl_xor_sync(0xffffffffu, a, d), ob = __shfl_xor_sync(0xffffffffu, b, d);
+        b = max(min(a, oa), max(b, ob));
+        a = max(a, oa);
+      }
+      mine = p.bias && p.group_size > 1 ? ordered(unordered(a) + unordered(b)) : a;
+      if (e0 >= p.experts) mine = 0;
+    } else {
+      for (int g = 0; g < p.groups; ++g) {
+        const int lo = g * p.group_size, hi = lo + p.group_size;
+        uint32_t a = 0, b = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const uint32_t k = e0 + i >= lo && e0 + i < hi ? key[i] : 0u;
+          b = max(b, min(a, k)); a = max(a, k);
+        }
+        const uint32_t best = __reduce_max_sync(0xffffffffu, a);
+        uint32_t score = best;
+        if (p.bias && p.group_size > 1) {
+          const int owner = __ffs(__ballot_sync(0xffffffffu, a == best)) - 1;
+          const uint32_t second = __reduce_max_sync(0xffffffffu, lane == owner ? b : a);
+          score = ordered(unordered(best) + unordered(second));
+        }
+        if (lane == g) mine = score;
+      }
+    }
+    // lane g takes group g's score and counts the better ones
+    const int group_of_lane = whole ? e0 / p.group_size : lane;
+    if (whole) mine = __shfl_sync(0xffffffffu, mine, min(lane * lanes, 31));
+    if (lane >= p.groups) mine = 0;
+    int better = 0;
+    for (int g = 0; g < p.groups; ++g) {
+      const uint32_t other = __shfl_sync(0xffffffffu, mine, g);
+      better += other > mine || (other == mine && g < lane);
+    }
+    const bool keep = lane < p.groups && better < p.top_groups;
+    const uint32_t kept = __ballot_sync(0xffffffffu, keep);
+    if (p.bias && p.top_groups < p.groups) {     // the order of the kept ones does not matter
+      const uint32_t last = __reduce_min_sync(0xffffffffu, keep ? mine : 0xffffffffu), next = __reduce_max_sync(0xffffffffu, keep ? 0u : mine);
+      wide = close(unordered(last), unordered(next));
+    }
+    if (whole) {
+      if (!(kept >> group_of_lane & 1)) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) key[i] = 0;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (e0 + i < p.experts && !(kept >> ((e0 + i) / p.group_size) & 1)) key[i] = 0;
     }
   }
-  int id = 0;                                    // of rank `lane`
+  // The (top_k + 1)-th of the lanes' best scores bounds what can be chosen, or come next: usually a dozen experts, which go to one lane
+  // each and are ranked by counting the better ones.  More than 32 of them (many ties, top_k near 32): one by one.
+  int id = 0, rank = 0x7fffffff;
+  bool listed = false;
+  if (p.top_k < 16) {
+    uint32_t rest = key[0], cut = 0;
+#pragma unroll
+    for (int i = 1; i < NV; ++i) rest = max(rest, key[i]);
+    for (int n = 0; n <= p.top_k; ++n) {
+      cut = __reduce_max_sync(0xffffffffu, rest);
+      if (lane == __ffs(__ballot_sync(0xffffffffu, rest == cut)) - 1) rest = 0;
+    }
+    cut = max(cut, 1u);
+    int at = 0, total = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const unsigned in = __ballot_sync(0xffffffffu, key[i] >= cut);
+      at += __popc(in & ((1u << lane) - 1));
+      total += __popc(in);
+    }
+    if (total <= 32) {
+      uint2* list = s_list[threadIdx.x >> 5];
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (key[i] >= cut) list[at++] = make_uint2(key[i], e0 + i);      // in the order of the experts
+      __syncwarp();
+      const uint2 own = lane < total ? list[lane] : make_uint2(0, 0);
+      int better = 0;
+      uint32_t below = 0;                                                 // the best of those behind this one
+      for (int j = 0; j < total; ++j) {
+        const uint32_t other = __shfl_sync(0xffffffffu, own.x, j);
+        const bool ahead = other > own.x || (other == own.x && j < lane);
+        better += ahead;
+        below = max(below, ahead || j == lane ? 0u : other);
+      }
+      if (lane < total && better < p.top_k) {
+        id = own.y;
+        rank = better;
+        if (p.bias && below) wide |= close(unordered(own.x), unordered(below));
+      }
+    }
+    listed = total <= 32;
+  }
+  if (!listed) {
+    uint32_t prev = 0;
+    for (int n = 0; n <= p.top_k; ++n) {
+      uint32_t a = key[0];
+      int at = 0;
+#pragma unroll
+      for (int i = 1; i < NV; ++i)
+        if (key[i] > a) { a = key[i]; at = i; }
+      const uint32_t best = __reduce_max_sync(0xffffffffu, a);
+      if (n > 0 && p.bias && best) wide |= close(unordered(prev), unordered(best));
+      prev = best;
+      if (n == p.top_k) break;
+      const int owner = __ffs(__ballot_sync(0xffffffffu, a == best)) - 1;
+      const int e = __shfl_sync(0xffffffffu, e0 + at, owner);
+      if (lane == owner) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+          if (i == at) key[i] = 0;
+      }
+      if (lane == n) { id = e; rank = n; }
+    }
+  }
+  if (__any_sync(0xffffffffu, wide)) { route_wide<T, NV>(p, t); return; }
   float w = 0.f;
-  for (int n = 0; n < p.top_k; ++n) {
-    double a = 2 * RT_OUT;
-    int at = 0;
-    float xv = 0.f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (c[i] > a) { a = c[i]; at = i * 32 + lane; xv = x[i]; }
-    const double best = warp_max(a);
-    const int e = (int)__reduce_min_sync(0xffffffffu, a == best ? (unsigned)at : 0xffffffffu);
-    const float xe = __shfl_sync(0xffffffffu, xv, e & 31);
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (i * 32 + lane == e) c[i] = 2 * RT_OUT;
-    if (lane == n) {
-      id = e;
-      w = p.sigmoid ? 1.f / (1.f + expf(-xe)) : expf(xe - top) / sum;
-    }
+  if (rank < p.top_k) {
+    const float xv = sane(to_f32<T>(row[id]));
+    w = p.sigmoid ? __fdividef(1.f, 1.f + expf(-xv)) : __fdividef(expf(xv - top), sum);
   }
-  if (p.renormalize) w /= fmaxf(warp_sum(w), 1.1754943508222875e-38f);
-  if (lane < p.top_k) {
-    p.weights[t * p.top_k + lane] = w * p.scale;
-    p.ids[t * p.top_k + lane] = id;
+  if (p.renormalize) w = __fdividef(w, fmaxf(warp_sum(w), 1.1754943508222875e-38f));
+  if (rank < p.top_k) {
+    p.weights[t * p.top_k + rank] = w * p.scale;
+    p.ids[t * p.top_k + rank] = id;
   }
 }
 
@@ -153,6 +367,7 @@ int run_route(const RouteParams& p, cudaStream_t st) {
 
 template <typename T>
 int run_route_size(const RouteParams& p, cudaStream_t st) {
+  if (p.experts <= 32) return run_route<T, 1>(p, st);
   if (p.experts <= 64) return run_route<T, 2>(p, st);
   if (p.experts <= 128) return run_route<T, 4>(p, st);
   if (p.experts <= 256) return run_route<T, 8>(p, st);
@@ -189,7 +404,7 @@ extern "C" int kq_moe_route(const void* logits, int dtype, int64_t tokens, int64
   RouteParams p;
   p.logits = logits; p.stride_t = stride_t; p.tokens = tokens; p.experts = (int)experts; p.top_k = (int)top_k; p.sigmoid = sigmoid != 0;
   p.groups = (int)groups; p.top_groups = (int)top_groups; p.group_size = (int)(experts / groups); p.renormalize = renormalize != 0;
-  p.bias = bias; p.scale = scale; p.weights = weights; p.ids = ids;
+  p.bias = bias; p.scale = scale; p.bias_aligned = (uintptr_t)bias % 16 == 0; p.aligned = (uintptr_t)logits % 16 == 0 && stride_t * (dtype == KQ_F32 ? 4 : 2) % 16 == 0; p.weights = weights; p.ids = ids;
   cudaStream_t st = (cudaStream_t)stream;
   switch (dtype) {
     case KQ_F32: return run_route_size<float>(p, st);
