@@ -16,7 +16,7 @@ from __future__ import annotations
 
 import torch
 
-from . import ops
+from .ops import PAGED_ATTENTION, PLAN_PAGES, QK_NORM_ROPE, QK_NORM_ROPE_STORE
 
 
 def qk_norm_rope(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, num_heads: int, num_kv_heads: int, *,
@@ -30,7 +30,7 @@ def qk_norm_rope(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Ten
     `factor` multiplies the rotated values (the attention factor of scaled rotations).  With q_weight / k_weight [D] (float32 or
     qkv's type) the head is first divided by sqrt(mean of squares + eps) and multiplied by the weight.  fp32 throughout, one
     rounding at the end.  D: even, up to 512."""
-    return ops.qk_norm_rope(qkv, positions, inv_freq, num_heads, num_kv_heads, q_weight, k_weight, eps, interleaved, factor)
+    return QK_NORM_ROPE(qkv, positions, inv_freq, num_heads, num_kv_heads, q_weight, k_weight, eps, interleaved, factor)
 
 
 def qk_norm_rope_store(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, num_heads: int, k_cache: torch.Tensor,
@@ -40,7 +40,7 @@ def qk_norm_rope_store(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: tor
     """`qk_norm_rope` that returns the queries and writes the rotated keys and the values of token t into slot slots[t] of the caches
     (slot = page * page size + place; int32 or int64; a slot outside the cache, -1 for instance, is skipped).  Slots should be
     distinct: one that is named twice holds values of either token."""
-    return ops.qk_norm_rope_store(qkv, positions, inv_freq, num_heads, k_cache, v_cache, slots, q_weight, k_weight, eps, interleaved, factor)
+    return QK_NORM_ROPE_STORE(qkv, positions, inv_freq, num_heads, k_cache, v_cache, slots, q_weight, k_weight, eps, interleaved, factor)
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, *,
@@ -52,8 +52,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     token j of sequence b is place j % page size of page block_table[b, j // page size]; entries outside the cache count as absent.
     A sequence without visible tokens gives zeros (lse -inf).  The token's own key has to be in the cache
     (`qk_norm_rope_store` first) and counted in seq_lens.  D: a multiple of 16 up to 256; float32, float16 or bfloat16."""
-    out, lse = ops.paged_attention(q, k_cache, v_cache, block_table, seq_lens, q.shape[-1] ** -0.5 if scale is None else scale, window,
-                                   softcap, return_lse)
+    out, lse = PAGED_ATTENTION(q, k_cache, v_cache, block_table, seq_lens, q.shape[-1] ** -0.5 if scale is None else scale, window, softcap,
+                               return_lse)
     return (out, lse) if return_lse else out
 
 
@@ -67,4 +67,4 @@ def plan_pages(block_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: torc
     raised by the pages asked for; above len(free_pages) the list has run out and the tokens concerned have slot -1, as have
     tokens beyond the table's width and the padding behind the last of the num_tokens entries.  num_tokens must be at least
     the sum of new_lens."""
-    return ops.plan_pages(block_table, seq_lens, new_lens, free_pages, taken, page_size, num_tokens)
+    return PLAN_PAGES(block_table, seq_lens, new_lens, free_pages, taken, page_size, num_tokens)

@@ -19,6 +19,7 @@
 #include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/CUDAEvent.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
 
@@ -292,6 +293,12 @@ at::Tensor fused_moe_swiglu(const at::Tensor& X, const at::Tensor& W1, const at:
   return out;
 }
 
+// an output or scratch tensor without the dispatcher's part of at::empty: a decode step makes these calls in every layer, and the
+// host's time is most of a call's there
+at::Tensor new_cuda(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& like) {
+  return at::Tensor(at::detail::empty_cuda(sizes, type, like.device(), std::nullopt));
+}
+
 void no_gradient(const char* fn, std::initializer_list<const at::Tensor*> ts) {
   if (!at::GradMode::is_enabled()) return;
   for (const at::Tensor* t : ts) TORCH_CHECK(!t->defined() || !t->requires_grad(), fn, ": has no derivative, and an input requires one");
@@ -349,7 +356,7 @@ std::tuple<at::Tensor, at::Tensor> qk_norm_rope(const at::Tensor& qkv, const at:
   const RopeCall c = rope_checks(fn, qkv, positions, inv_freq, heads, kv, q_weight, k_weight);
   const int dt = kq_dtype_of(qkv.scalar_type(), fn);
   const c10::cuda::CUDAGuard guard(qkv.device());
-  at::Tensor q = at::empty({c.tokens, heads, c.d}, qkv.options()), k = at::empty({c.tokens, kv, c.d}, qkv.options());
+  at::Tensor q = new_cuda({c.tokens, heads, c.d}, qkv.scalar_type(), qkv), k = new_cuda({c.tokens, kv, c.d}, qkv.scalar_type(), qkv);
   TORCH_CHECK(kq_qk_norm_rope(qkv.data_ptr(), dt, c.tokens, qkv.stride(0), heads, kv, c.d, positions.data_ptr(), positions.scalar_type() == at::kLong,
                               inv_freq.data_ptr<float>(), 2 * inv_freq.size(0), interleaved, (float)factor, c.qw, c.kw, c.wdt, (float)eps,
                               q.data_ptr(), k.data_ptr(), nullptr, nullptr, nullptr, nullptr, 0, 0, 0,
@@ -372,7 +379,7 @@ at::Tensor qk_norm_rope_store(const at::Tensor& qkv, const at::Tensor& positions
   TORCH_CHECK(slots.dim() == 1 && slots.size(0) == c.tokens && slots.is_contiguous(), fn, ": slots must be contiguous, one per token");
   const int dt = kq_dtype_of(qkv.scalar_type(), fn);
   const c10::cuda::CUDAGuard guard(qkv.device());
-  at::Tensor q = at::empty({c.tokens, heads, c.d}, qkv.options());
+  at::Tensor q = new_cuda({c.tokens, heads, c.d}, qkv.scalar_type(), qkv);
   TORCH_CHECK(kq_qk_norm_rope(qkv.data_ptr(), dt, c.tokens, qkv.stride(0), heads, c.kv, c.d, positions.data_ptr(), positions.scalar_type() == at::kLong,
                               inv_freq.data_ptr<float>(), 2 * inv_freq.size(0), interleaved, (float)factor, c.qw, c.kw, c.wdt, (float)eps,
                               q.data_ptr(), k_cache.data_ptr(), k_cache.strides().data(), v_cache.data_ptr(), v_cache.strides().data(),
@@ -396,9 +403,10 @@ std::tuple<at::Tensor, at::Tensor> paged_attention(const at::Tensor& q, const at
   no_gradient(fn, {&q});
   const int dt = kq_dtype_of(q.scalar_type(), fn);
   const c10::cuda::CUDAGuard guard(q.device());
-  at::Tensor out = at::empty({b, h, d}, q.options()), norm = at::empty({lse ? b : 0, h}, q.options().dtype(at::kFloat));
+  at::Tensor out = new_cuda({b, h, d}, q.scalar_type(), q), norm;
+  if (lse) norm = new_cuda({b, h}, at::kFloat, q);
   const size_t ws = kq_paged_attention_workspace_bytes(d);
-  at::Tensor scratch = at::empty({(int64_t)ws}, q.options().dtype(at::kByte));
+  at::Tensor scratch = new_cuda({(int64_t)ws}, at::kByte, q);
   TORCH_CHECK(kq_paged_attention(q.data_ptr(), dt, b, h, k_cache.size(2), d, q.stride(0), q.stride(1), k_cache.data_ptr(), k_cache.strides().data(),
                                  v_cache.data_ptr(), v_cache.strides().data(), k_cache.size(0), k_cache.size(1), block_table.data_ptr<int32_t>(),
                                  block_table.stride(0), block_table.size(1), seq_lens.data_ptr<int32_t>(), (float)scale, window, (float)softcap,
@@ -423,12 +431,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> plan_page
   TORCH_CHECK(seq_lens.size(0) == r && new_lens.size(0) == r && taken.size(0) == 1, fn, ": one length per row of block_table, and one value in taken");
   TORCH_CHECK(num_tokens >= 0 && page_size > 0, fn, ": page_size must be positive and num_tokens not negative");
   const c10::cuda::CUDAGuard guard(block_table.device());
-  const auto opt = block_table.options();
-  // one allocation for the four int32 results, the 8-byte slots in front
-  at::Tensor slots = at::empty({num_tokens}, opt.dtype(at::kLong));
-  at::Tensor rest = at::empty({r + (r + 1) + num_tokens + 1}, opt);
-  at::Tensor total = rest.narrow(0, 0, r), starts = rest.narrow(0, r, r + 1), positions = rest.narrow(0, 2 * r + 1, num_tokens),
-             after = rest.narrow(0, 2 * r + 1 + num_tokens, 1);
+  at::Tensor total = new_cuda({r}, at::kInt, block_table), starts = new_cuda({r + 1}, at::kInt, block_table),
+             positions = new_cuda({num_tokens}, at::kInt, block_table), slots = new_cuda({num_tokens}, at::kLong, block_table),
+             after = new_cuda({1}, at::kInt, block_table);
   TORCH_CHECK(kq_plan_pages(block_table.data_ptr<int32_t>(), block_table.stride(0), block_table.size(1), seq_lens.data_ptr<int32_t>(), new_lens.data_ptr<int32_t>(), r,
                             free_pages.data_ptr<int32_t>(), free_pages.size(0), taken.data_ptr<int32_t>(), page_size, num_tokens,
                             total.data_ptr<int32_t>(), starts.data_ptr<int32_t>(), positions.data_ptr<int32_t>(), slots.data_ptr<int64_t>(),
@@ -451,7 +456,7 @@ std::tuple<at::Tensor, at::Tensor> moe_route(const at::Tensor& logits, int64_t t
   no_gradient(fn, {&logits, &bias});
   TORCH_CHECK(top_k > 0 && top_k <= e, fn, ": top_k=", top_k, " is not between 1 and ", e);
   const c10::cuda::CUDAGuard guard(logits.device());
-  at::Tensor w = at::empty({t, top_k}, logits.options().dtype(at::kFloat)), ids = at::empty({t, top_k}, logits.options().dtype(at::kInt));
+  at::Tensor w = new_cuda({t, top_k}, at::kFloat, logits), ids = new_cuda({t, top_k}, at::kInt, logits);
   TORCH_CHECK(kq_moe_route(logits.data_ptr(), dt, t, e, logits.stride(0), top_k, sigmoid, bias.defined() ? bias.data_ptr<float>() : nullptr, groups, top_groups,
                            renormalize, (float)scale, w.data_ptr<float>(), ids.data_ptr<int32_t>(),
                            (void*)at::cuda::getCurrentCUDAStream(logits.get_device()).stream()) == KQ_OK, fn, ": ", kq_last_error());

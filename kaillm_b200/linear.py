@@ -145,7 +145,7 @@ def route_experts(router_logits: torch.Tensor, top_k: int, *, scoring: str = "so
     NaN counts as -inf; masked experts (-inf) come last with weight 0.  At most 1024 experts, top_k 32, 32 groups; no gradient."""
     if scoring not in ("softmax", "sigmoid"):
         raise ValueError(f"scoring must be 'softmax' or 'sigmoid', got {scoring!r}")
-    return ops.moe_route(router_logits, top_k, scoring == "sigmoid", bias, groups, top_groups, renormalize, scale)
+    return ops.MOE_ROUTE(router_logits, top_k, scoring == "sigmoid", bias, groups, top_groups, renormalize, scale)
 
 
 def moe_align_block_size(topk_ids: torch.Tensor, block_size: int, num_experts: int):

@@ -86,41 +86,42 @@ def fused_moe_swiglu(X: torch.Tensor, W1: torch.Tensor, W2: torch.Tensor, topk_w
     return torch.ops._C_gguf.fused_moe_swiglu(X, W1, W2, topk_weights, topk_ids, quant_type, quant_type2, block)
 
 
+# The overloads of the operators that a decode step calls in every layer; looking one up, and each Python function around it, costs as
+# much as a tenth of the call, so `attention` and `linear` call these
+QK_NORM_ROPE = torch.ops._C_gguf.qk_norm_rope.default
+QK_NORM_ROPE_STORE = torch.ops._C_gguf.qk_norm_rope_store.default
+PAGED_ATTENTION = torch.ops._C_gguf.paged_attention.default
+PLAN_PAGES = torch.ops._C_gguf.plan_pages.default
+MOE_ROUTE = torch.ops._C_gguf.moe_route.default
+
+
 def qk_norm_rope(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, num_heads: int, num_kv_heads: int,
                  q_weight: torch.Tensor | None, k_weight: torch.Tensor | None, eps: float, interleaved: bool,
                  factor: float) -> tuple[torch.Tensor, torch.Tensor]:
     """`attention.qk_norm_rope` (no gradient)."""
-    return _QK_NORM_ROPE(qkv, positions, inv_freq, num_heads, num_kv_heads, q_weight, k_weight, eps, interleaved, factor)
+    return QK_NORM_ROPE(qkv, positions, inv_freq, num_heads, num_kv_heads, q_weight, k_weight, eps, interleaved, factor)
 
 
 def qk_norm_rope_store(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, num_heads: int, k_cache: torch.Tensor,
                        v_cache: torch.Tensor, slots: torch.Tensor, q_weight: torch.Tensor | None, k_weight: torch.Tensor | None,
                        eps: float, interleaved: bool, factor: float) -> torch.Tensor:
     """`attention.qk_norm_rope_store` (no gradient)."""
-    return _QK_NORM_ROPE_STORE(qkv, positions, inv_freq, num_heads, k_cache, v_cache, slots, q_weight, k_weight, eps, interleaved, factor)
+    return QK_NORM_ROPE_STORE(qkv, positions, inv_freq, num_heads, k_cache, v_cache, slots, q_weight, k_weight, eps, interleaved, factor)
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
-                    scale: float, window: int, softcap: float, lse: bool) -> tuple[torch.Tensor, torch.Tensor]:
-    """`attention.paged_attention` (no gradient): the output and, if asked for, the log of the sum of exponentials (else empty)."""
-    return _PAGED_ATTENTION(q, k_cache, v_cache, block_table, seq_lens, scale, window, softcap, lse)
+                    scale: float, window: int, softcap: float, lse: bool) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """`attention.paged_attention` (no gradient): the output and, if asked for, the log of the sum of exponentials (else None)."""
+    return PAGED_ATTENTION(q, k_cache, v_cache, block_table, seq_lens, scale, window, softcap, lse)
 
 
 def plan_pages(block_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: torch.Tensor, taken: torch.Tensor,
                page_size: int, num_tokens: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """`attention.plan_pages`."""
-    return _PLAN_PAGES(block_table, seq_lens, new_lens, free_pages, taken, page_size, num_tokens)
+    return PLAN_PAGES(block_table, seq_lens, new_lens, free_pages, taken, page_size, num_tokens)
 
 
 def moe_route(logits: torch.Tensor, top_k: int, sigmoid: bool, bias: torch.Tensor | None, groups: int, top_groups: int, renormalize: bool,
               scale: float) -> tuple[torch.Tensor, torch.Tensor]:
     """`linear.route_experts` (no gradient): weights and ids."""
-    return _MOE_ROUTE(logits, top_k, sigmoid, bias, groups, top_groups, renormalize, scale)
-
-
-# the overloads themselves: a decode step makes these calls in every layer, and looking one up costs about as much as its launch
-_QK_NORM_ROPE = torch.ops._C_gguf.qk_norm_rope.default
-_QK_NORM_ROPE_STORE = torch.ops._C_gguf.qk_norm_rope_store.default
-_PAGED_ATTENTION = torch.ops._C_gguf.paged_attention.default
-_PLAN_PAGES = torch.ops._C_gguf.plan_pages.default
-_MOE_ROUTE = torch.ops._C_gguf.moe_route.default
+    return MOE_ROUTE(logits, top_k, sigmoid, bias, groups, top_groups, renormalize, scale)
