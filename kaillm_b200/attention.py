@@ -1,7 +1,7 @@
 """What a decode step runs between the q/k/v projection and the output projection, over a paged key-value cache.
 
-The reference leaves this part to vLLM, whose model code calls its linear method; here it is what `sharded.DecoderStack` calls
-between its projections:
+The reference leaves this part to vLLM, whose model code calls its linear method; here it is what `sharded.DecoderStack` runs
+between its projections when it is given a `StepAttention`:
 
     total, starts, positions, slots, taken = plan_pages(block_table, seq_lens, new_lens, free_pages, taken, page_size, tokens)
     q = qk_norm_rope_store(qkv, positions, inv_freq, heads, k_cache, v_cache, slots, q_weight=..., k_weight=...)   # every layer
@@ -68,3 +68,44 @@ def plan_pages(block_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: torc
     tokens beyond the table's width and the padding behind the last of the num_tokens entries.  num_tokens must be at least
     the sum of new_lens."""
     return PLAN_PAGES(block_table, seq_lens, new_lens, free_pages, taken, page_size, num_tokens)
+
+
+class StepAttention:
+    """The attention of a decode step of `sharded.DecoderStack`: one new token for each of m sequences over paged caches.
+
+    caches: per layer a pair (k_cache, v_cache) [pages, page size, kv heads, head dim].  block_table int32 [m, pages per sequence],
+    seq_lens int32 [m] (tokens in the caches), free_pages int32 and taken int32 [1] are the program's own tensors; every step moves
+    them on in place, so a captured step does so at each replay.  q_weights / k_weights: per layer the norm weights of queries and
+    keys, or None.  The other arguments are those of `qk_norm_rope_store` and `paged_attention`."""
+
+    def __init__(self, caches, num_heads: int, inv_freq: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                 free_pages: torch.Tensor, taken: torch.Tensor, *, q_weights=None, k_weights=None, eps: float = 1e-6,
+                 interleaved: bool = False, factor: float = 1.0, scale: float | None = None, window: int = 0, softcap: float = 0.0):
+        self.caches = [tuple(pair) for pair in caches]
+        if not self.caches or any(k.shape != self.caches[0][0].shape or v.shape != k.shape for k, v in self.caches):
+            raise ValueError("caches must be pairs of tensors of one shape, one pair per layer")
+        for name, w in (("q_weights", q_weights), ("k_weights", k_weights)):
+            if w is not None and len(w) != len(self.caches):
+                raise ValueError(f"{name} must hold one tensor per layer")
+        self.num_heads, self.inv_freq = num_heads, inv_freq
+        self.page_size, self.num_kv_heads, self.head_dim = self.caches[0][0].shape[1:]
+        self.block_table, self.seq_lens, self.free_pages, self.taken = block_table, seq_lens, free_pages, taken
+        self.q_weights, self.k_weights = (w if w is not None else [None] * len(self.caches) for w in (q_weights, k_weights))
+        self.eps, self.interleaved, self.factor, self.scale, self.window, self.softcap = eps, interleaved, factor, scale, window, softcap
+        self.one_each = torch.ones_like(seq_lens)
+        self.positions = self.slots = None
+
+    def begin_step(self) -> None:
+        """Room for one more token of every sequence; seq_lens counts it from here on."""
+        total, _, self.positions, self.slots, taken = plan_pages(self.block_table, self.seq_lens, self.one_each, self.free_pages, self.taken,
+                                                                 self.page_size, self.seq_lens.shape[0])
+        self.seq_lens.copy_(total)
+        self.taken.copy_(taken)
+
+    def layer(self, index: int, qkv: torch.Tensor) -> torch.Tensor:
+        """The attention output [m, num_heads * head dim] of layer `index` for this step's merged projection."""
+        k_cache, v_cache = self.caches[index]
+        q = qk_norm_rope_store(qkv, self.positions, self.inv_freq, self.num_heads, k_cache, v_cache, self.slots, q_weight=self.q_weights[index],
+                               k_weight=self.k_weights[index], eps=self.eps, interleaved=self.interleaved, factor=self.factor)
+        out = paged_attention(q, k_cache, v_cache, self.block_table, self.seq_lens, scale=self.scale, window=self.window, softcap=self.softcap)
+        return out.flatten(1)

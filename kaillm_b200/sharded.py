@@ -174,10 +174,10 @@ class ShardedGGUFLinear:
 class DecoderStack:
     """The linear layers of a decoder stack, row-sharded, chained through the fused activation producers.
 
-    Per layer, in the order a transformer runs them (attention itself is not part of this path and is left out):
+    Per layer, in the order a transformer runs them:
 
         h  -> RMSNorm -> q8_1 -> merged q/k/v projection  [M, 8192]   -> all-gather
-           -> q8_1 of the first `hidden` columns -> o projection [M, hidden] -> all-gather
+           -> attention -> q8_1 -> o projection [M, hidden] -> all-gather
            -> RMSNorm -> q8_1 -> merged gate/up projection [M, 2*ffn] -> all-gather
            -> silu(gate) * up -> q8_1 -> down projection [M, hidden]  -> all-gather -> h of the next layer
 
@@ -189,13 +189,15 @@ class DecoderStack:
     cover cost a separate gather launch.
 
     weights: per layer a dict {"qkv", "o", "gate_up", "down"} -> (local shard uint8 [N/world, rowbytes], type, N, K).
+    attention: an `attention.StepAttention` for M sequences, each pass then is one decode step (one GPU only: the caches are not
+    sharded).  Without it the first `hidden` columns of q/k/v stand in for the attention output.
     """
 
     GROUPS = ("qkv", "o", "gate_up", "down")
 
     def __init__(self, weights: list[dict], m: int, hidden: int, device: torch.device, p2p: "P2PGather | None" = None,
                  group=None, eps: float = 1e-6, dtype: torch.dtype = torch.bfloat16, wait_in_consumer: bool = True,
-                 unsharded: bool = False):
+                 unsharded: bool = False, attention=None):
         """`unsharded`: the weights are whole tensors and this process runs the stack alone, whatever process group
         exists (a single-GPU baseline inside a multi-rank job)."""
         from . import capi
@@ -207,6 +209,15 @@ class DecoderStack:
         self.group = group
         self.p2p = p2p
         self.dev = device
+        self.attention = attention
+        if attention is not None:
+            heads, kv, d = attention.num_heads, attention.num_kv_heads, attention.head_dim
+            if self.world > 1:
+                raise ValueError("a sharded stack takes no attention: the caches are not sharded")
+            if len(attention.caches) != len(weights) or attention.seq_lens.shape[0] != m:
+                raise ValueError(f"attention is for {len(attention.caches)} layers and {attention.seq_lens.shape[0]} sequences, the stack has {len(weights)} and {m}")
+            if weights[0]["qkv"][2] != (heads + 2 * kv) * d or weights[0]["o"][3] != heads * d:
+                raise ValueError(f"{heads} query and {kv} key and value heads of {d} do not match the q/k/v and o projections")
         # gathers without a hand-shake: the next producer polls the gathered values against the arrival sentinel
         self.wait_in_consumer = bool(wait_in_consumer) and p2p is not None
         self.gamma = torch.ones(hidden, dtype=dtype, device=device)
@@ -270,6 +281,8 @@ class DecoderStack:
         capi = self._capi
         m, hid = self.m, self.hidden
         wa = self.wait_in_consumer
+        if self.attention is not None:
+            self.attention.begin_step()
 
         def seen(name, buf):      # the hook reads the buffer with ordinary kernels: everything must have arrived
             if on_output:
@@ -288,7 +301,8 @@ class DecoderStack:
             qkv = self._project("qkv", W, qt, n, k)
             if seen("qkv", qkv): on_output(li, "qkv", qkv, prep)
             W, qt, n, k = layer["o"]
-            a = qkv[:, :hid]                                   # stands in for the attention output: [M, hidden], row stride 8192
+            # without attention the first columns stand in for its output: [M, hidden], row stride 8192
+            a = qkv[:, :hid] if self.attention is None else self.attention.layer(li, qkv)
             prep = lambda s, n_=n, qt_=qt, a_=keep(a): capi.prepare_q8(a_, qt_, n_, s)   # noqa: E731
             capi.prepare_q8(a, qt, n // self.world, self.scratch, wait_arrival=wa)
             o = self._project("o", W, qt, n, k)

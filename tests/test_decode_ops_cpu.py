@@ -92,3 +92,24 @@ def test_plain_forms():
     assert ids.tolist() == [[1, 0]] and w.sum() == pytest.approx(1.0)
     t, total, starts, pos, slots, taken = pages([[3, -1]], [7], [3], [9, 4], 1, 8, 4)
     assert (t, total, starts, pos, slots, taken) == ([[3, 4]], [10], [0, 3], [7, 8, 9, 0], [31, 32, 33, -1], 2)
+
+
+def test_a_stack_refuses_attention_that_does_not_fit():
+    from kaillm_b200 import sharded
+    from kaillm_b200.attention import StepAttention
+
+    def att(layers=1, seqs=2, heads=4, kv=2, d=16):
+        i32 = lambda *s: torch.zeros(s, dtype=torch.int32)    # noqa: E731
+        return StepAttention([[torch.zeros(3, 8, kv, d)] * 2] * layers, heads, torch.ones(d // 2), i32(seqs, 2), i32(seqs), i32(3), i32(1))
+
+    w = {name: (torch.zeros((n, k // 32 * 34), dtype=torch.uint8), 8, n, k) for name, (n, k) in
+         {"qkv": (128, 64), "o": (64, 64), "gate_up": (128, 64), "down": (64, 64)}.items()}
+    make = lambda a: sharded.DecoderStack([w], 2, 64, torch.device("cpu"), attention=a)    # noqa: E731
+    assert make(att()).attention is not None and make(None).attention is None
+    for bad in (att(layers=2), att(seqs=3), att(heads=8), att(kv=1), att(d=32)):
+        with pytest.raises(ValueError):
+            make(bad)
+    with pytest.raises(ValueError):
+        StepAttention([], 4, torch.ones(8), torch.zeros(1, 1), torch.zeros(1), torch.zeros(1), torch.zeros(1))
+    with pytest.raises(ValueError):
+        StepAttention([[torch.zeros(3, 8, 2, 16)] * 2], 4, torch.ones(8), torch.zeros(1, 1), torch.zeros(1), torch.zeros(1), torch.zeros(1), q_weights=[])
