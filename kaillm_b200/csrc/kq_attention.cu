@@ -201,45 +201,52 @@ template <typename T> struct RowOut {
   }
 };
 
-// Adds the partial results of the item that starts in share c and ends in share meta.y: a warp takes every fourth of them, the four
-// sums are added in order.
+// Adds the partial results of the item that starts in share blockIdx.x and ends in share meta.y, for one row, in the order of the keys.
 template <typename T>
-__global__ void __launch_bounds__(128) attend_join_kernel(const AttnParams p) {
-  __shared__ float s_o[4][256];
-  __shared__ float s_l[4];
+__global__ void __launch_bounds__(64) attend_join_kernel(const AttnParams p) {
   pdl_trigger();
   pdl_wait();
-  const int c = blockIdx.x, r = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int c = blockIdx.x, r = blockIdx.y;
   const int2 it = p.meta[c];
   if (it.x < 0) return;
   const int per = p.kv_heads * p.row_tiles;
   const int b = it.x / per, sub = it.x - b * per, h = sub / p.row_tiles, x = sub - h * p.row_tiles;
   const int head0 = h * p.group + x * p.rows;
   if (r >= min(p.rows, p.group - x * p.rows)) return;
-  auto at = [&](int i) { return (int64_t)(2 * i + (i == c)) * p.rows + r; };
-  float m = -INFINITY;
-  for (int i = c + lane; i <= it.y; i += 32) m = fmaxf(m, p.part_ml[at(i)].x);
+  for (int d0 = 0; d0 < p.dim; d0 += 128) {
+    const int d = d0 + threadIdx.x * 2;
+    const bool in = d < p.dim;
+    const float2* ml0 = p.part_ml + r;
+    const float* o0 = p.part_o + (int64_t)r * p.dim + (in ? d : 0);
+    float m = -INFINITY, l = 0.f;
+    float2 o = make_float2(0.f, 0.f);
+    // maxima, sums and values are loaded together, eight parts at a time: the chain is two loads long
+    for (int i0 = c; i0 <= it.y; i0 += 8) {
+      float2 ml[8], v[8];
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-  const float use = m == -INFINITY ? 0.f : m;
-  float l = 0.f, o[8] = {};
-#pragma unroll 4
-  for (int i = c + warp; i <= it.y; i += 4) {
-    const float2 ml = p.part_ml[at(i)];
-    const float f = ex2(ml.x - use);
-    const float* src = p.part_o + at(i) * p.dim;
-    l += ml.y * f;
+      for (int k = 0; k < 8; ++k) {
+        const int i = min(i0 + k, it.y), at = (2 * i + (i == c)) * p.rows;      // the first part is in slot 2 c + 1, the others in 2 i
+        ml[k] = ml0[at];
+        v[k] = *reinterpret_cast<const float2*>(o0 + (int64_t)at * p.dim);
+      }
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (e * 32 + lane < p.dim) o[e] += src[e * 32 + lane] * f;
+      for (int k = 0; k < 8; ++k) {
+        if (i0 + k <= it.y) {
+          const float mn = fmaxf(m, ml[k].x), use = mn == -INFINITY ? 0.f : mn;
+          const float f = ex2(m - use), g = ex2(ml[k].x - use);
+          m = mn;
+          l = l * f + ml[k].y * g;
+          o.x = o.x * f + v[k].x * g;
+          o.y = o.y * f + v[k].y * g;
+        }
+      }
+    }
+    if (in) {
+      const RowOut<T> out(p, -1, b, head0 + r, r, m, l, d == 0);
+      out.put(d, o.x);
+      out.put(d + 1, o.y);
+    }
   }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) s_o[warp][e * 32 + lane] = o[e];
-  if (lane == 0) s_l[warp] = l;
-  __syncthreads();
-  l = s_l[0] + s_l[1] + s_l[2] + s_l[3];
-  const RowOut<T> out(p, -1, b, head0 + r, r, m, l, threadIdx.x == 0);
-  for (int d = threadIdx.x; d < p.dim; d += 128) out.put(d, s_o[0][d] + s_o[1][d] + s_o[2][d] + s_o[3][d]);
 }
 
 // Where key j of sequence b lies: page name and place inside the page; false where there is no such page.
@@ -803,7 +810,7 @@ int launch_both(void (*kern)(const AttnParams), AttnParams& p, int threads, int 
   KQ_CUDA_TRY(launch_pdl(kern, dim3(grid), dim3(threads), (size_t)smem, st, pdl, p));
   options().launches += 1;
   if (p.split) {
-    KQ_CUDA_TRY(launch_pdl(attend_join_kernel<T>, dim3(grid, (unsigned)p.rows), dim3(128), (size_t)0, st, pdl, p));
+    KQ_CUDA_TRY(launch_pdl(attend_join_kernel<T>, dim3(grid, (unsigned)p.rows), dim3(64), (size_t)0, st, pdl, p));
     options().launches += 1;
   }
   return KQ_OK;
