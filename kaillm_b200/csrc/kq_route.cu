@@ -5,9 +5,9 @@
 //   ids = the top_k experts by c, descending, ties to the lowest index;  w = p[ids] (/ sum) * scale
 //
 // A warp per token, NV experts next to each other per lane.  Without a bias the choice compares the logits themselves.  With one, two of
-// a few hundred scores lie closer than fp32 tells apart once in some thousand tokens, and a router's choice should not depend on the
-// last bit of an exponential: a token whose chosen scores (or group scores) come within RT_CLOSE of one another, or of the first one
-// left out, is routed again in fp64 (route_wide).
+// a few hundred scores lie closer than fp32 tells apart once in some hundred tokens, and a router's choice should not depend on the
+// last bit of an exponential: candidates of a sigmoid whose scores come within RT_CLOSE of one another are ranked again in fp64; where
+// it is the groups' scores, or a softmax, the whole token is routed again in fp64 (route_wide).
 //
 // Bound by instructions, about 500 per token (17 MB and 2.7 us of memory for 16384 x 256 fp32 logits): the best of 32 lanes is one
 // redux.sync on order-preserving integers, and where whole lanes make up a group all groups are scored at once.
@@ -53,7 +53,8 @@ __device__ __forceinline__ unsigned long long warp_max64(unsigned long long v) {
   return (unsigned long long)hi << 32 | lo;
 }
 
-// A token whose choice fp32 cannot make, with a bias: scores, groups and choice in fp64; NV experts next to each other per lane.
+// A token whose choice the kernels below leave open (scores too close for fp32, too many ties): scores, groups and choice in fp64; NV
+// experts next to each other per lane.
 template <typename T, int NV>
 __device__ __noinline__ void route_wide(const RouteParams& p, int64_t t) {
   const int lane = threadIdx.x & 31, e0 = lane * NV;
@@ -81,7 +82,8 @@ __device__ __noinline__ void route_wide(const RouteParams& p, int64_t t) {
   unsigned long long key[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i)
-    key[i] = e0 + i < p.experts ? ordered64((p.sigmoid ? 1. / (1. + c[i]) : c[i] / sum) + (double)sane(p.bias[e0 + i])) : RT_TAKEN;
+    key[i] = e0 + i >= p.experts ? RT_TAKEN
+             : p.bias ? ordered64((p.sigmoid ? 1. / (1. + c[i]) : c[i] / sum) + (double)sane(p.bias[e0 + i])) : ordered64((double)x[i]);
   if (p.groups > 1) {
     unsigned long long mine = RT_TAKEN;          // score of group `lane`
     for (int g = 0; g < p.groups; ++g) {
@@ -94,7 +96,7 @@ __device__ __noinline__ void route_wide(const RouteParams& p, int64_t t) {
       }
       const unsigned long long best = warp_max64(a);
       unsigned long long score = best;
-      if (p.group_size > 1) {
+      if (p.bias && p.group_size > 1) {
         const int owner = __ffs(__ballot_sync(0xffffffffu, a == best)) - 1;
         score = ordered64(unordered64(best) + unordered64(warp_max64(lane == owner ? b : a)));
       }
@@ -154,8 +156,26 @@ __device__ __forceinline__ float fast_exp(float x) {        // relative error 2^
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
   return y;
 }
+__device__ __forceinline__ float fast_rcp(float x) {        // relative error 2^-23; 0 from 2^126 on
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
-template <typename T, int NV>
+// what a candidate must reach so that none is missed whose fp64 score is above that of key `cut`
+__device__ __forceinline__ uint32_t below_cut(const RouteParams& p, uint32_t cut) {
+  if (cut == 0) return 1;
+  const float c = unordered(cut);
+  return p.bias ? max(1u, ordered(c - RT_CLOSE * fmaxf(1.f, fabsf(c)))) : cut;
+}
+// a candidate's score in fp64 (sigmoid)
+template <typename T>
+__device__ __forceinline__ double score64(const RouteParams& p, const T* row, int e) {
+  return 1. / (1. + exp(-(double)sane(to_f32<T>(row[e])))) + (double)sane(p.bias[e]);
+}
+
+// FULL: 32 x NV experts, in rows (and with a bias) that take vector loads
+template <typename T, int NV, bool FULL>
 __global__ void __launch_bounds__(RT_WARPS * 32) route_kernel(const RouteParams p) {
   const int lane = threadIdx.x & 31;
   const int64_t t = (int64_t)blockIdx.x * RT_WARPS + (threadIdx.x >> 5);
@@ -167,18 +187,18 @@ __global__ void __launch_bounds__(RT_WARPS * 32) route_kernel(const RouteParams 
   __shared__ uint2 s_list[RT_WARPS][32];
   float x[NV];
   constexpr int VEC = NV * (int)sizeof(T) >= 16 ? 16 / (int)sizeof(T) : NV;      // values of one load
-  if (p.aligned && (p.experts % NV == 0)) {
+  if (FULL || (p.aligned && (p.experts % NV == 0))) {
 #pragma unroll
     for (int i = 0; i < NV; i += VEC) {
       alignas(16) T v[VEC];
-      if (e0 < p.experts) {
+      if (FULL || e0 < p.experts) {
         if constexpr (VEC * sizeof(T) == 16) *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(row + e0 + i);
         else if constexpr (VEC * sizeof(T) == 8) *reinterpret_cast<uint2*>(v) = *reinterpret_cast<const uint2*>(row + e0 + i);
         else if constexpr (VEC * sizeof(T) == 4) *reinterpret_cast<uint32_t*>(v) = *reinterpret_cast<const uint32_t*>(row + e0 + i);
         else v[0] = row[e0];
       }
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) x[i + j] = e0 < p.experts ? sane(to_f32<T>(v[j])) : -INFINITY;
+      for (int j = 0; j < VEC; ++j) x[i + j] = FULL || e0 < p.experts ? sane(to_f32<T>(v[j])) : -INFINITY;
     }
   } else {
 #pragma unroll
@@ -201,22 +221,22 @@ __global__ void __launch_bounds__(RT_WARPS * 32) route_kernel(const RouteParams 
   if (p.bias) {
     const float inv = p.sigmoid ? 1.f : 1.f / sum;
     float bias[NV];
-    if (NV % 4 == 0 && p.bias_aligned && p.experts % NV == 0) {
+    if (NV % 4 == 0 && (FULL || (p.bias_aligned && p.experts % NV == 0))) {
 #pragma unroll
       for (int i = 0; i < NV; i += 4)
-        if (e0 < p.experts) *reinterpret_cast<float4*>(bias + i) = *reinterpret_cast<const float4*>(p.bias + e0 + i);
+        if (FULL || e0 < p.experts) *reinterpret_cast<float4*>(bias + i) = *reinterpret_cast<const float4*>(p.bias + e0 + i);
     } else {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) bias[i] = e0 + i < p.experts ? p.bias[e0 + i] : 0.f;
+      for (int i = 0; i < NV; ++i) bias[i] = FULL || e0 + i < p.experts ? p.bias[e0 + i] : 0.f;
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const float pr = p.sigmoid ? __fdividef(1.f, 1.f + fast_exp(-x[i])) : fast_exp(x[i] - top) * inv;
-      key[i] = e0 + i < p.experts ? ordered(pr + sane(bias[i])) : 0u;
+      const float pr = p.sigmoid ? fast_rcp(1.f + fast_exp(-x[i])) : fast_exp(x[i] - top) * inv;
+      key[i] = FULL || e0 + i < p.experts ? ordered(pr + sane(bias[i])) : 0u;
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) key[i] = e0 + i < p.experts ? ordered(x[i]) : 0u;
+    for (int i = 0; i < NV; ++i) key[i] = FULL || e0 + i < p.experts ? ordered(x[i]) : 0u;
   }
   bool wide = false;                             // too close to call
   if (p.groups > 1) {
@@ -234,7 +254,7 @@ __global__ void __launch_bounds__(RT_WARPS * 32) route_kernel(const RouteParams 
         a = max(a, oa);
       }
       mine = p.bias && p.group_size > 1 ? ordered(unordered(a) + unordered(b)) : a;
-      if (e0 >= p.experts) mine = 0;
+      if (!FULL && e0 >= p.experts) mine = 0;
     } else {
       for (int g = 0; g < p.groups; ++g) {
         const int lo = g * p.group_size, hi = lo + p.group_size;
@@ -292,7 +312,7 @@ __global__ void __launch_bounds__(RT_WARPS * 32) route_kernel(const RouteParams 
       cut = __reduce_max_sync(0xffffffffu, rest);
       if (lane == __ffs(__ballot_sync(0xffffffffu, rest == cut)) - 1) rest = 0;
     }
-    cut = max(cut, 1u);
+    cut = below_cut(p, cut);
     int at = 0, total = 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -315,11 +335,21 @@ __global__ void __launch_bounds__(RT_WARPS * 32) route_kernel(const RouteParams 
         better += ahead;
         below = max(below, ahead || j == lane ? 0u : other);
       }
-      if (lane < total && better < p.top_k) {
-        id = own.y;
-        rank = better;
-        if (p.bias && below) wide |= close(unordered(own.x), unordered(below));
+      const bool open = p.bias && lane < total && better < p.top_k && below && close(unordered(own.x), unordered(below));
+      if (__any_sync(0xffffffffu, open)) {
+        if (p.sigmoid) {
+          const unsigned long long mine = lane < total ? ordered64(score64<T>(p, row, own.y)) : 0;
+          better = 0;
+#pragma unroll 4
+          for (int j = 0; j < total; ++j) {
+            const unsigned long long other = __shfl_sync(0xffffffffu, mine, j);
+            better += other > mine || (other == mine && j < lane);
+          }
+        } else {
+          wide = true;
+        }
       }
+      if (lane < total && better < p.top_k) { id = own.y; rank = better; }
     }
     listed = total <= 32;
   }
@@ -360,7 +390,9 @@ __global__ void __launch_bounds__(RT_WARPS * 32) route_kernel(const RouteParams 
 
 template <typename T, int NV>
 int run_route(const RouteParams& p, cudaStream_t st) {
-  KQ_CUDA_TRY(launch_pdl(route_kernel<T, NV>, dim3((unsigned)((p.tokens + RT_WARPS - 1) / RT_WARPS)), dim3(RT_WARPS * 32), (size_t)0, st, options().pdl != 0, p));
+  const bool full = p.experts == 32 * NV && p.aligned && (!p.bias || p.bias_aligned);
+  KQ_CUDA_TRY(launch_pdl(full ? route_kernel<T, NV, true> : route_kernel<T, NV, false>, dim3((unsigned)((p.tokens + RT_WARPS - 1) / RT_WARPS)), dim3(RT_WARPS * 32),
+                         (size_t)0, st, options().pdl != 0, p));
   options().launches += 1;
   return KQ_OK;
 }
