@@ -352,9 +352,9 @@ int kq_qk_norm_rope(const void* qkv, int dtype, int64_t tokens, int64_t stride_t
  * q: [batch, heads, head_dim] with strides q_stride_batch, q_stride_head, head_dim dense; out: dense; lse: [batch, heads] fp32 log
  * of the sum of exponentials, or NULL.  q, caches and out have one dtype; scores, softmax and sums are fp32.  head_dim: a
  * multiple of 16 up to 256 (KQ_EUNSUPPORTED otherwise); caches and their strides 16-byte aligned.
- * scratch: kq_paged_attention_workspace_bytes(head_dim) bytes on the current device, 256-byte aligned, not initialised; calls
- * that may overlap need one each. */
-size_t kq_paged_attention_workspace_bytes(int64_t head_dim);
+ * scratch: kq_paged_attention_workspace_bytes(...) bytes for the current device (0 for sizes that are not served), 256-byte aligned,
+ * not initialised; calls that may overlap need one each. */
+size_t kq_paged_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim);
 int kq_paged_attention(const void* q, int dtype, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
                        int64_t q_stride_batch, int64_t q_stride_head, const void* k_cache, const int64_t* k_strides,
                        const void* v_cache, const int64_t* v_strides, int64_t num_pages, int64_t page_size,

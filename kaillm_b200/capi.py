@@ -80,7 +80,7 @@ def _load() -> ctypes.CDLL:
     lib.kq_qk_norm_rope.argtypes = [vp, i32, i64, i64, i64, i64, i64, vp, i32, vp, i64, i32, f32, vp, vp, i32, f32, vp, vp, i64p, vp, i64p,
                                     vp, i32, i64, i64, vp]
     lib.kq_paged_attention_workspace_bytes.restype = sz
-    lib.kq_paged_attention_workspace_bytes.argtypes = [i64]
+    lib.kq_paged_attention_workspace_bytes.argtypes = [i64, i64, i64, i64]
     lib.kq_paged_attention.argtypes = [vp, i32, i64, i64, i64, i64, i64, i64, vp, i64p, vp, i64p, i64, i64, vp, i64, i64, vp, f32, i64, f32,
                                        vp, vp, vp, sz, vp]
     lib.kq_plan_pages.argtypes = [vp, i64, i64, vp, vp, i64, vp, i64, vp, i64, i64, vp, vp, vp, vp, vp, vp]
@@ -357,8 +357,8 @@ def qk_norm_rope(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Ten
             k_out.shape[1] if store else 0, _stream(qkv.device)))
 
 
-def paged_attention_workspace_bytes(head_dim: int) -> int:
-    return int(lib.kq_paged_attention_workspace_bytes(head_dim))
+def paged_attention_workspace_bytes(batch: int, heads: int, kv_heads: int, head_dim: int) -> int:
+    return int(lib.kq_paged_attention_workspace_bytes(batch, heads, kv_heads, head_dim))
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,

@@ -7,11 +7,14 @@
 // share a key head (their rows are one tile) in registers, in fp32, and rescales them when a new maximum comes.
 //
 // The work is cut by cached keys, not by sequences: an item is (sequence, key head, row tile) and has one unit of work per
-// tile of keys, behind a few units for its beginning and end; the units of all items, in order, are divided evenly over the
-// CTAs of one wave.  A CTA finds its share from the lengths themselves (a sum and a scan, the lengths stay on the GPU), so a batch of any mix of lengths is balanced and a
-// captured call follows the lengths of each replay.  An item inside one CTA is finished there; one that crosses CTAs leaves
-// partial results (unnormalised values, maximum, sum) that attend_join_kernel adds in the order of the keys: no atomics, the
-// same bits every time.
+// tile of keys, behind a few units for its beginning and end; the units of all items, in order, are divided evenly over the workers
+// of one wave.  A worker finds its share from the lengths themselves (a sum and a scan, the lengths stay on the GPU), so a batch of any
+// mix of lengths is balanced and a captured call follows the lengths of each replay.  An item inside one worker is finished there; one that
+// crosses workers leaves partial results (unnormalised values, maximum, sum) that attend_join_kernel adds in the order of the
+// keys: no atomics, the same bits every time.
+//
+// A worker is a CTA whose warps take turns at the tiles and join their results at the end of an item, or, where there are items enough
+// for every warp of the wave, a warp on its own, which has nothing to join.
 #include <type_traits>
 
 #include "kq_common.cuh"
@@ -40,8 +43,9 @@ struct AttnParams {
   int window;
   void* out;                                           // [batch][heads][dim]
   float* lse;                                          // [batch][heads] or null
-  float* part_o; float2* part_ml; int2* meta;          // two partial results per CTA; which item starts in a CTA and ends in which other
+  float* part_o; float2* part_ml; int2* meta;          // two partial results per worker; which item starts in a worker and ends in which other
   int split;                                           // 0: one CTA per item
+  int solo;                                            // a worker is a warp (of the computing ones), not a CTA
 };
 
 // tiles of TK keys of sequence b (at least one, so that an empty row is visited too); *first..*end: its visible keys
@@ -54,21 +58,19 @@ __device__ __forceinline__ int tiles_of(const AttnParams& p, int b, int* first, 
   return max(1, (*end + TK - 1) / TK - *first / TK);
 }
 
-// A stretch of an item's tiles that one CTA works on.
+// A stretch of an item's tiles that one worker covers.
 struct Segment {
   int b, sub;            // sequence, (key head, row tile)
   int first, end;        // visible keys
   int t0, t1, tiles;     // tiles [t0, t1) of `tiles`; tile 0 starts at the last multiple of TK not above `first`
-  int last;              // the CTA that works on the item's last tile
+  int last;              // the worker that has the item's last tile, where that is another one
 };
 
-// The segments of one CTA, in order.  START: what an item costs beside its tiles, in tiles (loading q, joining the warps; without
-// it the CTAs that get the short sequences of a mixed batch end last).
+// The segments of one worker, in order.  START: what an item costs beside its tiles, in tiles (loading q, joining the warps; without
+// it the workers that get the short sequences of a mixed batch end last).
 template <int TK, int START>
 struct Walk {
   int64_t left, pos;              // units left, unit index
-  int64_t share, more;            // of `ctas` CTAs the first `more` have share + 1 units, the others `share`
-  int ctas;
   int b, sub, at, first, end, tiles;
   int first2, end2, tiles2;       // of the next sequence, loaded ahead
 
@@ -79,19 +81,20 @@ struct Walk {
     b = item / per; sub = item - b * per; at = START;
     tiles = tiles2 = tiles_of<TK>(p, b, &first, &end);
     first2 = first; end2 = end;
-    pos = 0; share = left = tiles; more = 0; ctas = 1;
+    pos = 0; left = tiles;
   }
 
-  __device__ int64_t begin_of(int c) const { return share * c + min((int64_t)c, more); }
-  __device__ int cta_of(int64_t unit) const {     // the CTA whose share holds `unit`
+  // the worker whose share holds `unit`; s_div: of the workers the first s_div[1] have s_div[0] + 1 units, the others s_div[0]
+  static __device__ int worker_of(const int64_t* s_div, int64_t unit) {
+    const int64_t share = s_div[0], more = s_div[1];
     return (int)(unit < more * (share + 1) ? div(unit, share + 1) : more + div(unit - more * (share + 1), share));
   }
   static __device__ int64_t div(int64_t x, int64_t y) {
     return (x | y) >> 32 ? x / y : (int64_t)((uint32_t)x / (uint32_t)y);
   }
 
-  // called by `threads` threads at once; s_red: one int64 per warp
-  __device__ void begin_share(const AttnParams& p, int64_t* s_red, int threads) {
+  // called by all `threads` threads of the CTA at once, which meet before next(); worker: the same for a warp; s_red: one int64 per warp
+  __device__ void begin_share(const AttnParams& p, int64_t* s_red, int64_t* s_div, int threads, int worker, int workers) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int per = p.kv_heads * p.row_tiles;
     int f, e;
@@ -120,13 +123,13 @@ struct Walk {
         if (p.batch <= 32) total = sum;
         total *= per;
         // a share that is hardly more than a beginning would only add partial results
-        ctas = (int)min((int64_t)gridDim.x, div(total + START, START + 2) + 1);
-        share = div(total, ctas);
-        more = total - share * ctas;
-        pos = begin_of(blockIdx.x);
-        left = begin_of(blockIdx.x + 1) - pos;
+        workers = (int)min((int64_t)workers, div(total + START, START + 2) + 1);
+        const int64_t share = div(total, workers), more = total - share * workers;
+        if (tid == 0) { s_div[0] = share; s_div[1] = more; }
+        pos = share * worker + min((int64_t)worker, more);
+        left = share + (worker < more);
         b = sub = at = 0;
-        if ((int)blockIdx.x >= ctas) { left = 0; return; }
+        if (worker >= workers) { left = 0; return; }
       }
       const unsigned past = __ballot_sync(0xffffffffu, (run + v) * per > pos);
       if (past) {
@@ -143,13 +146,13 @@ struct Walk {
     }
   }
 
-  __device__ bool next(const AttnParams& p, Segment* s) {
+  __device__ bool next(const AttnParams& p, const int64_t* s_div, Segment* s) {
     while (left > 0) {
       const int cost = START + tiles, take = (int)min((int64_t)(cost - at), left);
       s->b = b; s->sub = sub; s->first = first; s->end = end; s->tiles = tiles;
       s->t0 = max(at - START, 0); s->t1 = at + take - START;
       s->last = -1;
-      if (s->t0 == 0 && s->t1 > 0 && s->t1 < tiles) s->last = cta_of(pos + cost - at - 1);
+      if (s->t0 == 0 && s->t1 > 0 && s->t1 < tiles) s->last = worker_of(s_div, pos + cost - at - 1);
       left -= take; pos += take; at += take;
       if (at == cost) {
         at = 0;
@@ -159,15 +162,15 @@ struct Walk {
           load(p);
         }
       }
-      if (s->t1 > 0) return true;                 // otherwise the next CTA begins this item
+      if (s->t1 > 0) return true;                 // otherwise the next worker begins this item
     }
     return false;
   }
 };
 
 // index of a segment's partial result, -1 if it is the whole item
-__device__ __forceinline__ int part_of(const Segment& s) {
-  return s.t0 == 0 && s.t1 == s.tiles ? -1 : 2 * (int)blockIdx.x + (s.t0 == 0);
+__device__ __forceinline__ int part_of(const Segment& s, int worker) {
+  return s.t0 == 0 && s.t1 == s.tiles ? -1 : 2 * worker + (s.t0 == 0);
 }
 
 // 16 bytes, or with live = false 16 bytes of zeros and no read
@@ -199,14 +202,24 @@ template <typename T> struct RowOut {
   __device__ __forceinline__ void put(int d, float o) const {
     if (part) part[d] = o; else out[d] = from_f32<T>(o * scale);
   }
+  __device__ __forceinline__ void put2(int d, float a, float b) const {       // d even
+    if (part) {
+      *reinterpret_cast<float2*>(part + d) = make_float2(a, b);
+    } else {
+      alignas(2 * sizeof(T)) T v[2] = {from_f32<T>(a * scale), from_f32<T>(b * scale)};
+      if constexpr (sizeof(T) == 2) *reinterpret_cast<uint32_t*>(out + d) = *reinterpret_cast<const uint32_t*>(v);
+      else *reinterpret_cast<float2*>(out + d) = *reinterpret_cast<const float2*>(v);
+    }
+  }
 };
 
-// Adds the partial results of the item that starts in share blockIdx.x and ends in share meta.y, for one row, in the order of the keys.
+// Adds the partial results of the item that starts in a worker and ends in worker meta.y, for one row, in the order of the keys; 64
+// threads per worker.
 template <typename T>
-__global__ void __launch_bounds__(64) attend_join_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(256) attend_join_kernel(const AttnParams p) {
   pdl_trigger();
   pdl_wait();
-  const int c = blockIdx.x, r = blockIdx.y;
+  const int c = blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6), r = blockIdx.y, lane = threadIdx.x & 63;
   const int2 it = p.meta[c];
   if (it.x < 0) return;
   const int per = p.kv_heads * p.row_tiles;
@@ -214,7 +227,7 @@ __global__ void __launch_bounds__(64) attend_join_kernel(const AttnParams p) {
   const int head0 = h * p.group + x * p.rows;
   if (r >= min(p.rows, p.group - x * p.rows)) return;
   for (int d0 = 0; d0 < p.dim; d0 += 128) {
-    const int d = d0 + threadIdx.x * 2;
+    const int d = d0 + lane * 2;
     const bool in = d < p.dim;
     const float2* ml0 = p.part_ml + r;
     const float* o0 = p.part_o + (int64_t)r * p.dim + (in ? d : 0);
@@ -279,7 +292,7 @@ __global__ void __launch_bounds__(FM_WARPS * 32) attend_fma_kernel(const AttnPar
   constexpr int ROW = NI * 32 * CH;
   constexpr int SLOT = 2 * KB * ROW;              // keys, then values
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ int64_t s_red[FM_WARPS];
+  __shared__ int64_t s_red[FM_WARPS], s_div[2];
   __shared__ float2 s_ml[FM_WARPS * R];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * (STAGES * SLOT) + lane * CH;
@@ -289,13 +302,14 @@ __global__ void __launch_bounds__(FM_WARPS * 32) attend_fma_kernel(const AttnPar
 
   Walk<KB, FM_START> walk;
   if (p.split) {
-    walk.begin_share(p, s_red, FM_WARPS * 32);
+    walk.begin_share(p, s_red, s_div, FM_WARPS * 32, blockIdx.x, gridDim.x);
     if (tid == 0) p.meta[blockIdx.x] = make_int2(-1, 0);
   } else {
     walk.begin_item(p, blockIdx.x);
   }
+  __syncthreads();
   Segment s;
-  while (walk.next(p, &s)) {
+  while (walk.next(p, s_div, &s)) {
     const int b = s.b, first = s.first, end = s.end, t0 = s.t0, t1 = s.t1;
     const int h = s.sub / p.row_tiles, x = s.sub - h * p.row_tiles;
     const int head0 = h * p.group + x * p.rows, rows = min(p.rows, p.group - x * p.rows);
@@ -426,7 +440,7 @@ __global__ void __launch_bounds__(FM_WARPS * 32) attend_fma_kernel(const AttnPar
         if (d < p.dim) *reinterpret_cast<float4*>(s_o + (warp * R + r) * p.dim + d) = make_float4(o[r][i * 4], o[r][i * 4 + 1], o[r][i * 4 + 2], o[r][i * 4 + 3]);
       }
     __syncthreads();
-    const int part = part_of(s);
+    const int part = part_of(s, blockIdx.x);
     for (int i = tid; i < rows * p.dim; i += FM_WARPS * 32) {
       const int r = i / p.dim, d = i - r * p.dim;
       float top = -INFINITY, sum = 0.f, val = 0.f;
@@ -510,7 +524,8 @@ __device__ __forceinline__ void ring_wait(uint32_t bar, uint32_t parity, volatil
 // Four warps copy, the others compute.  The copiers walk the tiles of all segments of the CTA into one ring without a stop (cp.async,
 // whose arrival the slot's barrier counts), so the loads of the next segment are under way while this one's warps join; tile n goes to
 // computing warp n % NC, from copier n % NC.  The warps' results of a segment are added through shared memory, 32 columns at a time.
-template <typename T, int DP, bool TWO>
+// With SOLO each pair of a copier and a computing warp is a worker with segments of its own, which it finishes from its registers.
+template <typename T, int DP, bool TWO, bool SOLO>
 __global__ void __launch_bounds__(MmaShape<DP, TWO>::THREADS, 1) attend_mma_kernel(const AttnParams p) {
   using S = MmaShape<DP, TWO>;
   constexpr int R = S::R, NC = S::NC, NS = S::SLOTS, KEYS = S::KEYS, NT = KEYS / 8;
@@ -523,7 +538,7 @@ __global__ void __launch_bounds__(MmaShape<DP, TWO>::THREADS, 1) attend_mma_kern
   float2* s_row = s_ml + NC * R;                                                        // [R] of the segment
   __shared__ __align__(8) uint64_t s_full[NS], s_empty[NS];
   __shared__ uint32_t s_live[NS];
-  __shared__ int64_t s_red[S::THREADS / 32];
+  __shared__ int64_t s_red[S::THREADS / 32], s_div[2];
   __shared__ int s_gave_up;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t ring = s_u32(tl_smem), full = s_u32(s_full), empty = s_u32(s_empty);
@@ -535,10 +550,12 @@ __global__ void __launch_bounds__(MmaShape<DP, TWO>::THREADS, 1) attend_mma_kern
   if (tid == 0) s_gave_up = 0;
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   pdl_wait();
+  auto worker_of_warp = [&] { return (int)(SOLO ? blockIdx.x * NC + (threadIdx.x >> 5) % NC : blockIdx.x); };
+  const int stride = SOLO ? 1 : NC;                             // from a tile of this warp's to the next one
   Walk<KEYS, S::START> walk;
   if (p.split) {
-    walk.begin_share(p, s_red, S::THREADS);
-    if (tid == 0) p.meta[blockIdx.x] = make_int2(-1, 0);
+    walk.begin_share(p, s_red, s_div, S::THREADS, worker_of_warp(), SOLO ? gridDim.x * NC : gridDim.x);
+    if (warp < NC && lane == 0 && (SOLO || warp == 0)) p.meta[worker_of_warp()] = make_int2(-1, 0);
   } else {
     walk.begin_item(p, blockIdx.x);
   }
@@ -552,20 +569,20 @@ __global__ void __launch_bounds__(MmaShape<DP, TWO>::THREADS, 1) attend_mma_kern
     const int piece = lane % LPR;
     const bool in_row = piece * 8 < DP, in_dim = piece * 8 < p.dim;   // pieces from dim on are filled with zeros
     const bool one_page = p.page_size % 16 == 0;                  // 16 keys from a multiple of 16 on lie in one page
-    int n = warp - NC, n0 = 0;                                    // this warp's next tile; tiles before the segment
-    int slot = n, use = 0;                                        // n % NS, n / NS
-    while (walk.next(p, &s)) {
+    int n = SOLO ? 0 : warp - NC, n0 = 0;                       // this warp's next tile; tiles before the segment
+    int slot = warp - NC, use = 0;                                // every fourth slot, round by round
+    while (walk.next(p, s_div, &s)) {
       const int h = s.sub / p.row_tiles;
       const T* k_lane = static_cast<const T*>(p.k) + ((int64_t)h * p.k_head + (lane / LPR) * p.k_slot + piece * 8);
       const T* v_lane = static_cast<const T*>(p.v) + ((int64_t)h * p.v_head + (lane / LPR) * p.v_slot + piece * 8);
       const int key0 = s.first / KEYS * KEYS + lane, count = s.t1 - s.t0;
       int page = 0, place = 0;
       bool ok = n - n0 < count && lane < KEYS && find_key(p, s.b, key0 + (s.t0 + n - n0) * KEYS, s.first, s.end, &page, &place);
-      for (; n - n0 < count; n += MM_COPIERS) {
+      for (; n - n0 < count; n += stride) {
         const uint32_t live = __ballot_sync(0xffffffffu, ok);
         if (use > 0) ring_wait(empty + slot * 8, (use - 1) & 1, &s_gave_up);
         const int page_now = page, place_now = place;
-        ok = n + MM_COPIERS - n0 < count && lane < KEYS && find_key(p, s.b, key0 + (s.t0 + n + MM_COPIERS - n0) * KEYS, s.first, s.end, &page, &place);
+        ok = n + stride - n0 < count && lane < KEYS && find_key(p, s.b, key0 + (s.t0 + n + stride - n0) * KEYS, s.first, s.end, &page, &place);
 #pragma unroll
         for (int half = 0; half < KEYS / 16; ++half) {
           const uint32_t dst = ring + slot * S::SLOT + (half * 16 + lane / LPR) * S::ROW + piece * 16;
@@ -619,8 +636,8 @@ __global__ void __launch_bounds__(MmaShape<DP, TWO>::THREADS, 1) attend_mma_kern
   const uint32_t k_at = ring + ((lane >> 4) * 8 + (lane & 7)) * S::ROW + (lane >> 3 & 1) * 16;
   const uint32_t v_at = ring + (KEYS + (lane >> 3 & 1) * 8 + (lane & 7)) * S::ROW + (lane >> 4) * 16;
   uint32_t q[DP / 16][TWO ? 4 : 2];
-  int n0 = 0, n = warp, slot = warp % NS, use = warp / NS;
-  bool more = walk.next(p, &s);
+  int n0 = 0, n = SOLO ? 0 : warp, slot = warp, use = 0;
+  bool more = walk.next(p, s_div, &s);
   auto load_q = [&]() {
     const int h = s.sub / p.row_tiles, x = s.sub - h * p.row_tiles;
     const int head0 = h * p.group + x * p.rows, rows = min(p.rows, p.group - x * p.rows);
@@ -647,7 +664,7 @@ __global__ void __launch_bounds__(MmaShape<DP, TWO>::THREADS, 1) attend_mma_kern
       for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};       // rows g and g + 8, m less LIFT; l: of the lane's own keys
 
-    for (; n - n0 < count; n += NC) {
+    for (; n - n0 < count; n += stride) {
       ring_wait(full + slot * 8, use & 1, &s_gave_up);
       const uint32_t live = s_live[slot];
       const uint32_t off = slot * S::SLOT;
@@ -735,7 +752,7 @@ __global__ void __launch_bounds__(MmaShape<DP, TWO>::THREADS, 1) attend_mma_kern
       if (slot >= NS) { slot -= NS; ++use; }
     }
     n0 += count;
-    more = walk.next(p, &s);
+    more = walk.next(p, s_div, &s);
     if (more) load_q();                                           // arrives while the warps join
 
 #pragma unroll
@@ -743,6 +760,29 @@ __global__ void __launch_bounds__(MmaShape<DP, TWO>::THREADS, 1) attend_mma_kern
       l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
       l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
       if (t4 == 0) s_ml[warp * R + g + half * 8] = make_float2(m[half], l[half]);
+    }
+    if constexpr (!TWO) {                                         // high and low parts
+#pragma unroll
+      for (int i = 0; i < DP / 8; ++i) { o[i][0] += o[i][2]; o[i][1] += o[i][3]; }
+    }
+    const int h = now.sub / p.row_tiles, x = now.sub - h * p.row_tiles;
+    const int head0 = h * p.group + x * p.rows, rows = min(p.rows, p.group - x * p.rows);
+    const int part = part_of(now, worker_of_warp());
+    if (now.last >= 0 && lane == 0 && (SOLO || warp == 0)) p.meta[worker_of_warp()] = make_int2(now.b * p.kv_heads * p.row_tiles + now.sub, now.last);
+    if constexpr (SOLO) {
+#pragma unroll
+      for (int half = 0; half < (TWO ? 2 : 1); ++half) {
+        const int r = g + half * 8;
+        if (r < rows) {
+          const RowOut<T> out(p, part, now.b, head0 + r, r, m[half], l[half], t4 == 0);
+#pragma unroll
+          for (int i = 0; i < DP / 8; ++i) {
+            const int d = i * 8 + t4 * 2;
+            if (d < p.dim) out.put2(d, o[i][2 * half], o[i][2 * half + 1]);
+          }
+        }
+      }
+      continue;
     }
     auto meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(NC * 32) : "memory"); };
     meet();
@@ -762,9 +802,6 @@ __global__ void __launch_bounds__(MmaShape<DP, TWO>::THREADS, 1) attend_mma_kern
       for (int w = 0; w < NC; ++w) sum += s_ml[w * R + tid].y * ex2(s_ml[w * R + tid].x - (top == -INFINITY ? 0.f : top));
       s_row[tid] = make_float2(top, sum);
     }
-    const int h = now.sub / p.row_tiles, x = now.sub - h * p.row_tiles;
-    const int head0 = h * p.group + x * p.rows, rows = min(p.rows, p.group - x * p.rows);
-    const int part = part_of(now);
     auto lay_down = [&](int sl) {
       float* buf = s_join + (sl & 1) * (NC * R * S::JROW) + (warp * R + g) * S::JROW + t4 * 2;
 #pragma unroll
@@ -772,8 +809,7 @@ __global__ void __launch_bounds__(MmaShape<DP, TWO>::THREADS, 1) attend_mma_kern
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int nt = sl * 4 + i;
-          const float a = TWO ? o[nt][2 * half] : o[nt][0] + o[nt][2], e = TWO ? o[nt][2 * half + 1] : o[nt][1] + o[nt][3];
-          *reinterpret_cast<float2*>(buf + half * 8 * S::JROW + i * 8) = make_float2(a * f[half], e * f[half]);
+          *reinterpret_cast<float2*>(buf + half * 8 * S::JROW + i * 8) = make_float2(o[nt][2 * half] * f[half], o[nt][2 * half + 1] * f[half]);
         }
     };
     lay_down(0);
@@ -799,7 +835,6 @@ __global__ void __launch_bounds__(MmaShape<DP, TWO>::THREADS, 1) attend_mma_kern
       }
       if (sl + 1 < DP / 32) lay_down(sl + 1);
     }
-    if (now.last >= 0 && tid == 0) p.meta[blockIdx.x] = make_int2(now.b * p.kv_heads * p.row_tiles + now.sub, now.last);
   }
 }
 
@@ -810,7 +845,7 @@ int launch_both(void (*kern)(const AttnParams), AttnParams& p, int threads, int 
   KQ_CUDA_TRY(launch_pdl(kern, dim3(grid), dim3(threads), (size_t)smem, st, pdl, p));
   options().launches += 1;
   if (p.split) {
-    KQ_CUDA_TRY(launch_pdl(attend_join_kernel<T>, dim3(grid, (unsigned)p.rows), dim3(64), (size_t)0, st, pdl, p));
+    KQ_CUDA_TRY(launch_pdl(attend_join_kernel<T>, dim3(grid, (unsigned)p.rows), dim3(p.solo ? 256 : 64), (size_t)0, st, pdl, p));
     options().launches += 1;
   }
   return KQ_OK;
@@ -833,13 +868,13 @@ int run_fma(AttnParams& p, cudaStream_t st) {
 template <typename T, int DP, bool TWO>
 int run_mma(AttnParams& p, cudaStream_t st) {
   using S = MmaShape<DP, TWO>;
-  auto kern = attend_mma_kernel<T, DP, TWO>;
   static DeviceOnce attr_set;
   if (attr_set.first_time()) {
-    KQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
+    KQ_CUDA_TRY(cudaFuncSetAttribute(attend_mma_kernel<T, DP, TWO, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
+    KQ_CUDA_TRY(cudaFuncSetAttribute(attend_mma_kernel<T, DP, TWO, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
     attr_set.done();
   }
-  return launch_both<T>(kern, p, S::THREADS, S::SMEM, 1, st);
+  return launch_both<T>(p.solo ? attend_mma_kernel<T, DP, TWO, true> : attend_mma_kernel<T, DP, TWO, false>, p, S::THREADS, S::SMEM, 1, st);
 }
 
 // the query heads of a key head in tiles of at most `most` rows, of even sizes
@@ -855,9 +890,17 @@ int run_f32(AttnParams& p, cudaStream_t st) {
   return p.dim > 128 ? run_fma<8, 2>(p, st) : run_fma<8, 1>(p, st);
 }
 
+// From how many items on a worker is a warp.  As warps / as CTAs, us, 148 multiprocessors: 256 sequences of 1..500 tokens with 8 key heads
+// 59.3 / 88.8, 64 of 1..1000 34.4 / 41.8, 64 of 4096 187.9 / 185.7, 16 of 900..3100 (128 items) 31.4 / 32.7, 16 of 4000 with heads of 64 31.8 / 37.9;
+// 66 items of 100..7001 with heads of 256 57.0 / 53.8, 64 items of 8000 59.2 / 54.5, 8 items of 131071 102.7 / 98.7: few items are cut into
+// many more parts.  Where short lengths need no division at all (a CTA per item, no join): 1024 items of 1..200 21.3 / 38.9, within a wave the CTAs.
+bool solo_pays(int64_t items, bool split) { return split ? 4 * items >= 3 * (int64_t)sm_count() : items > 2 * (int64_t)sm_count(); }
+
 template <typename T>
 int run_16bit(AttnParams& p, cudaStream_t st) {
   set_rows(p, 16);
+  p.solo = solo_pays((int64_t)p.batch * p.kv_heads * p.row_tiles, p.split);
+  p.split |= p.solo;
   if (p.rows <= 8)
     return p.dim <= 64 ? run_mma<T, 64, false>(p, st) : p.dim <= 96 ? run_mma<T, 96, false>(p, st) : p.dim <= 128 ? run_mma<T, 128, false>(p, st)
          : p.dim <= 192 ? run_mma<T, 192, false>(p, st) : run_mma<T, 256, false>(p, st);
@@ -865,15 +908,19 @@ int run_16bit(AttnParams& p, cudaStream_t st) {
        : p.dim <= 192 ? run_mma<T, 192, true>(p, st) : run_mma<T, 256, true>(p, st);
 }
 
-constexpr int AT_MAX_ROWS = 16;         // rows of a partial result at most
-
 struct Scratch { size_t o, ml, meta, total; };
-Scratch scratch_of(int64_t ctas, int64_t dim) {
+Scratch scratch_of(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim) {
+  AttnParams p;
+  p.group = (int)(heads / kv_heads);
+  set_rows(p, 16);
+  const int64_t rows = p.rows > 8 ? p.rows : 8;              // of either type's tiles
+  const int64_t workers = sm_count() * (solo_pays(batch * kv_heads * p.row_tiles, true) ? 4 : FM_CTAS);
+  auto up = [](int64_t bytes) { return (size_t)((bytes + 255) / 256 * 256); };
   Scratch s;
   s.o = 0;
-  s.ml = s.o + (size_t)(2 * ctas * AT_MAX_ROWS * dim * 4 + 255) / 256 * 256;
-  s.meta = s.ml + (size_t)(2 * ctas * AT_MAX_ROWS * 8 + 255) / 256 * 256;
-  s.total = s.meta + (size_t)(ctas * 8 + 255) / 256 * 256;
+  s.ml = s.o + up(2 * workers * rows * dim * 4);
+  s.meta = s.ml + up(2 * workers * rows * 8);
+  s.total = s.meta + up(workers * 8);
   return s;
 }
 
@@ -885,9 +932,13 @@ using namespace kq;
 
 extern "C" {
 
-size_t kq_paged_attention_workspace_bytes(int64_t head_dim) {
-  if (head_dim <= 0 || head_dim > 256) return 0;
-  return scratch_of((int64_t)sm_count() * FM_CTAS, head_dim).total;
+static bool attention_sizes_ok(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim) {
+  return batch >= 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && head_dim >= 16 && head_dim <= 256 && head_dim % 16 == 0 &&
+         batch <= (1 << 20) && heads <= (1 << 16) && batch * heads <= 0x7fffffff;
+}
+
+size_t kq_paged_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim) {
+  return attention_sizes_ok(batch, heads, kv_heads, head_dim) ? scratch_of(batch, heads, kv_heads, head_dim).total : 0;
 }
 
 int kq_paged_attention(const void* q, int dtype, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t q_stride_batch,
@@ -922,8 +973,7 @@ int kq_paged_attention(const void* q, int dtype, int64_t batch, int64_t heads, i
       return KQ_EINVAL;
     }
   if ((uintptr_t)k_cache % 16 || (uintptr_t)v_cache % 16 || (uintptr_t)q % size || (uintptr_t)out % 16) { set_error("%s: misaligned pointer", fn); return KQ_EINVAL; }
-  const int64_t ctas = (int64_t)sm_count() * FM_CTAS;
-  const Scratch L = scratch_of(ctas, head_dim);
+  const Scratch L = scratch_of(batch, heads, kv_heads, head_dim);
   if (!scratch || (uintptr_t)scratch % 256) { set_error("%s: scratch must be non-null and 256-byte aligned", fn); return KQ_ESCRATCH; }
   if (scratch_bytes < L.total) { set_error("%s: scratch too small (%zu < %zu)", fn, scratch_bytes, L.total); return KQ_ESCRATCH; }
 
@@ -938,6 +988,7 @@ int kq_paged_attention(const void* q, int dtype, int64_t batch, int64_t heads, i
   p.out = out; p.lse = lse;
   uint8_t* sb = (uint8_t*)scratch;
   p.part_o = (float*)(sb + L.o); p.part_ml = (float2*)(sb + L.ml); p.meta = (int2*)(sb + L.meta);
+  p.solo = 0;
   int64_t most = table_width * page_size;          // keys that a sequence can show
   if (window > 0 && window < most) most = window;
   p.split = most > 256;      // short sequences: one launch, one CTA per item

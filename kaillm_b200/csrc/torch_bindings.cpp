@@ -427,7 +427,7 @@ std::tuple<at::Tensor, at::Tensor> paged_attention(const at::Tensor& q, const at
   const c10::cuda::CUDAGuard guard(q.device());
   at::Tensor out = new_cuda({b, h, d}, q.scalar_type(), q), norm;
   if (lse) norm = new_cuda({b, h}, at::kFloat, q);
-  const size_t ws = kq_paged_attention_workspace_bytes(d);
+  const size_t ws = kq_paged_attention_workspace_bytes(b, h, k_cache.size(2), d);
   at::Tensor scratch = new_cuda({(int64_t)ws}, at::kByte, q);
   TORCH_CHECK(kq_paged_attention(q.data_ptr(), dt, b, h, k_cache.size(2), d, q.stride(0), q.stride(1), k_cache.data_ptr(), k_cache.strides().data(),
                                  v_cache.data_ptr(), v_cache.strides().data(), k_cache.size(0), k_cache.size(1), block_table.data_ptr<int32_t>(),

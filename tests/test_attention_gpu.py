@@ -68,6 +68,17 @@ def test_long_and_short_together(dtype):
     run([9000, 1, 0, 37, 4096, 2], 8, 1, 128, 16, dtype)
 
 
+@pytest.mark.parametrize("heads,kv,dim", [(8, 8, 128), (20, 2, 64), (16, 1, 256), (18, 9, 96)])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_items_enough_for_every_warp(heads, kv, dim, dtype):
+    """Many items: warps work on their own; few of them cross from one to the next, one of them over many."""
+    lens = [(37 * i) % 211 for i in range(120 if kv < 4 else 40)]
+    run(lens, heads, kv, dim, 16, dtype, width=14)                # lengths that need no division
+    lens[5] = 2500
+    run(lens, heads, kv, dim, 16, dtype)
+    run(lens, heads, kv, dim, 8, dtype, window=70)
+
+
 def test_many_sequences():
     """More sequences than one scan step of a CTA covers, in an order of lengths that a static split would serve badly."""
     lens = [(i * i) % 97 for i in range(700)]

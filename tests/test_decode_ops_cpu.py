@@ -30,8 +30,9 @@ def test_paged_attention():
         assert "kq_paged_attention" in capi.lib.kq_last_error().decode()
     assert _attend(scratch=None) == ESCRATCH and _attend(scratch=0x7010) == ESCRATCH and _attend(sbytes=1000) == ESCRATCH
     assert _attend(b=1 << 21) == ELIMIT and _attend(page=1 << 31) == ELIMIT and _attend(width=1 << 31) == ELIMIT and _attend(b=1 << 20, h=1 << 12, kv=1) == ELIMIT
-    assert capi.lib.kq_paged_attention_workspace_bytes(0) == 0 and capi.lib.kq_paged_attention_workspace_bytes(272) == 0
-    assert 0 < capi.lib.kq_paged_attention_workspace_bytes(64) < capi.lib.kq_paged_attention_workspace_bytes(256) < 64 << 20
+    ws = capi.paged_attention_workspace_bytes
+    assert ws(1, 8, 2, 0) == 0 and ws(1, 8, 2, 272) == 0 and ws(1, 8, 3, 64) == 0 and ws(-1, 8, 2, 64) == 0
+    assert 0 < ws(1, 8, 2, 64) < ws(1, 8, 2, 256) <= ws(1, 40, 2, 256) < ws(1000, 40, 2, 256) < 64 << 20
 
 
 def _rope(qkv=0x1000, dt=2, t=4, st=1536, h=8, kv=2, d=128, pos=0x2000, p64=0, freq=0x3000, rot=128, inter=0, qw=None, kw=None, wdt=0, q=0x4000, k=0x5000,
