@@ -78,7 +78,7 @@ __device__ __noinline__ void route_wide(const RouteParams& p, int64_t t) {
   }
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-  sum = fmax(sum, 1e-300);
+  sum = fmax(sum, 1.1754943508222875e-38);
   unsigned long long key[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i)
@@ -114,7 +114,7 @@ __device__ __noinline__ void route_wide(const RouteParams& p, int64_t t) {
       if (e0 + i < p.experts && !(kept >> ((e0 + i) / p.group_size) & 1)) key[i] = RT_OUTSIDE;
   }
   int id = 0;                                    // of rank `lane`
-  float w = 0.f;
+  float chosen = 0.f;
   for (int n = 0; n < p.top_k; ++n) {
     unsigned long long a = key[0];
     int at = 0;
@@ -129,11 +129,10 @@ __device__ __noinline__ void route_wide(const RouteParams& p, int64_t t) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if (e0 + i == e) key[i] = RT_TAKEN;
-    if (lane == n) {
-      id = e;
-      w = (float)(p.sigmoid ? 1. / (1. + exp(-(double)xe)) : exp((double)xe - (double)top) / sum);
-    }
+    if (lane == n) { id = e; chosen = xe; }
   }
+  float w = 0.f;
+  if (lane < p.top_k) w = p.sigmoid ? 1.f / (1.f + expf(-chosen)) : expf(chosen - top) / (float)sum;
   if (p.renormalize) w /= fmaxf(warp_sum(w), 1.1754943508222875e-38f);
   if (lane < p.top_k) {
     p.weights[t * p.top_k + lane] = w * p.scale;
