@@ -16,6 +16,8 @@ void set_error(const char* fmt, ...) {
   va_end(ap);
 }
 
+void clear_error() { t_err[0] = 0; }
+
 int cuda_fail(cudaError_t e, const char* what) {
   set_error("CUDA error %d (%s) at %s", (int)e, cudaGetErrorString(e), what);
   return KQ_ECUDA;

@@ -947,7 +947,7 @@ int kq_paged_attention(const void* q, int dtype, int64_t batch, int64_t heads, i
                        int64_t table_width, const int32_t* seq_lens, float scale, int64_t window, float softcap, void* out, float* lse,
                        void* scratch, size_t scratch_bytes, void* stream) {
   const char* fn = "kq_paged_attention";
-  set_error("%s", "");
+  clear_error();
   if (dtype != KQ_F32 && dtype != KQ_F16 && dtype != KQ_BF16) { set_error("%s: unsupported dtype %d", fn, dtype); return KQ_EUNSUPPORTED; }
   if (batch < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads) {
     set_error("%s: heads=%lld must be a positive multiple of kv_heads=%lld", fn, (long long)heads, (long long)kv_heads);
@@ -1001,7 +1001,7 @@ int kq_paged_attention(const void* q, int dtype, int64_t batch, int64_t heads, i
 }
 
 int kq_paged_attention_status(int* status, int clear) {
-  set_error("%s", "");
+  clear_error();
   KQ_CUDA_TRY(cudaDeviceSynchronize());   // the copy does not wait for non-blocking streams
   int v = 0;
   KQ_CUDA_TRY(cudaMemcpyFromSymbol(&v, g_attend_status, sizeof(int)));

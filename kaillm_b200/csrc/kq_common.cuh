@@ -15,6 +15,7 @@ namespace kq {
 
 // ------------------------------------------------------------------ host side plumbing
 void set_error(const char* fmt, ...);
+void clear_error();
 int cuda_fail(cudaError_t e, const char* what);
 #define KQ_CUDA_TRY(expr)                                  \
   do {                                                     \

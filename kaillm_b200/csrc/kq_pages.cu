@@ -125,7 +125,7 @@ extern "C" int kq_plan_pages(int32_t* block_table, int64_t table_stride, int64_t
                              const int32_t* taken, int64_t page_size, int64_t num_tokens, int32_t* total_lens, int32_t* starts,
                              int32_t* positions, int64_t* slots, int32_t* taken_out, void* stream) {
   const char* fn = "kq_plan_pages";
-  set_error("%s", "");
+  clear_error();
   if (requests < 0 || table_width < 0 || num_free < 0 || num_tokens < 0 || page_size <= 0) { set_error("%s: page_size must be positive, the other sizes not negative", fn); return KQ_EINVAL; }
   if (requests > (1 << 20) || table_width > 0x7fffffff || num_free > 0x7fffffff || num_tokens > 0x7fffffff || page_size > 0x7fffffff) { set_error("%s: size out of range", fn); return KQ_ELIMIT; }
   if (requests > 1 && table_stride < table_width) { set_error("%s: rows of the table overlap", fn); return KQ_EINVAL; }

@@ -333,7 +333,7 @@ extern "C" int kq_qk_norm_rope(const void* qkv, int dtype, int64_t tokens, int64
                                void* q_out, void* k_out, const int64_t* k_strides, void* v_cache, const int64_t* v_strides,
                                const void* slots, int slots64, int64_t num_pages, int64_t page_size, void* stream) {
   const char* fn = "kq_qk_norm_rope";
-  set_error("%s", "");
+  clear_error();
   if (dtype != KQ_F32 && dtype != KQ_F16 && dtype != KQ_BF16) { set_error("%s: unsupported dtype %d", fn, dtype); return KQ_EUNSUPPORTED; }
   if ((q_weight || k_weight) && w_dtype != KQ_F32 && w_dtype != dtype) { set_error("%s: norm weights must be float32 or of the activations' type", fn); return KQ_EUNSUPPORTED; }
   if (tokens < 0 || heads <= 0 || kv_heads <= 0) { set_error("%s: heads and kv_heads must be positive, tokens not negative", fn); return KQ_EINVAL; }

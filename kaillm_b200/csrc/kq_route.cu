@@ -416,7 +416,7 @@ extern "C" int kq_moe_route(const void* logits, int dtype, int64_t tokens, int64
                             const float* bias, int64_t groups, int64_t top_groups, int renormalize, float scale, float* weights,
                             int32_t* ids, void* stream) {
   const char* fn = "kq_moe_route";
-  set_error("%s", "");
+  clear_error();
   if (dtype != KQ_F32 && dtype != KQ_F16 && dtype != KQ_BF16) { set_error("%s: unsupported dtype %d", fn, dtype); return KQ_EUNSUPPORTED; }
   if (tokens < 0 || experts <= 0 || top_k <= 0 || top_k > experts) { set_error("%s: top_k=%lld is not between 1 and experts=%lld", fn, (long long)top_k, (long long)experts); return KQ_EINVAL; }
   if (experts > RT_MAX_EXPERTS || top_k > RT_MAX_TOP || groups > RT_MAX_GROUPS || tokens > 0x7fffffff) {
