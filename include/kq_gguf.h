@@ -351,7 +351,9 @@ int kq_qk_norm_rope(const void* qkv, int dtype, int64_t tokens, int64_t stride_t
  *   - a sequence that shows no token: zeros, lse = -infinity
  * q: [batch, heads, head_dim] with strides q_stride_batch, q_stride_head, head_dim dense; out: dense; lse: [batch, heads] fp32 log
  * of the sum of exponentials, or NULL.  q, caches and out have one dtype; scores, softmax and sums are fp32.  head_dim: a
- * multiple of 16 up to 256 (KQ_EUNSUPPORTED otherwise); caches and their strides 16-byte aligned.
+ * multiple of 16 up to 256 (KQ_EUNSUPPORTED otherwise); caches and their strides and out 16-byte aligned; out is not q.  scale and
+ * softcap: at most 1e30.  Where a visible value is not finite, neither are the outputs of its column (NaN also where one infinity alone
+ * would give infinity).
  * scratch: kq_paged_attention_workspace_bytes(...) bytes for the current device (0 for sizes that are not served), 256-byte aligned,
  * not initialised; calls that may overlap need one each. */
 size_t kq_paged_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim);
@@ -375,7 +377,8 @@ int kq_paged_attention_status(int* status, int clear);
  *   positions, slots [num_tokens] of the new tokens, request by request; slot -1 (and position 0 behind the last token) for
  *                padding, tokens beyond the row and tokens without a page
  *   taken_out    [1]             taken + pages asked for: above num_free means that some were not there
- * num_tokens must not be below the sum of new_lens: tokens that do not fit get neither a slot nor a table entry. */
+ * num_tokens must not be below the sum of new_lens: tokens that do not fit get neither a slot nor a table entry.  No output but
+ * block_table may be an input. */
 int kq_plan_pages(int32_t* block_table, int64_t table_stride, int64_t table_width, const int32_t* seq_lens,
                   const int32_t* new_lens, int64_t requests, const int32_t* free_pages, int64_t num_free,
                   const int32_t* taken, int64_t page_size, int64_t num_tokens, int32_t* total_lens, int32_t* starts,

@@ -960,7 +960,8 @@ int kq_paged_attention(const void* q, int dtype, int64_t batch, int64_t heads, i
   }
   if (page_size <= 0 || num_pages < 0 || table_width < 0) { set_error("%s: page_size must be positive, num_pages and table_width not negative", fn); return KQ_EINVAL; }
   if (window < 0 || window > 0x7fffffff) { set_error("%s: window=%lld is outside [0, 2^31)", fn, (long long)window); return KQ_EINVAL; }
-  if (!(scale > 0.f) || scale > 3e38f || !(softcap >= 0.f) || softcap > 3e38f) { set_error("%s: scale must be positive and softcap not negative, both finite", fn); return KQ_EINVAL; }
+  // up to 1e30, so that neither overflows when multiplied by log2(e), nor score / softcap leaves fp32's normal numbers
+  if (!(scale > 0.f) || scale > 1e30f || !(softcap >= 0.f) || softcap > 1e30f) { set_error("%s: scale must be positive and softcap not negative, both at most 1e30", fn); return KQ_EINVAL; }
   if (batch == 0) return KQ_OK;
   if (!q || !out || !seq_lens || (table_width > 0 && !block_table) || (num_pages > 0 && (!k_cache || !v_cache)) || !k_strides || !v_strides) {
     set_error("%s: null pointer", fn);
@@ -972,7 +973,11 @@ int kq_paged_attention(const void* q, int dtype, int64_t batch, int64_t heads, i
       set_error("%s: cache strides must be multiples of 16 bytes", fn);
       return KQ_EINVAL;
     }
-  if ((uintptr_t)k_cache % 16 || (uintptr_t)v_cache % 16 || (uintptr_t)q % size || (uintptr_t)out % 16) { set_error("%s: misaligned pointer", fn); return KQ_EINVAL; }
+  if ((uintptr_t)k_cache % 16 || (uintptr_t)v_cache % 16 || (uintptr_t)q % size || (uintptr_t)out % 16 || ((uintptr_t)block_table | (uintptr_t)seq_lens | (uintptr_t)lse) % 4) {
+    set_error("%s: misaligned pointer", fn);
+    return KQ_EINVAL;
+  }
+  if (q == out) { set_error("%s: out must not be q", fn); return KQ_EINVAL; }   // several workers read a row of q
   const Scratch L = scratch_of(batch, heads, kv_heads, head_dim);
   if (!scratch || (uintptr_t)scratch % 256) { set_error("%s: scratch must be non-null and 256-byte aligned", fn); return KQ_ESCRATCH; }
   if (scratch_bytes < L.total) { set_error("%s: scratch too small (%zu < %zu)", fn, scratch_bytes, L.total); return KQ_ESCRATCH; }

@@ -134,7 +134,13 @@ extern "C" int kq_plan_pages(int32_t* block_table, int64_t table_stride, int64_t
     set_error("%s: null pointer", fn);
     return KQ_EINVAL;
   }
-  if (taken == taken_out) { set_error("%s: taken_out must not be taken", fn); return KQ_EINVAL; }   // other CTAs may still read it
+  if (((uintptr_t)block_table | (uintptr_t)seq_lens | (uintptr_t)new_lens | (uintptr_t)free_pages | (uintptr_t)taken | (uintptr_t)total_lens | (uintptr_t)starts |
+       (uintptr_t)positions | (uintptr_t)taken_out) % 4 || (uintptr_t)slots % 8) {
+    set_error("%s: misaligned pointer", fn);
+    return KQ_EINVAL;
+  }
+  // other CTAs may still read what the first one would overwrite
+  if (taken == taken_out || (requests && (total_lens == seq_lens || total_lens == new_lens))) { set_error("%s: outputs must not be inputs", fn); return KQ_EINVAL; }
   PageParams p;
   p.table = block_table; p.table_r = table_stride; p.width = (int)table_width; p.seen = seq_lens; p.fresh = new_lens;
   p.requests = (int)requests; p.free_pages = free_pages; p.num_free = (int)num_free; p.taken = taken; p.page_size = (int)page_size;

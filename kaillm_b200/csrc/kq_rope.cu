@@ -346,7 +346,11 @@ extern "C" int kq_qk_norm_rope(const void* qkv, int dtype, int64_t tokens, int64
   if (!qkv || !positions || (rotated && !inv_freq) || !q_out || !k_out || (store && (!k_strides || !v_strides || !slots))) { set_error("%s: null pointer", fn); return KQ_EINVAL; }
   if (store && (num_pages <= 0 || page_size <= 0)) { set_error("%s: the cache has no pages", fn); return KQ_EINVAL; }
   const uintptr_t size = dtype == KQ_F32 ? 4 : 2;
-  if ((uintptr_t)qkv % size || (uintptr_t)q_out % size || (uintptr_t)k_out % size || (uintptr_t)v_cache % size || (uintptr_t)inv_freq % 4) { set_error("%s: misaligned pointer", fn); return KQ_EINVAL; }
+  if ((uintptr_t)qkv % size || (uintptr_t)q_out % size || (uintptr_t)k_out % size || (uintptr_t)v_cache % size || (uintptr_t)inv_freq % 4 ||
+      (uintptr_t)positions % (positions64 ? 8 : 4) || (store && (uintptr_t)slots % (slots64 ? 8 : 4)) || ((uintptr_t)q_weight | (uintptr_t)k_weight) % (w_dtype == KQ_F32 ? 4 : 2)) {
+    set_error("%s: misaligned pointer", fn);
+    return KQ_EINVAL;
+  }
   RopeParams p;
   p.qkv = qkv; p.qkv_t = stride_t; p.positions = positions; p.pos64 = positions64; p.inv_freq = inv_freq;
   p.qw = q_weight; p.kw = k_weight; p.w_f32 = w_dtype == KQ_F32; p.eps = eps; p.factor = factor; p.inv_dim = 1.f / (float)head_dim; p.tokens = tokens;

@@ -25,7 +25,8 @@ def test_paged_attention():
     for bad in (dict(b=-1), dict(h=0), dict(kv=0), dict(h=7), dict(page=0), dict(pages=-1), dict(width=-1), dict(window=-1), dict(window=1 << 31), dict(scale=0.0),
                 dict(scale=float("nan")), dict(scale=float("inf")), dict(cap=-1.0), dict(cap=float("nan")), dict(q=None), dict(out=None), dict(lens=None),
                 dict(table=None), dict(k=None), dict(v=None), dict(k=0x2008), dict(v=0x3002), dict(q=0x1001), dict(out=0x6004), dict(ks=(4097, 256, 128)),
-                dict(vs=(4096, 256, 4)), dict(ks=(-4096, 256, 128))):
+                dict(vs=(4096, 256, 4)), dict(ks=(-4096, 256, 128)), dict(out=0x1000), dict(lens=0x5002), dict(table=0x4001), dict(lse=0x8002),
+                dict(scale=2e30), dict(cap=2e30)):
         assert _attend(**bad) == EINVAL, bad
         assert "kq_paged_attention" in capi.lib.kq_last_error().decode()
     assert _attend(scratch=None) == ESCRATCH and _attend(scratch=0x7010) == ESCRATCH and _attend(sbytes=1000) == ESCRATCH
@@ -47,7 +48,8 @@ def test_qk_norm_rope():
     assert _rope(qw=0x8000, wdt=1) == EUNSUPPORTED and "norm weights" in capi.lib.kq_last_error().decode()
     for bad in (dict(t=-1), dict(h=0), dict(kv=0), dict(rot=130), dict(rot=3), dict(rot=-2), dict(st=1535), dict(qkv=None), dict(pos=None), dict(freq=None), dict(q=None),
                 dict(k=None), dict(qkv=0x1001), dict(q=0x4001), dict(freq=0x3002), dict(cache, slots=None), dict(cache, ks=None), dict(cache, vs=None),
-                dict(cache, pages=0), dict(cache, page=0), dict(cache, v=0x6001)):
+                dict(cache, pages=0), dict(cache, page=0), dict(cache, v=0x6001), dict(pos=0x2002), dict(pos=0x2004, p64=1), dict(cache, slots=0x7002),
+                dict(cache, slots=0x7004, s64=1), dict(qw=0x8001, wdt=2), dict(kw=0x8002, wdt=0)):
         assert _rope(**bad) == EINVAL, bad
     assert _rope(h=1 << 17) == ELIMIT and _rope(**dict(cache, page=1 << 31)) == ELIMIT and _rope(t=1 << 31) == ELIMIT
 
@@ -59,7 +61,9 @@ def _plan(table=0x1000, ts=8, width=8, seen=0x2000, new=0x3000, r=4, free=0x4000
 
 def test_plan_pages():
     for bad in (dict(page=0), dict(r=-1), dict(width=-1), dict(nfree=-1), dict(tokens=-1), dict(ts=7), dict(table=None), dict(seen=None), dict(new=None),
-                dict(free=None), dict(taken=None), dict(total=None), dict(starts=None), dict(pos=None), dict(slots=None), dict(out=None), dict(out=0x5000)):
+                dict(free=None), dict(taken=None), dict(total=None), dict(starts=None), dict(pos=None), dict(slots=None), dict(out=None), dict(out=0x5000),
+                dict(total=0x2000), dict(total=0x3000), dict(table=0x1002), dict(seen=0x2001), dict(new=0x3002), dict(free=0x4001), dict(taken=0x5002), dict(total=0x6001),
+                dict(starts=0x7002), dict(pos=0x8001), dict(slots=0x9004), dict(out=0xa002)):
         assert _plan(**bad) == EINVAL, bad
     assert _plan(r=(1 << 20) + 1) == ELIMIT and _plan(tokens=1 << 31) == ELIMIT and _plan(page=1 << 31) == ELIMIT
 
@@ -71,7 +75,7 @@ def _route(x=0x1000, dt=0, t=4, e=64, st=64, k=8, sig=0, bias=None, g=1, tg=1, r
 def test_moe_route():
     assert _route(t=0) == OK and _route(dt=5) == EUNSUPPORTED
     for bad in (dict(t=-1), dict(e=0), dict(k=0), dict(k=65), dict(g=0), dict(g=3), dict(g=4, tg=0), dict(g=4, tg=5), dict(g=16, tg=1), dict(x=None), dict(w=None), dict(ids=None),
-                dict(st=63), dict(x=0x1002), dict(bias=0x4001)):
+                dict(st=63), dict(x=0x1002), dict(bias=0x4001), dict(w=0x2002), dict(ids=0x3001)):
         assert _route(**bad) == EINVAL, bad
     assert _route(e=1025, st=1025) == ELIMIT and _route(k=33) == ELIMIT and _route(g=64, tg=64) == ELIMIT
 
