@@ -55,7 +55,7 @@ __device__ __forceinline__ int tiles_of(const AttnParams& p, int b, int* first, 
   const int64_t held = (int64_t)p.width * p.page_size;
   *end = (int)min((int64_t)len, held);
   *first = p.window > 0 && len > p.window ? len - p.window : 0;
-  return max(1, (*end + TK - 1) / TK - *first / TK);
+  return max(1, (int)(((unsigned)*end + TK - 1) / TK) - *first / TK);     // a length may be 2^31 - 1
 }
 
 // A stretch of an item's tiles that one worker covers.
@@ -263,10 +263,10 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const AttnParams p) {
 }
 
 // Where key j of sequence b lies: page name and place inside the page; false where there is no such page.
-__device__ __forceinline__ bool find_key(const AttnParams& p, int b, int j, int first, int end, int* page, int* place) {
-  if (j < first || j >= end) return false;
-  const int at = (int)((unsigned)j / (unsigned)p.page_size);
-  *place = j - at * p.page_size;
+__device__ __forceinline__ bool find_key(const AttnParams& p, int b, unsigned j, int first, int end, int* page, int* place) {
+  if (j < (unsigned)first || j >= (unsigned)end) return false;
+  const int at = (int)(j / (unsigned)p.page_size);
+  *place = (int)j - at * p.page_size;
   *page = p.table[(int64_t)b * p.table_b + at];
   return *page >= 0 && *page < p.num_pages;
 }
@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(FM_WARPS * 32) attend_fma_kernel(const AttnPar
     uint32_t live_ring[STAGES];
     auto fetch = [&](int t, int slot) -> uint32_t {
       int page = 0, place = 0;
-      const int j = key0 + t * KB + (lane % KB);
+      const unsigned j = (unsigned)key0 + (unsigned)t * KB + (lane % KB);
       const bool ok = t < t1 && find_key(p, b, j, first, end, &page, &place);
       const uint32_t live = __ballot_sync(0xffffffffu, ok);
       if (t < t1) {
@@ -575,7 +575,8 @@ __global__ void __launch_bounds__(MmaShape<DP, TWO>::THREADS, 1) attend_mma_kern
       const int h = s.sub / p.row_tiles;
       const T* k_lane = static_cast<const T*>(p.k) + ((int64_t)h * p.k_head + (lane / LPR) * p.k_slot + piece * 8);
       const T* v_lane = static_cast<const T*>(p.v) + ((int64_t)h * p.v_head + (lane / LPR) * p.v_slot + piece * 8);
-      const int key0 = s.first / KEYS * KEYS + lane, count = s.t1 - s.t0;
+      const unsigned key0 = s.first / KEYS * KEYS + lane;
+      const int count = s.t1 - s.t0;
       int page = 0, place = 0;
       bool ok = n - n0 < count && lane < KEYS && find_key(p, s.b, key0 + (s.t0 + n - n0) * KEYS, s.first, s.end, &page, &place);
       for (; n - n0 < count; n += stride) {

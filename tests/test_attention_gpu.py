@@ -68,6 +68,19 @@ def test_long_and_short_together(dtype):
     run([9000, 1, 0, 37, 4096, 2], 8, 1, 128, 16, dtype)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_lengths_up_to_the_last_one(dtype):
+    """Lengths that a tile more would take past 2^31; the sequences' pages are the same few over and over."""
+    page, g = 1 << 20, torch.Generator().manual_seed(5)
+    k, v = (torch.randn((2, page, 1, 16), generator=g).to(DT[dtype]).to(dev()) for _ in range(2))
+    table = (torch.arange(2 * 2049, dtype=torch.int32, device=dev()) % 2).view(2, 2049)
+    lens = [2 ** 31 - 1, 2 ** 31 - 20]
+    q = torch.randn((2, 2, 16), generator=g).to(DT[dtype]).to(dev())
+    got = attention.paged_attention(q, k, v, table, torch.tensor(lens, dtype=torch.int32, device=dev()), window=300)
+    want, _, eo, _ = attend(q, k, v, table, lens, 0.25, 300, 0.0)
+    check_attention(got, want, eo, dtype)
+
+
 @pytest.mark.parametrize("heads,kv,dim", [(8, 8, 128), (20, 2, 64), (16, 1, 256), (18, 9, 96)])
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 def test_items_enough_for_every_warp(heads, kv, dim, dtype):
