@@ -969,11 +969,16 @@ int kq_paged_attention(const void* q, int dtype, int64_t batch, int64_t heads, i
     return KQ_EINVAL;
   }
   const int64_t size = dtype == KQ_F32 ? 4 : 2;
-  for (int i = 0; i < 3; ++i)
-    if (k_strides[i] < 0 || v_strides[i] < 0 || k_strides[i] * size % 16 || v_strides[i] * size % 16) {
+  const int64_t extent[3] = {num_pages, page_size, kv_heads};
+  int64_t ks[3], vs[3];
+  for (int i = 0; i < 3; ++i) {
+    ks[i] = extent[i] > 1 ? k_strides[i] : 0;          // a stride that no step follows may be anything
+    vs[i] = extent[i] > 1 ? v_strides[i] : 0;
+    if (ks[i] < 0 || vs[i] < 0 || ks[i] * size % 16 || vs[i] * size % 16) {
       set_error("%s: cache strides must be multiples of 16 bytes", fn);
       return KQ_EINVAL;
     }
+  }
   if ((uintptr_t)k_cache % 16 || (uintptr_t)v_cache % 16 || (uintptr_t)q % size || (uintptr_t)out % 16 || ((uintptr_t)block_table | (uintptr_t)seq_lens | (uintptr_t)lse) % 4) {
     set_error("%s: misaligned pointer", fn);
     return KQ_EINVAL;
@@ -985,8 +990,8 @@ int kq_paged_attention(const void* q, int dtype, int64_t batch, int64_t heads, i
 
   AttnParams p;
   p.q = q; p.q_b = q_stride_batch; p.q_h = q_stride_head; p.q_words = !((uintptr_t)q % 4 || q_stride_batch % 2 || q_stride_head % 2);
-  p.k = k_cache; p.k_page = k_strides[0]; p.k_slot = k_strides[1]; p.k_head = k_strides[2];
-  p.v = v_cache; p.v_page = v_strides[0]; p.v_slot = v_strides[1]; p.v_head = v_strides[2];
+  p.k = k_cache; p.k_page = ks[0]; p.k_slot = ks[1]; p.k_head = ks[2];
+  p.v = v_cache; p.v_page = vs[0]; p.v_slot = vs[1]; p.v_head = vs[2];
   p.table = block_table; p.table_b = table_stride; p.width = (int)table_width; p.lens = seq_lens;
   p.batch = (int)batch; p.heads = (int)heads; p.kv_heads = (int)kv_heads; p.group = (int)(heads / kv_heads); p.dim = (int)head_dim;
   p.page_size = (int)page_size; p.num_pages = num_pages;

@@ -352,13 +352,14 @@ extern "C" int kq_qk_norm_rope(const void* qkv, int dtype, int64_t tokens, int64
     return KQ_EINVAL;
   }
   RopeParams p;
-  p.qkv = qkv; p.qkv_t = stride_t; p.positions = positions; p.pos64 = positions64; p.inv_freq = inv_freq;
+  p.qkv = qkv; p.qkv_t = tokens > 1 ? stride_t : 0; p.positions = positions; p.pos64 = positions64; p.inv_freq = inv_freq;
   p.qw = q_weight; p.kw = k_weight; p.w_f32 = w_dtype == KQ_F32; p.eps = eps; p.factor = factor; p.inv_dim = 1.f / (float)head_dim; p.tokens = tokens;
   p.heads = (int)heads; p.kv_heads = (int)kv_heads; p.dim = (int)head_dim; p.half = (int)(rotated / 2); p.interleaved = interleaved != 0;
   p.q = q_out; p.k = k_out; p.v = v_cache; p.slots = slots; p.slot64 = slots64; p.store = store;
   p.num_slots = store ? num_pages * page_size : 0; p.page_size = store ? (int)page_size : 1;
-  p.k_page = store ? k_strides[0] : 0; p.k_slot = store ? k_strides[1] : 0; p.k_head = store ? k_strides[2] : 0;
-  p.v_page = store ? v_strides[0] : 0; p.v_slot = store ? v_strides[1] : 0; p.v_head = store ? v_strides[2] : 0;
+  // a stride that no step follows may be anything
+  p.k_page = store && num_pages > 1 ? k_strides[0] : 0; p.k_slot = store && page_size > 1 ? k_strides[1] : 0; p.k_head = store && kv_heads > 1 ? k_strides[2] : 0;
+  p.v_page = store && num_pages > 1 ? v_strides[0] : 0; p.v_slot = store && page_size > 1 ? v_strides[1] : 0; p.v_head = store && kv_heads > 1 ? v_strides[2] : 0;
   cudaStream_t st = (cudaStream_t)stream;
   switch (dtype) {
     case KQ_F32: return run_rope<float>(p, st);

@@ -433,9 +433,9 @@ extern "C" int kq_moe_route(const void* logits, int dtype, int64_t tokens, int64
   if (tokens > 1 && stride_t < experts) { set_error("%s: rows of the logits overlap", fn); return KQ_EINVAL; }
   if ((uintptr_t)logits % (dtype == KQ_F32 ? 4 : 2) || ((uintptr_t)bias | (uintptr_t)weights | (uintptr_t)ids) % 4) { set_error("%s: misaligned pointer", fn); return KQ_EINVAL; }
   RouteParams p;
-  p.logits = logits; p.stride_t = stride_t; p.tokens = tokens; p.experts = (int)experts; p.top_k = (int)top_k; p.sigmoid = sigmoid != 0;
+  p.logits = logits; p.stride_t = tokens > 1 ? stride_t : 0; p.tokens = tokens; p.experts = (int)experts; p.top_k = (int)top_k; p.sigmoid = sigmoid != 0;
   p.groups = (int)groups; p.top_groups = (int)top_groups; p.group_size = (int)(experts / groups); p.renormalize = renormalize != 0;
-  p.bias = bias; p.scale = scale; p.bias_aligned = (uintptr_t)bias % 16 == 0; p.aligned = (uintptr_t)logits % 16 == 0 && stride_t * (dtype == KQ_F32 ? 4 : 2) % 16 == 0; p.weights = weights; p.ids = ids;
+  p.bias = bias; p.scale = scale; p.bias_aligned = (uintptr_t)bias % 16 == 0; p.aligned = (uintptr_t)logits % 16 == 0 && p.stride_t * (dtype == KQ_F32 ? 4 : 2) % 16 == 0; p.weights = weights; p.ids = ids;
   cudaStream_t st = (cudaStream_t)stream;
   switch (dtype) {
     case KQ_F32: return run_route_size<float>(p, st);

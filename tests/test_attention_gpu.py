@@ -115,6 +115,18 @@ def test_head_major_cache_and_strided_queries(dtype):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_strides_that_no_step_follows(dtype):
+    """Dimensions of one entry may carry any stride."""
+    q, k, v, table, n, got = run([30], 2, 1, 64, 32, dtype, spare=0)
+    assert k.shape == (1, 32, 1, 64)
+    odd = [c.as_strided(c.shape, (7, 64, 3, 1)) for c in (k, v)]
+    assert torch.equal(attention.paged_attention(q.as_strided(q.shape, (5, 64, 1)), *odd, table, n, scale=0.125), got)
+    k1, v1 = (c[:1, :1].contiguous().as_strided((1, 1, 1, 64), (3, 5, 7, 1)) for c in (k, v))
+    want = attention.paged_attention(q, k[:, :1].contiguous(), v[:, :1].contiguous(), table, torch.ones_like(n))
+    assert torch.equal(attention.paged_attention(q, k1, v1, table, torch.ones_like(n)), want)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_absent_pages_and_lengths_beyond_the_table(dtype):
     lens = [200, 64, 500]
     k, v, table = paged_cache(lens, 2, 64, 16, dtype, dev(), spare=2)
