@@ -279,17 +279,20 @@ __device__ __forceinline__ float4 lds4(uint32_t a) {
 
 constexpr int FM_WARPS = 4;            // each walks every fourth tile of keys of the CTA's share on its own
 constexpr int FM_START = 8;
-constexpr int FM_CTAS = 2;             // per multiprocessor
+constexpr int FM_MOST = 4;             // CTAs per multiprocessor at most
 
-// fp32: products on the fp32 pipes (three tf32 products would be needed for as many bits): a lane owns four neighbouring dimensions in every 128 (NI groups), so a key row is one dense read
-// of the warp and q and the values stay in registers; R rows x 32 / R keys of partial dot products are summed over the lanes by
-// halving the rows and keys that a lane still holds (31 shuffles for 32 sums), after which lane = (row, key) holds one score.
-// Keys and values come through a ring of cp.async copies; a lane copies exactly the bytes that it reads back.
-template <int R, int NI, int STAGES>
-__global__ void __launch_bounds__(FM_WARPS * 32) attend_fma_kernel(const AttnParams p) {
-  constexpr int KB = 32 / R;                      // keys of a tile
+// fp32: products on the fp32 pipes (as many bits from the tensor cores would take three tf32 products).  A lane owns four neighbouring
+// dimensions of a key, and NI times as many in steps of 128 from 128 on; up to 64 dimensions a warp covers two keys at once, one on either
+// LD = 16 lanes.  A key row is one dense read, q and the values stay in registers.  R rows x KB keys of partial dot products are summed over
+// the LD lanes by halving the rows and keys that a lane still holds (31 shuffles for 32 sums), after which a lane holds one
+// score.  Keys and values come through a ring of cp.async copies; a lane copies exactly the bytes that it reads back.
+template <int R, int LD, int NI, int STAGES, int KB, int LEAST>
+__global__ void __launch_bounds__(FM_WARPS * 32, LEAST) attend_fma_kernel(const AttnParams p) {
+  constexpr int SIDES = 32 / LD, KT = KB * SIDES;     // keys next to each other, keys of a tile
+  constexpr int N = R * KB, SH = LD / N, RL = LD / R;   // scores of a side, lanes that hold the same one, lanes of a row
+  static_assert(N <= LD && (LD == 32 || NI == 1), "a score per lane");
   constexpr int CH = 16;                          // bytes of a lane's piece of a row
-  constexpr int ROW = NI * 32 * CH;
+  constexpr int ROW = NI * 32 * CH;               // of SIDES keys
   constexpr int SLOT = 2 * KB * ROW;              // keys, then values
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int64_t s_red[FM_WARPS], s_div[2];
@@ -300,7 +303,7 @@ __global__ void __launch_bounds__(FM_WARPS * 32) attend_fma_kernel(const AttnPar
   pdl_trigger();
   pdl_wait();
 
-  Walk<KB, FM_START> walk;
+  Walk<KT, FM_START> walk;
   if (p.split) {
     walk.begin_share(p, s_red, s_div, FM_WARPS * 32, blockIdx.x, gridDim.x);
     if (tid == 0) p.meta[blockIdx.x] = make_int2(-1, 0);
@@ -313,7 +316,7 @@ __global__ void __launch_bounds__(FM_WARPS * 32) attend_fma_kernel(const AttnPar
     const int b = s.b, first = s.first, end = s.end, t0 = s.t0, t1 = s.t1;
     const int h = s.sub / p.row_tiles, x = s.sub - h * p.row_tiles;
     const int head0 = h * p.group + x * p.rows, rows = min(p.rows, p.group - x * p.rows);
-    const int key0 = first / KB * KB;              // tiles start at multiples of KB
+    const int key0 = first / KT * KT;              // tiles start at multiples of KT
 
     float q[R][NI * 4], o[R][NI * 4];
 #pragma unroll
@@ -322,7 +325,7 @@ __global__ void __launch_bounds__(FM_WARPS * 32) attend_fma_kernel(const AttnPar
       for (int i = 0; i < NI; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int d = i * 128 + lane * 4 + e;
+          const int d = i * 128 + lane % LD * 4 + e;
           q[r][i * 4 + e] = r < rows && d < p.dim ? static_cast<const float*>(p.q)[(int64_t)b * p.q_b + (int64_t)(head0 + r) * p.q_h + d] : 0.f;
           o[r][i * 4 + e] = 0.f;
         }
@@ -331,19 +334,20 @@ __global__ void __launch_bounds__(FM_WARPS * 32) attend_fma_kernel(const AttnPar
     uint32_t live_ring[STAGES];
     auto fetch = [&](int t, int slot) -> uint32_t {
       int page = 0, place = 0;
-      const unsigned j = (unsigned)key0 + (unsigned)t * KB + (lane % KB);
+      const unsigned j = (unsigned)key0 + (unsigned)t * KT + (lane % KT);
       const bool ok = t < t1 && find_key(p, b, j, first, end, &page, &place);
       const uint32_t live = __ballot_sync(0xffffffffu, ok);
       if (t < t1) {
 #pragma unroll
         for (int kk = 0; kk < KB; ++kk) {
-          const int64_t pg = __shfl_sync(0xffffffffu, page, kk), pl = __shfl_sync(0xffffffffu, place, kk);
-          const bool on = live >> kk & 1;
+          const int row = kk * SIDES + lane / LD;
+          const int64_t pg = __shfl_sync(0xffffffffu, page, row), pl = __shfl_sync(0xffffffffu, place, row);
+          const bool on = live >> row & 1;
           const float* kr = static_cast<const float*>(p.k) + (on ? pg * p.k_page + pl * p.k_slot + h * p.k_head : 0);
           const float* vr = static_cast<const float*>(p.v) + (on ? pg * p.v_page + pl * p.v_slot + h * p.v_head : 0);
 #pragma unroll
           for (int i = 0; i < NI; ++i) {
-            const int d = i * 128 + lane * 4;
+            const int d = i * 128 + lane % LD * 4;
             const bool in = on && d < p.dim;       // otherwise zeros are written and nothing is read
             cp_async(ring + slot * SLOT + kk * ROW + i * 32 * CH, kr + (in ? d : 0), in);
             cp_async(ring + slot * SLOT + (KB + kk) * ROW + i * 32 * CH, vr + (in ? d : 0), in);
@@ -365,7 +369,7 @@ __global__ void __launch_bounds__(FM_WARPS * 32) attend_fma_kernel(const AttnPar
       cp_wait<STAGES - 1>();
       const uint32_t at = ring + slot * SLOT;
       slot = slot + 1 == STAGES ? 0 : slot + 1;
-      float v[32];                                 // index r * KB + kk
+      float v[N];                                 // index r * KB + kk
 #pragma unroll
       for (int kk = 0; kk < KB; ++kk) {
 #pragma unroll
@@ -383,21 +387,24 @@ __global__ void __launch_bounds__(FM_WARPS * 32) attend_fma_kernel(const AttnPar
         }
       }
 #pragma unroll
-      for (int half = 16; half > 0; half >>= 1) {
-        const bool up = lane & half;
+      for (int half = N / 2; half > 0; half >>= 1) {
+        const bool up = lane & (half * SH);
 #pragma unroll
         for (int i = 0; i < half; ++i) {
           const float send = up ? v[i] : v[i + half];
           const float keep = up ? v[i + half] : v[i];
-          v[i] = keep + __shfl_xor_sync(0xffffffffu, send, half);
+          v[i] = keep + __shfl_xor_sync(0xffffffffu, send, half * SH);
         }
       }
+#pragma unroll
+      for (int d = 1; d < SH; d <<= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], d);
       float sc = v[0] * p.scale;
       if (p.cap > 0.f) sc = p.cap * AT_LOG2E * tanhf(sc / p.cap);
-      if (!(got >> (lane % KB) & 1)) sc = -INFINITY;
+      if (!(got >> (lane / SH % KB * SIDES + lane / LD) & 1)) sc = -INFINITY;
       float top = sc;
 #pragma unroll
-      for (int d = 1; d < KB; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+      for (int d = SH; d < RL; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+      if constexpr (SIDES == 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, LD));
       const float mn = fmaxf(m, top);
       const float use = mn == -INFINITY ? 0.f : mn;
       if (__any_sync(0xffffffffu, mn > m)) {       // a new maximum in some row: rescale what is there
@@ -405,7 +412,7 @@ __global__ void __launch_bounds__(FM_WARPS * 32) attend_fma_kernel(const AttnPar
         l *= f;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          const float fr = __shfl_sync(0xffffffffu, f, r * KB);
+          const float fr = __shfl_sync(0xffffffffu, f, r * RL);
 #pragma unroll
           for (int i = 0; i < NI * 4; ++i) o[r][i] *= fr;
         }
@@ -420,7 +427,7 @@ __global__ void __launch_bounds__(FM_WARPS * 32) attend_fma_kernel(const AttnPar
           const float4 vx = lds4(at + (KB + kk) * ROW + i * 32 * CH);
 #pragma unroll
           for (int r = 0; r < R; ++r) {
-            const float wr = __shfl_sync(0xffffffffu, w, r * KB + kk);
+            const float wr = __shfl_sync(0xffffffffu, w, (r * KB + kk) * SH + lane / LD * LD);
             o[r][i * 4] = fmaf(wr, vx.x, o[r][i * 4]); o[r][i * 4 + 1] = fmaf(wr, vx.y, o[r][i * 4 + 1]);
             o[r][i * 4 + 2] = fmaf(wr, vx.z, o[r][i * 4 + 2]); o[r][i * 4 + 3] = fmaf(wr, vx.w, o[r][i * 4 + 3]);
           }
@@ -430,14 +437,21 @@ __global__ void __launch_bounds__(FM_WARPS * 32) attend_fma_kernel(const AttnPar
     cp_wait<0>();
     __syncthreads();                               // the ring becomes the place where the warps' results meet
 #pragma unroll
-    for (int d = 1; d < KB; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
-    if (lane % KB == 0) s_ml[warp * R + lane / KB] = make_float2(m, l);
+    for (int d = SH; d < RL; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+    if constexpr (SIDES == 2) {
+      l += __shfl_xor_sync(0xffffffffu, l, LD);
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[r][e] += __shfl_xor_sync(0xffffffffu, o[r][e], LD);
+    }
+    if (lane < LD && lane % RL == 0) s_ml[warp * R + lane / RL] = make_float2(m, l);
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
-        const int d = i * 128 + lane * 4;
-        if (d < p.dim) *reinterpret_cast<float4*>(s_o + (warp * R + r) * p.dim + d) = make_float4(o[r][i * 4], o[r][i * 4 + 1], o[r][i * 4 + 2], o[r][i * 4 + 3]);
+        const int d = i * 128 + lane * 4;          // of both sides, where there are two, the first one
+        if (d < p.dim && lane < LD) *reinterpret_cast<float4*>(s_o + (warp * R + r) * p.dim + d) = make_float4(o[r][i * 4], o[r][i * 4 + 1], o[r][i * 4 + 2], o[r][i * 4 + 3]);
       }
     __syncthreads();
     const int part = part_of(s, blockIdx.x);
@@ -852,18 +866,18 @@ int launch_both(void (*kern)(const AttnParams), AttnParams& p, int threads, int 
   return KQ_OK;
 }
 
-template <int R, int NI>
+template <int R, int LD, int NI, int STAGES, int KB, int CTAS, int LEAST>
 int run_fma(AttnParams& p, cudaStream_t st) {
-  constexpr int STAGES = R == 8 ? 3 : 2;
-  constexpr int ring = FM_WARPS * STAGES * 2 * (32 / R) * NI * 512, join = FM_WARPS * R * NI * 128 * 4;
+  constexpr int ring = FM_WARPS * STAGES * 2 * KB * NI * 512, join = FM_WARPS * R * NI * 128 * 4;
   constexpr int smem = ring > join ? ring : join;
-  auto kern = attend_fma_kernel<R, NI, STAGES>;
+  static_assert(CTAS <= (NI == 2 ? 2 : FM_MOST), "more workers than scratch_of counts");
+  auto kern = attend_fma_kernel<R, LD, NI, STAGES, KB, LEAST>;
   static DeviceOnce attr_set;
   if (attr_set.first_time()) {
     KQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     attr_set.done();
   }
-  return launch_both<float>(kern, p, FM_WARPS * 32, smem, FM_CTAS, st);
+  return launch_both<float>(kern, p, FM_WARPS * 32, smem, CTAS, st);
 }
 
 template <typename T, int DP, bool TWO>
@@ -885,10 +899,16 @@ void set_rows(AttnParams& p, int most) {
   p.row_tiles = (p.group + p.rows - 1) / p.rows;
 }
 
+// Tiles of up to 4 or 8 rows.  Bound by instruction issue, so the tile, the ring and the registers are those that keep most warps busy;
+// us before (tiles of 32 / R keys, a warp per key, two CTAs) / as chosen, 16 sequences of 4000 tokens, 8 key heads: heads of 64 in
+// groups of 4 103 / 58, of 8 197 / 86; heads of 128 in groups of 8 197 / 139 (2.7 / 3.8 TB/s); 33 sequences of up to 10000 with heads
+// of 256 in groups of 4 120 / 104; listed in turn: stages, keys side by side, CTAs per multiprocessor, and those that the registers must allow
+// (at least; with 155 instead of 128 registers <4, 32, 1> takes 72 instead of 60 us for 16 sequences of 900..3100).
 int run_f32(AttnParams& p, cudaStream_t st) {
   set_rows(p, 8);
-  if (p.rows <= 4) return p.dim > 128 ? run_fma<4, 2>(p, st) : run_fma<4, 1>(p, st);
-  return p.dim > 128 ? run_fma<8, 2>(p, st) : run_fma<8, 1>(p, st);
+  if (p.rows <= 4)
+    return p.dim > 128 ? run_fma<4, 32, 2, 3, 4, 2, 2>(p, st) : p.dim > 64 ? run_fma<4, 32, 1, 2, 8, 2, 4>(p, st) : run_fma<4, 16, 1, 2, 4, 4, 4>(p, st);
+  return p.dim > 128 ? run_fma<8, 32, 2, 3, 4, 2, 2>(p, st) : p.dim > 64 ? run_fma<8, 32, 1, 2, 4, 3, 3>(p, st) : run_fma<8, 16, 1, 2, 2, 4, 4>(p, st);
 }
 
 // From how many items on a worker is a warp.  As warps / as CTAs, us, 148 multiprocessors: 256 sequences of 1..500 tokens with 8 key heads
@@ -915,7 +935,7 @@ Scratch scratch_of(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim) 
   p.group = (int)(heads / kv_heads);
   set_rows(p, 16);
   const int64_t rows = p.rows > 8 ? p.rows : 8;              // of either type's tiles
-  const int64_t workers = sm_count() * (solo_pays(batch * kv_heads * p.row_tiles, true) ? 4 : FM_CTAS);
+  const int64_t workers = sm_count() * (solo_pays(batch * kv_heads * p.row_tiles, true) || dim <= 128 ? FM_MOST : 2);   // fp32 heads above 128 have two
   auto up = [](int64_t bytes) { return (size_t)((bytes + 255) / 256 * 256); };
   Scratch s;
   s.o = 0;

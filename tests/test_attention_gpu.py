@@ -92,6 +92,15 @@ def test_items_enough_for_every_warp(heads, kv, dim, dtype):
     run(lens, heads, kv, dim, 8, dtype, window=70)
 
 
+@pytest.mark.parametrize("heads,kv", [(1, 1), (4, 1), (10, 2), (8, 1), (12, 1)])
+@pytest.mark.parametrize("dim", [32, 64, 128, 144, 256])
+def test_f32_tiles(heads, kv, dim):
+    """Every tile of the fp32 form, at lengths that end inside one, whole and divided."""
+    run([5, 0, 190, 64, 1], heads, kv, dim, 16, "f32", seed=dim)
+    run([1203, 7, 0, 402], heads, kv, dim, 24, "f32", seed=dim)
+    run([1203, 7, 0, 402], heads, kv, dim, 16, "f32", window=333, cap=9.0, seed=dim)
+
+
 def test_many_sequences():
     """More sequences than one scan step of a CTA covers, in an order of lengths that a static split would serve badly."""
     lens = [(i * i) % 97 for i in range(700)]
