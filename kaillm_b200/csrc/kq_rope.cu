@@ -65,13 +65,11 @@ __device__ __forceinline__ T* target_of(const RopeParams& p, int64_t t, int head
              : static_cast<T*>(p.v) + page * p.v_page + place * p.v_slot + h * p.v_head;
 }
 
-// Rows of 16-byte pieces.  A lane owns two pieces A and B of a head whose values turn into one another: a pair of pieces half the rotated
-// width apart, or (interleaved, and behind the rotated part, where nothing turns) two neighbouring ones; D / 2V lanes share a
-// head (V values per piece), rounded up to a power of two for the sum of squares, and the other lanes take further heads.  So nothing but
-// that sum crosses lanes, and out_A = A * c0 + A' * c1, out_B = B * c2 + B' * c3 (A', B': the partners) with factors made of the norm's
-// weight and the token's cosine and sine, which a lane forms once for all heads of a kind and token and keeps in registers.
-// A CTA forms its token's angles while the first rows of queries, keys and values are on their way; its warps share the token's steps
-// (a step: as many heads as a warp holds).  SPREAD: queries, keys and values in CTAs of their own (blockIdx.z).
+// Rows of 16-byte pieces.  A lane owns two pieces A and B of a head, half the rotated width apart (behind the rotated part, half of what is
+// left), so that the values of a pair stand at the same place of A and B, or interleaved next to each other in one of them; D / 2V lanes
+// share a head (V values per piece), rounded up to a power of two for the sum of squares, and the other lanes take further heads.  So nothing
+// but that sum crosses lanes, and out_A = A * c0 + A' * c1, out_B = B * c2 + B' * c3 (A', B': the partners) with factors made of the
+// norm's weight and the token's cosine and sine, which a lane forms once for all heads of a kind and token and keeps in registers.
 typedef unsigned long long f32x2;
 __device__ __forceinline__ f32x2 pack2(float x, float y) { f32x2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y)); return r; }
 __device__ __forceinline__ float2 unpack2(f32x2 v) { float2 r; asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v)); return r; }
@@ -113,74 +111,46 @@ __device__ __forceinline__ void weights_of(const RopeParams& p, const void* w, i
   }
 }
 
-// HALVES: pairs half a head apart and nothing unturned, so that no lane has to choose its partners.
-template <typename T, int WARPS, int AHEAD, bool HALVES, bool SPREAD>
-__global__ void __launch_bounds__(WARPS * 32, SPREAD ? 4 : 16 / WARPS) rope_rows_kernel(const RopeParams p, int lanes_log2) {
-  constexpr int V = 16 / (int)sizeof(T), P = V / 2;                               // values, pairs of them in a piece
-  __shared__ float2 s_turn[RP_MAX_DIM / 2];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t t = blockIdx.x;
-  const bool q_here = !SPREAD || blockIdx.z == 0, k_here = !SPREAD || blockIdx.z == 1, v_here = p.store && (!SPREAD || blockIdx.z == 2);
-  const int unit = lane & ((1 << lanes_log2) - 1);                               // this lane's pieces
-  const bool active = unit * 2 * V < p.dim;
-  const bool turned = HALVES || unit * 2 * V < 2 * p.half, apart = HALVES || (turned && !p.interleaved);
-  const int da = apart ? unit * V : unit * 2 * V, db = apart ? p.half + unit * V : unit * 2 * V + V;
-  const int per = 32 >> lanes_log2, step = gridDim.y * WARPS * per;               // heads of a step, from step to step of this warp
-  const int h0 = (blockIdx.y * WARPS + warp) * per + (lane >> lanes_log2);
-  pdl_trigger();
-  pdl_wait();
-  const T* src = static_cast<const T*>(p.qkv) + t * p.qkv_t + h0 * p.dim;
-  auto load = [&](const T* from, bool on, uint4& va, uint4& vb) {
-    va = vb = make_uint4(0, 0, 0, 0);
-    if (on) { va = *reinterpret_cast<const uint4*>(from + da); vb = *reinterpret_cast<const uint4*>(from + db); }
-  };
-  // the first steps of all three kinds are on their way before the angles are formed
-  uint4 a[AHEAD], b[AHEAD], ka, kb, va, vb;
-#pragma unroll
-  for (int i = 0; i < AHEAD; ++i) load(src + i * step * p.dim, q_here && active && h0 + i * step < p.heads, a[i], b[i]);
-  const T* k_src = src + p.heads * p.dim;
-  const T* v_src = k_src + p.kv_heads * p.dim;
-  load(k_src, k_here && active && h0 < p.kv_heads, ka, kb);
-  load(v_src, v_here && active && h0 < p.kv_heads, va, vb);
+enum RopeForm { HALVES, NEIGHBOURS, MIXED };   // all values turn, in pairs half a head apart; all, interleaved; some do not
 
-  const int64_t pos = index_at(p.positions, p.pos64, t);
-  for (int i = threadIdx.x; i < p.half; i += WARPS * 32) s_turn[i] = angle_of(p, pos, i);
-  T* k_dst = static_cast<T*>(p.k) + (t * p.kv_heads + h0) * p.dim;
-  T* v_dst = nullptr;
-  int64_t k_head = p.dim;
-  bool kept = active;
-  if (p.store && active) {
-    const int64_t slot = index_at(p.slots, p.slot64, t);
-    kept = slot >= 0 && slot < p.num_slots;
-    if (kept) {
-      const int64_t page = slot >> 31 ? slot / p.page_size : (int64_t)((uint32_t)slot / (uint32_t)p.page_size), place = slot - page * p.page_size;
-      k_dst = static_cast<T*>(p.k) + page * p.k_page + place * p.k_slot + h0 * p.k_head;
-      v_dst = static_cast<T*>(p.v) + page * p.v_page + place * p.v_slot + h0 * p.v_head;
-    }
-    k_head = p.k_head;
-  }
-  __syncthreads();
-
+// A lane's pieces of a head and what they are multiplied by.  Only MIXED has lanes that differ, and choose their partners.
+template <typename T, RopeForm FORM> struct RopeLane {
+  static constexpr int V = 16 / (int)sizeof(T), P = V / 2;                        // values, pairs of them in a piece
+  int log2;                                                                       // of the lanes of a head
+  bool active, turned, apart;
+  int da, db;                                                                     // first values of the pieces
   f32x2 c0[P], c1[P], c2[P], c3[P];
-  const float2* turn = s_turn + unit * V;
-  auto factors = [&](const void* w) {
+
+  __device__ __forceinline__ RopeLane(const RopeParams& p, int lanes_log2) : log2(lanes_log2) {
+    const int unit = threadIdx.x & ((1 << log2) - 1);
+    active = unit * 2 * V < p.dim;
+    turned = FORM != MIXED || unit * V < p.half;
+    apart = FORM == HALVES || (FORM == MIXED && turned && !p.interleaved);
+    da = turned ? unit * V : p.half + unit * V;                                   // 2 half + (unit V - half)
+    db = turned ? p.half + unit * V : p.dim / 2 + unit * V;                       // and (dim - 2 half) / 2 behind
+  }
+  __device__ __forceinline__ int head_of_step() const { return (threadIdx.x & 31) >> log2; }
+
+  __device__ __forceinline__ void factors(const RopeParams& p, const void* w, const float2* s_turn) {
     float wa[V], wb[V];
     weights_of<T, V>(p, active ? w : nullptr, da, wa);
     weights_of<T, V>(p, active ? w : nullptr, db, wb);
+    const bool on = turned && active;
 #pragma unroll
     for (int e = 0; e < V; e += 2) {
-      if (HALVES || apart || !turned) {
-        const float2 u = turned && active ? turn[e] : make_float2(1.f, 0.f), v = turned && active ? turn[e + 1] : make_float2(1.f, 0.f);
+      if (FORM != NEIGHBOURS && (apart || !turned)) {
+        const float2 u = on ? s_turn[da + e] : make_float2(1.f, 0.f), v = on ? s_turn[da + e + 1] : make_float2(1.f, 0.f);
         c0[e / 2] = pack2(wa[e] * u.x, wa[e + 1] * v.x); c1[e / 2] = pack2(-wb[e] * u.y, -wb[e + 1] * v.y);
         c2[e / 2] = pack2(wb[e] * u.x, wb[e + 1] * v.x); c3[e / 2] = pack2(wa[e] * u.y, wa[e + 1] * v.y);
       } else {
-        const float2 u = turn[e / 2], v = turn[P + e / 2];
+        const float2 u = on ? s_turn[(da + e) / 2] : make_float2(1.f, 0.f), v = on ? s_turn[(db + e) / 2] : make_float2(1.f, 0.f);
         c0[e / 2] = pack2(wa[e] * u.x, wa[e + 1] * u.x); c1[e / 2] = pack2(-wa[e + 1] * u.y, wa[e] * u.y);
         c2[e / 2] = pack2(wb[e] * v.x, wb[e + 1] * v.x); c3[e / 2] = pack2(-wb[e + 1] * v.y, wb[e] * v.y);
       }
     }
-  };
-  auto turn_and_put = [&](uint4 ra, uint4 rb, bool normed, T* dst, bool on) {
+  }
+  // all lanes of the warp together; a lane without a head has zeros
+  __device__ __forceinline__ void turn(const RopeParams& p, uint4& ra, uint4& rb, bool normed) const {
     f32x2 x[P], y[P];
 #pragma unroll
     for (int e = 0; e < P; ++e) { x[e] = widen<T>(ra, e); y[e] = widen<T>(rb, e); }
@@ -190,7 +160,7 @@ __global__ void __launch_bounds__(WARPS * 32, SPREAD ? 4 : 16 / WARPS) rope_rows
 #pragma unroll
       for (int e = 0; e < P; ++e) sq = fma2(y[e], y[e], e ? fma2(x[e], x[e], sq) : sq);
       float sum = unpack2(sq).x + unpack2(sq).y;
-      for (int m = 1 << lanes_log2 >> 1; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+      for (int m = 1 << log2 >> 1; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
       const float f = rsqrtf(fmaf(sum, p.inv_dim, p.eps));
       inv = pack2(f, f);
     }
@@ -203,40 +173,175 @@ __global__ void __launch_bounds__(WARPS * 32, SPREAD ? 4 : 16 / WARPS) rope_rows
       narrow<T>(ra, e, u);
       narrow<T>(rb, e, v);
     }
-    if (on) { *reinterpret_cast<uint4*>(dst + da) = ra; *reinterpret_cast<uint4*>(dst + db) = rb; }
+  }
+  __device__ __forceinline__ void put(T* dst, const uint4& ra, const uint4& rb) const {
+    *reinterpret_cast<uint4*>(dst + da) = ra;
+    *reinterpret_cast<uint4*>(dst + db) = rb;
+  }
+};
+
+// Where keys and values of token t go; false: nowhere.  Their first head; k_head: from head to head of the keys.
+template <typename T>
+__device__ __forceinline__ bool rows_of(const RopeParams& p, int64_t t, T** k, T** v, int64_t* k_head) {
+  *k = static_cast<T*>(p.k) + t * p.kv_heads * p.dim;
+  *v = nullptr;
+  *k_head = p.dim;
+  if (!p.store) return true;
+  const int64_t slot = index_at(p.slots, p.slot64, t);
+  if (slot < 0 || slot >= p.num_slots) return false;
+  const int64_t page = slot >> 31 ? slot / p.page_size : (int64_t)((uint32_t)slot / (uint32_t)p.page_size), place = slot - page * p.page_size;
+  *k = static_cast<T*>(p.k) + page * p.k_page + place * p.k_slot;
+  *v = static_cast<T*>(p.v) + page * p.v_page + place * p.v_slot;
+  *k_head = p.k_head;
+  return true;
+}
+
+// A CTA per token, or with SPREAD three (queries, keys and values: blockIdx.z); its warps share the token's steps (a step: as many heads as a
+// warp holds).  The first rows of all kinds are on their way while the angles are formed.
+template <typename T, int WARPS, int AHEAD, RopeForm FORM, bool SPREAD>
+__global__ void __launch_bounds__(WARPS * 32, SPREAD ? 4 : 16 / WARPS) rope_rows_kernel(const RopeParams p, int lanes_log2) {
+  __shared__ float2 s_turn[RP_MAX_DIM / 2];
+  RopeLane<T, FORM> L(p, lanes_log2);
+  const int warp = threadIdx.x >> 5, sub = L.head_of_step();
+  const int64_t t = blockIdx.x;
+  const bool q_here = !SPREAD || blockIdx.z == 0, k_here = !SPREAD || blockIdx.z == 1, v_here = p.store && (!SPREAD || blockIdx.z == 2);
+  const int per = 32 >> lanes_log2, step = gridDim.y * WARPS * per;               // heads of a step, from step to step of this warp
+  const int h0 = (blockIdx.y * WARPS + warp) * per + sub;
+  pdl_trigger();
+  pdl_wait();
+  const T* src = static_cast<const T*>(p.qkv) + t * p.qkv_t + h0 * p.dim;
+  auto load = [&](const T* from, bool on, uint4& va, uint4& vb) {
+    va = vb = make_uint4(0, 0, 0, 0);
+    if (on) { va = *reinterpret_cast<const uint4*>(from + L.da); vb = *reinterpret_cast<const uint4*>(from + L.db); }
   };
+  uint4 a[AHEAD], b[AHEAD], ka, kb, va, vb;
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) load(src + i * step * p.dim, q_here && L.active && h0 + i * step < p.heads, a[i], b[i]);
+  const T* k_src = src + p.heads * p.dim;
+  const T* v_src = k_src + p.kv_heads * p.dim;
+  load(k_src, k_here && L.active && h0 < p.kv_heads, ka, kb);
+  load(v_src, v_here && L.active && h0 < p.kv_heads, va, vb);
+
+  const int64_t pos = index_at(p.positions, p.pos64, t);
+  for (int i = threadIdx.x; i < p.half; i += WARPS * 32) s_turn[i] = angle_of(p, pos, i);
+  T *k_dst, *v_dst;
+  int64_t k_head;
+  const bool kept = L.active && rows_of<T>(p, t, &k_dst, &v_dst, &k_head);
+  __syncthreads();
+
   if (v_here) {                                                   // values go as they came
-    for (int h = h0; h - (lane >> lanes_log2) < p.kv_heads; h += step) {
-      if (kept && active && h < p.kv_heads) { *reinterpret_cast<uint4*>(v_dst + da) = va; *reinterpret_cast<uint4*>(v_dst + db) = vb; }
+    for (int h = h0; h - sub < p.kv_heads; h += step) {
+      if (kept && h < p.kv_heads) L.put(v_dst + h * p.v_head, va, vb);
       v_src += step * p.dim;
-      v_dst += step * p.v_head;
-      load(v_src, active && h + step < p.kv_heads, va, vb);
+      load(v_src, L.active && h + step < p.kv_heads, va, vb);
     }
   }
-  factors(q_here ? p.qw : p.kw);
+  L.factors(p, q_here ? p.qw : p.kw, s_turn);
   T* dst = static_cast<T*>(p.q) + (t * p.heads + h0) * p.dim;
   src += AHEAD * step * p.dim;
-  for (int h = h0; q_here && h - (lane >> lanes_log2) < p.heads; h += AHEAD * step) {
+  for (int h = h0; q_here && h - sub < p.heads; h += AHEAD * step) {
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
       const int hi = h + i * step;
-      if (hi - (lane >> lanes_log2) >= p.heads) break;
-      const uint4 ra = a[i], rb = b[i];
-      load(src, active && hi + AHEAD * step < p.heads, a[i], b[i]);
+      if (hi - sub >= p.heads) break;
+      uint4 ra = a[i], rb = b[i];
+      load(src, L.active && hi + AHEAD * step < p.heads, a[i], b[i]);
       src += step * p.dim;
-      turn_and_put(ra, rb, p.qw != nullptr, dst, active && hi < p.heads);
+      L.turn(p, ra, rb, p.qw != nullptr);
+      if (L.active && hi < p.heads) L.put(dst, ra, rb);
       dst += step * p.dim;
     }
   }
-  if (!k_here || h0 - (lane >> lanes_log2) >= p.kv_heads) return;
-  if (!SPREAD && p.kw != p.qw) factors(p.kw);
-  for (int h = h0; h - (lane >> lanes_log2) < p.kv_heads; h += step) {
-    const uint4 ra = ka, rb = kb;
+  if (!k_here || h0 - sub >= p.kv_heads) return;
+  if (!SPREAD && p.kw != p.qw) L.factors(p, p.kw, s_turn);
+  for (int h = h0; h - sub < p.kv_heads; h += step) {
+    uint4 ra = ka, rb = kb;
     k_src += step * p.dim;
-    load(k_src, active && h + step < p.kv_heads, ka, kb);
-    turn_and_put(ra, rb, p.kw != nullptr, k_dst, kept && active && h < p.kv_heads);
-    k_dst += step * k_head;
+    load(k_src, L.active && h + step < p.kv_heads, ka, kb);
+    L.turn(p, ra, rb, p.kw != nullptr);
+    if (kept && h < p.kv_heads) L.put(k_dst + h * k_head, ra, rb);
   }
+}
+
+// 16 bytes, or with live = false 16 bytes of zeros and no read
+__device__ __forceinline__ void copy_piece(uint4* dst, const void* src, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+
+// Many tokens: a warp per token walks its values, queries and keys through a ring in shared memory, two steps in use and the others under
+// way.  A lane copies the pieces that it reads back itself, so nothing but its own copies is waited for.
+// Bound by memory: 8192 tokens with 40 + 2 x 8 heads of 128, norms and cache, bf16 (235 MB) 41.5 us, 5.7 TB/s; interleaved 40.9; fp32 78. Two warps
+// per token with their next rows in registers (rope_rows_kernel) took 49.6, 52 and 84: as much on the way as registers hold, at 16 warps per
+// multiprocessor.  Steps of the ring and least warps of a multiprocessor: 16-bit 6 and 18 (41.5; 8 and 18 43.2, 5 and 20 41.8, 6 and 16
+// 44.9), fp32 10 and 16 (4096 tokens 42.4; 6 and 18 46.9), whose heads take twice the steps.
+template <typename T> constexpr int RING_WARPS = sizeof(T) == 4 ? 16 : 18;
+template <typename T, RopeForm FORM>
+__global__ void __launch_bounds__(32, RING_WARPS<T>) rope_ring_kernel(const RopeParams p, int lanes_log2) {
+  constexpr int RING_STEPS = sizeof(T) == 4 ? 10 : 6;
+  __shared__ float2 s_turn[RP_MAX_DIM / 2];
+  __shared__ uint4 s_ring[RING_STEPS][2][32];
+  RopeLane<T, FORM> L(p, lanes_log2);
+  const int lane = threadIdx.x, h0 = L.head_of_step();
+  const int64_t t = blockIdx.x;
+  const int per = 32 >> lanes_log2, nq = (p.heads + per - 1) >> (5 - lanes_log2), nk = (p.kv_heads + per - 1) >> (5 - lanes_log2), nv = p.store ? nk : 0;
+  pdl_trigger();
+  pdl_wait();
+  const T* src = static_cast<const T*>(p.qkv) + t * p.qkv_t;
+  int into = 0, from = 0, next = RING_STEPS - 2;                                  // places in the ring; the step to be fetched
+  auto fetch = [&](int s) {
+    if (s < nv + nq + nk) {
+      const bool is_v = s < nv, is_q = !is_v && s < nv + nq;
+      const int h = h0 + (is_v ? s : is_q ? s - nv : s - nv - nq) * per;
+      const bool on = L.active && h < (is_q ? p.heads : p.kv_heads);
+      const T* row = src + (on ? (h + (is_q ? 0 : is_v ? p.heads + p.kv_heads : p.heads)) * p.dim : 0);
+      copy_piece(&s_ring[into][0][lane], row + (on ? L.da : 0), on);
+      copy_piece(&s_ring[into][1][lane], row + (on ? L.db : 0), on);
+    }
+    into = into + 1 == RING_STEPS ? 0 : into + 1;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int s = 0; s < RING_STEPS - 2; ++s) fetch(s);
+  auto take = [&](uint4& ra, uint4& rb) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(RING_STEPS - 3) : "memory");
+    ra = s_ring[from][0][lane];
+    rb = s_ring[from][1][lane];
+    from = from + 1 == RING_STEPS ? 0 : from + 1;
+    fetch(next++);                                                                // into the place of the step before the last one
+  };
+
+  const int64_t pos = index_at(p.positions, p.pos64, t);
+  for (int i = lane; i < p.half; i += 32) s_turn[i] = angle_of(p, pos, i);
+  T *k_dst, *v_dst;
+  int64_t k_head;
+  const bool kept = L.active && rows_of<T>(p, t, &k_dst, &v_dst, &k_head);
+  uint4 ra, rb, sa, sb;
+  for (int i = 0, h = h0; i < nv; ++i, h += per) {
+    take(ra, rb);
+    if (kept && h < p.kv_heads) L.put(v_dst + h * p.v_head, ra, rb);
+  }
+  __syncwarp();
+  // two steps at a time, so that one's sum over the lanes overlaps with the other's
+  auto turn_all = [&](int steps, int heads, bool normed, T* dst, int64_t to_head, bool on) {
+    int i = 0, h = h0;
+    for (; i + 2 <= steps; i += 2, h += 2 * per) {
+      take(ra, rb);
+      take(sa, sb);
+      L.turn(p, ra, rb, normed);
+      if (on && h < heads) L.put(dst + h * to_head, ra, rb);
+      L.turn(p, sa, sb, normed);
+      if (on && h + per < heads) L.put(dst + (h + per) * to_head, sa, sb);
+    }
+    if (i < steps) {
+      take(ra, rb);
+      L.turn(p, ra, rb, normed);
+      if (on && h < heads) L.put(dst + h * to_head, ra, rb);
+    }
+  };
+  L.factors(p, p.qw, s_turn);
+  turn_all(nq, p.heads, p.qw != nullptr, static_cast<T*>(p.q) + t * p.heads * p.dim, p.dim, L.active);
+  if (p.kw != p.qw) L.factors(p, p.kw, s_turn);
+  turn_all(nk, p.kv_heads, p.kw != nullptr, k_dst, k_head, kept);
 }
 
 // Any even width, any alignment: one CTA per token (or part of its heads), a warp per head, the angles once into shared memory.
@@ -293,26 +398,33 @@ bool in_pieces(const RopeParams& p) {
   return p.dim % (2 * V) == 0 && p.half % V == 0 && p.dim <= 64 * V && strides % V == 0 && at % 16 == 0;
 }
 
+template <typename T, RopeForm FORM>
+int run_rows(const RopeParams& p, cudaStream_t st) {
+  int log2 = 0;
+  while ((1 << log2) * (32 / (int)sizeof(T)) < p.dim) ++log2;
+  const bool pdl = options().pdl != 0;
+  // Few tokens, more than a few, more than a wave of ring_kernel's warps; with 40 + 2 x 8 heads of 128, us: 16 tokens 2.9 spread; 600 7.0 by two warps
+  // each, 16 spread, 9.0 by the ring; 2000 16.6, 54.7, 16.0; 5000 33.5, 132, 28.8
+  if (p.tokens >= 20 * sm_count()) {
+    KQ_CUDA_TRY(launch_pdl(rope_ring_kernel<T, FORM>, dim3((unsigned)p.tokens), dim3(32), (size_t)0, st, pdl, p, log2));
+  } else if (p.tokens >= 4 * sm_count()) {
+    // two warps walk a token's heads
+    KQ_CUDA_TRY(launch_pdl(rope_rows_kernel<T, 2, 2, FORM, false>, dim3((unsigned)p.tokens), dim3(64), (size_t)0, st, pdl, p, log2));
+  } else {
+    // few: a step per warp, queries, keys and values apart, spread over the multiprocessors
+    const int steps = ((p.heads > p.kv_heads ? p.heads : p.kv_heads) + (32 >> log2) - 1) >> (5 - log2);
+    const dim3 grid((unsigned)p.tokens, (unsigned)((steps + 3) / 4), p.store ? 3 : 2);
+    KQ_CUDA_TRY(launch_pdl(rope_rows_kernel<T, 4, 1, FORM, true>, grid, dim3(128), (size_t)0, st, pdl, p, log2));
+  }
+  options().launches += 1;
+  return KQ_OK;
+}
+
 template <typename T>
 int run_rope(const RopeParams& p, cudaStream_t st) {
+  if (in_pieces<T>(p)) return 2 * p.half < p.dim ? run_rows<T, MIXED>(p, st) : p.interleaved ? run_rows<T, NEIGHBOURS>(p, st) : run_rows<T, HALVES>(p, st);
   const int all = p.heads + (p.store ? 2 : 1) * p.kv_heads;
   const bool pdl = options().pdl != 0;
-  if (in_pieces<T>(p)) {
-    int log2 = 0;
-    while ((1 << log2) * (32 / (int)sizeof(T)) < p.dim) ++log2;
-    const bool halves = !p.interleaved && 2 * p.half == p.dim;
-    if (p.tokens >= 4 * sm_count()) {
-      // many tokens: two warps walk a token's heads
-      KQ_CUDA_TRY(launch_pdl(halves ? rope_rows_kernel<T, 2, 2, true, false> : rope_rows_kernel<T, 2, 2, false, false>, dim3((unsigned)p.tokens), dim3(64), (size_t)0, st, pdl, p, log2));
-    } else {
-      // few: a step per warp, queries, keys and values apart, spread over the multiprocessors
-      const int steps = ((p.heads > p.kv_heads ? p.heads : p.kv_heads) + (32 >> log2) - 1) >> (5 - log2);
-      const dim3 grid((unsigned)p.tokens, (unsigned)((steps + 3) / 4), p.store ? 3 : 2);
-      KQ_CUDA_TRY(launch_pdl(halves ? rope_rows_kernel<T, 4, 1, true, true> : rope_rows_kernel<T, 4, 1, false, true>, grid, dim3(128), (size_t)0, st, pdl, p, log2));
-    }
-    options().launches += 1;
-    return KQ_OK;
-  }
   // few tokens: the heads of one token over several CTAs
   int64_t split = 1;
   while (p.tokens * split < 2 * sm_count() && split * (RP_THREADS / 32) < all) split *= 2;

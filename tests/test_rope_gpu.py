@@ -105,6 +105,41 @@ def test_store(dtype, t, page, d, slot64, heads_first):
     assert torch.equal(kc.reshape(-1, kv, d), want_k) and torch.equal(vc.reshape(-1, kv, d), want_v)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("h,kv,d,rotated,interleaved", [(40, 8, 128, 128, False), (9, 3, 64, 64, True), (5, 2, 256, 64, False), (5, 3, 80, 48, True), (2, 1, 128, 0, False),
+                                                        (7, 7, 16, 16, False), (3, 1, 256, 256, True), (6, 2, 96, 96, False), (5, 5, 80, 48, False)])
+def test_many_tokens(dtype, h, kv, d, rotated, interleaved):
+    """So many that a warp takes a token."""
+    t, page = 20 * 160 + 1, 16
+    qkv, pos, w = inputs(t, h, kv, d, dtype, True, seed=d)
+    qkv[5, d - 1] = float("nan")                   # of the first head of one token
+    freq = inv_freq(rotated)
+    x = qkv.cpu().reshape(t, h + 2 * kv, d)
+    kc, vc = (torch.full((t // page + 3, page, kv, d), 9.0, dtype=DT[dtype], device=dev()) for _ in range(2))
+    slots = torch.randperm(kc.shape[0] * page, generator=torch.Generator().manual_seed(1))[:t]
+    slots[3], slots[7], slots[9] = -1, kc.shape[0] * page, -2 ** 31
+    free = torch.ones(kc.shape[0] * page, dtype=torch.bool)
+    rest = torch.ones(t, dtype=torch.bool)
+    rest[[3, 7, 9]] = False
+    free[slots[rest]] = False
+    for weights in (w, [None, w[1]]):
+        q = attention.qk_norm_rope_store(qkv, pos, freq, h, kc, vc, slots.to(dev()), q_weight=weights[0], k_weight=weights[1], interleaved=interleaved)
+        bad = torch.isnan(q.cpu())
+        bad_at = bad.nonzero()[:, :2].unique(dim=0).tolist()
+        assert bad_at == [[5, 0]] and (weights[0] is None or bool(bad[5, 0].all()))
+        q[5, 0], qkv0 = 0, x[5, 0].clone()
+        x[5, 0] = 0
+        close(q, *rotate(x[:, :h], pos, freq, weights[0], 1e-6, interleaved, 1.0), dtype)
+        x[5, 0] = qkv0
+        kept = kc.reshape(-1, kv, d)[slots[rest].to(dev())]
+        want, bound = rotate(x[:, h:h + kv], pos, freq, weights[1], 1e-6, interleaved, 1.0)
+        close(kept, want[rest], bound[rest] if torch.is_tensor(bound) else bound, dtype)
+        assert torch.equal(vc.reshape(-1, kv, d)[slots[rest].to(dev())].cpu(), x[rest, h + kv:])
+        assert bool((kc.reshape(-1, kv, d).cpu()[free] == 9.0).all()) and bool((vc.reshape(-1, kv, d).cpu()[free] == 9.0).all())
+    dense = attention.qk_norm_rope(qkv, pos, freq, h, kv, q_weight=None, k_weight=w[1], interleaved=interleaved)
+    assert torch.equal(dense[1][rest.to(dev())], kept)
+
+
 def test_nothing_to_do_and_capture():
     qkv, pos, w = inputs(4, 4, 2, 128, "bf16", True)
     freq = inv_freq(128)
