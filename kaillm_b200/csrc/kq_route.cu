@@ -6,11 +6,13 @@
 //
 // A warp per token, NV experts next to each other per lane.  Without a bias the choice compares the logits themselves.  With one, two of
 // a few hundred scores lie closer than fp32 tells apart once in some hundred tokens, and a router's choice should not depend on the
-// last bit of an exponential: candidates of a sigmoid whose scores come within RT_CLOSE of one another are ranked again in fp64; where
-// it is the groups' scores, or a softmax, the whole token is routed again in fp64 (route_wide).
+// last bit of an exponential: candidates whose scores come within RT_CLOSE of one another are ranked again in fp64, and so are the groups
+// of a sigmoid that whole lanes make up; what else is open sends the whole token through fp64 (route_wide), which takes a warp 5 us: left to
+// that, one such token among the last ones was felt in the time of the call (16384 x 256 in 8 groups 21.3 us, with groups_wide 17.4).
 //
-// Bound by instructions, about 500 per token (17 MB and 2.7 us of memory for 16384 x 256 fp32 logits): the best of 32 lanes is one
-// redux.sync on order-preserving integers, and where whole lanes make up a group all groups are scored at once.
+// Bound by instructions, several hundred per token (17 MB and 2.7 us of memory for 16384 x 256 fp32 logits; 16.9 us): the best of 32 lanes
+// is one redux.sync on order-preserving integers, and where whole lanes make up a group all groups are scored at once.  With up to 102, 64 and
+// 51 registers for 16, 8 and fewer experts per lane, as below; left to the compiler 16384 x 256 takes 17.4 us, x 128 11.8 instead of 11.4.
 #include "kq_common.cuh"
 
 namespace kq {
@@ -140,6 +142,33 @@ __device__ __noinline__ void route_wide(const RouteParams& p, int64_t t) {
   }
 }
 
+// Which groups stay, in fp64, where `lanes` whole lanes (a power of two) make up a group: sigmoid with a bias.
+template <typename T, int NV>
+__device__ __forceinline__ uint32_t groups_wide(const RouteParams& p, int64_t t, int lanes) {
+  const int lane = threadIdx.x & 31, e0 = lane * NV;
+  const T* row = static_cast<const T*>(p.logits) + t * p.stride_t;
+  unsigned long long a = RT_TAKEN, b = RT_TAKEN;                  // the two best of the lane, then of its group
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if (e0 + i >= p.experts) break;
+    const unsigned long long k = ordered64(1. / (1. + exp(-(double)sane(to_f32<T>(row[e0 + i])))) + (double)sane(p.bias[e0 + i]));
+    if (k > a) { b = a; a = k; } else if (k > b) b = k;
+  }
+  for (int d = 1; d < lanes; d <<= 1) {
+    const unsigned long long oa = __shfl_xor_sync(0xffffffffu, a, d), ob = __shfl_xor_sync(0xffffffffu, b, d);
+    b = max(min(a, oa), max(b, ob));
+    a = max(a, oa);
+  }
+  unsigned long long mine = p.group_size > 1 ? ordered64(unordered64(a) + unordered64(b)) : a;
+  mine = __shfl_sync(0xffffffffu, mine, min(lane * lanes, 31));   // lane g takes group g's score
+  int better = 0;
+  for (int g = 0; g < p.groups; ++g) {
+    const unsigned long long other = __shfl_sync(0xffffffffu, mine, g);
+    better += other > mine || (other == mine && g < lane);
+  }
+  return __ballot_sync(0xffffffffu, lane < p.groups && better < p.top_groups);
+}
+
 __device__ __forceinline__ uint32_t ordered(float v) {      // compares as v does (both zeros alike)
   const uint32_t u = __float_as_uint(v + 0.f);
   return u ^ (u >> 31 ? 0xffffffffu : 0x80000000u);
@@ -167,15 +196,21 @@ __device__ __forceinline__ uint32_t below_cut(const RouteParams& p, uint32_t cut
   const float c = unordered(cut);
   return p.bias ? max(1u, ordered(c - RT_CLOSE * fmaxf(1.f, fabsf(c)))) : cut;
 }
-// a candidate's score in fp64 (sigmoid)
+// this lane's candidate's score in fp64
 template <typename T>
-__device__ __forceinline__ double score64(const RouteParams& p, const T* row, int e) {
-  return 1. / (1. + exp(-(double)sane(to_f32<T>(row[e])))) + (double)sane(p.bias[e]);
+__device__ __forceinline__ unsigned long long score64(const RouteParams& p, const T* row, int e, bool live, float top) {
+  const double x = live ? (double)sane(to_f32<T>(row[e])) : 0., c = live ? (double)sane(p.bias[e]) : 0.;
+  if (p.sigmoid) return live ? ordered64(1. / (1. + exp(-x)) + c) : RT_TAKEN;
+  double sum = 0.;
+  for (int i = threadIdx.x & 31; i < p.experts; i += 32) sum += exp((double)sane(to_f32<T>(row[i])) - (double)top);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  return live ? ordered64(exp(x - (double)top) / fmax(sum, 1.1754943508222875e-38) + c) : RT_TAKEN;
 }
 
 // FULL: 32 x NV experts, in rows (and with a bias) that take vector loads
 template <typename T, int NV, bool FULL>
-__global__ void __launch_bounds__(RT_WARPS * 32) route_kernel(const RouteParams p) {
+__global__ void __launch_bounds__(RT_WARPS * 32, NV >= 32 ? 2 : NV == 16 ? 5 : NV == 8 ? 8 : 10) route_kernel(const RouteParams p) {
   const int lane = threadIdx.x & 31;
   const int64_t t = (int64_t)blockIdx.x * RT_WARPS + (threadIdx.x >> 5);
   pdl_trigger();
@@ -183,7 +218,8 @@ __global__ void __launch_bounds__(RT_WARPS * 32) route_kernel(const RouteParams 
   if (t >= p.tokens) return;
   const T* row = static_cast<const T*>(p.logits) + t * p.stride_t;
   const int e0 = lane * NV;
-  __shared__ uint2 s_list[RT_WARPS][32];
+  __shared__ __align__(16) uint32_t s_key[RT_WARPS][36];
+  __shared__ int s_id[RT_WARPS][32];
   float x[NV];
   constexpr int VEC = NV * (int)sizeof(T) >= 16 ? 16 / (int)sizeof(T) : NV;      // values of one load
   if (FULL || (p.aligned && (p.experts % NV == 0))) {
@@ -274,19 +310,22 @@ __global__ void __launch_bounds__(RT_WARPS * 32) route_kernel(const RouteParams 
       }
     }
     // lane g takes group g's score and counts the better ones
-    const int group_of_lane = whole ? e0 / p.group_size : lane;
+    const int group_of_lane = whole ? lane >> (__ffs(lanes) - 1) : lane;
     if (whole) mine = __shfl_sync(0xffffffffu, mine, min(lane * lanes, 31));
     if (lane >= p.groups) mine = 0;
     int better = 0;
-    for (int g = 0; g < p.groups; ++g) {
-      const uint32_t other = __shfl_sync(0xffffffffu, mine, g);
-      better += other > mine || (other == mine && g < lane);
-    }
+    for (int g0 = 0; g0 < p.groups; g0 += 4)     // lanes behind the groups count as 0
+#pragma unroll
+      for (int g = g0; g < g0 + 4; ++g) better += __shfl_sync(0xffffffffu, mine, g) >= mine + (g >= lane);
     const bool keep = lane < p.groups && better < p.top_groups;
-    const uint32_t kept = __ballot_sync(0xffffffffu, keep);
+    uint32_t kept = __ballot_sync(0xffffffffu, keep);
     if (p.bias && p.top_groups < p.groups) {     // the order of the kept ones does not matter
       const uint32_t last = __reduce_min_sync(0xffffffffu, keep ? mine : 0xffffffffu), next = __reduce_max_sync(0xffffffffu, keep ? 0u : mine);
       wide = close(unordered(last), unordered(next));
+      if (wide && whole && p.sigmoid) {          // the same for all lanes
+        kept = groups_wide<T, NV>(p, t, lanes);
+        wide = false;
+      }
     }
     if (whole) {
       if (!(kept >> group_of_lane & 1)) {
@@ -299,17 +338,34 @@ __global__ void __launch_bounds__(RT_WARPS * 32) route_kernel(const RouteParams 
         if (e0 + i < p.experts && !(kept >> ((e0 + i) / p.group_size) & 1)) key[i] = 0;
     }
   }
-  // The (top_k + 1)-th of the lanes' best scores bounds what can be chosen, or come next: usually a dozen experts, which go to one lane
-  // each and are ranked by counting the better ones.  More than 32 of them (many ties, top_k near 32): one by one.
+  // The (top_k + 1)-th of the lanes' best scores, or one shortly below it, bounds what can be chosen, or come next: usually a dozen experts,
+  // which go to one lane each and are ranked by counting the better ones.  From 8 experts per lane on the bound is found by halving an
+  // interval until top_k + 1 to + 3 lanes reach it (16384 x 256 22.7 -> 21.3 us); below, by taking the best lane top_k + 1 times (x 128 in
+  // 11.8, by halving 13.3: all lanes take part, and the list grows).  More than 32 of them (many ties, top_k near 32): one by one.
   int id = 0, rank = 0x7fffffff;
   bool listed = false;
   if (p.top_k < 16) {
-    uint32_t rest = key[0], cut = 0;
+    uint32_t best = key[0], cut = 0;
 #pragma unroll
-    for (int i = 1; i < NV; ++i) rest = max(rest, key[i]);
-    for (int n = 0; n <= p.top_k; ++n) {
-      cut = __reduce_max_sync(0xffffffffu, rest);
-      if (lane == __ffs(__ballot_sync(0xffffffffu, rest == cut)) - 1) rest = 0;
+    for (int i = 1; i < NV; ++i) best = max(best, key[i]);
+    if (NV < 8) {
+      for (int n = 0; n <= p.top_k; ++n) {
+        cut = __reduce_max_sync(0xffffffffu, best);
+        if (lane == __ffs(__ballot_sync(0xffffffffu, best == cut)) - 1) best = 0;
+      }
+    } else if (__popc(__ballot_sync(0xffffffffu, best != 0)) > p.top_k) {
+      uint32_t hi = __reduce_max_sync(0xffffffffu, best);
+      cut = __reduce_min_sync(0xffffffffu, best ? best : 0xffffffffu);     // more than top_k lanes reach it
+      for (int n = 0; n < 8 && cut < hi; ++n) {
+        const uint32_t mid = cut + ((hi - cut + 1) >> 1);
+        const int reach = __popc(__ballot_sync(0xffffffffu, best >= mid));
+        if (reach > p.top_k) {
+          cut = mid;
+          if (reach <= p.top_k + 2) break;
+        } else {
+          hi = mid - 1;
+        }
+      }
     }
     cut = below_cut(p, cut);
     int at = 0, total = 0;
@@ -320,35 +376,42 @@ __global__ void __launch_bounds__(RT_WARPS * 32) route_kernel(const RouteParams 
       total += __popc(in);
     }
     if (total <= 32) {
-      uint2* list = s_list[threadIdx.x >> 5];
+      uint32_t* keys = s_key[threadIdx.x >> 5];
+      int* ids = s_id[threadIdx.x >> 5];
+      keys[lane] = 0;
+      __syncwarp();
 #pragma unroll
       for (int i = 0; i < NV; ++i)
-        if (key[i] >= cut) list[at++] = make_uint2(key[i], e0 + i);      // in the order of the experts
+        if (key[i] >= cut) { keys[at] = key[i]; ids[at++] = e0 + i; }     // in the order of the experts
       __syncwarp();
-      const uint2 own = lane < total ? list[lane] : make_uint2(0, 0);
+      const uint32_t own = keys[lane];
+      const int own_id = ids[lane];
       int better = 0;
-      uint32_t below = 0;                                                 // the best of those behind this one
-      for (int j = 0; j < total; ++j) {
-        const uint32_t other = __shfl_sync(0xffffffffu, own.x, j);
-        const bool ahead = other > own.x || (other == own.x && j < lane);
-        better += ahead;
-        below = max(below, ahead || j == lane ? 0u : other);
+      for (int j0 = 0; j0 < total; j0 += 4) {                             // keys behind the last one are 0
+        const uint4 other = *reinterpret_cast<const uint4*>(keys + j0);
+        better += other.x >= own + (j0 >= lane);
+        better += other.y >= own + (j0 + 1 >= lane);
+        better += other.z >= own + (j0 + 2 >= lane);
+        better += other.w >= own + (j0 + 3 >= lane);
       }
-      const bool open = p.bias && lane < total && better < p.top_k && below && close(unordered(own.x), unordered(below));
+      bool open = false;
+      if (p.bias) {                                                       // is the next one too close?
+        __syncwarp();
+        if (lane < total) keys[better] = own;
+        __syncwarp();
+        open = better + 1 < total && better < p.top_k && close(unordered(own), unordered(keys[better + 1]));
+        open = open && lane < total;
+      }
       if (__any_sync(0xffffffffu, open)) {
-        if (p.sigmoid) {
-          const unsigned long long mine = lane < total ? ordered64(score64<T>(p, row, own.y)) : 0;
-          better = 0;
+        const unsigned long long mine = score64<T>(p, row, own_id, lane < total, top);
+        better = 0;
 #pragma unroll 4
-          for (int j = 0; j < total; ++j) {
-            const unsigned long long other = __shfl_sync(0xffffffffu, mine, j);
-            better += other > mine || (other == mine && j < lane);
-          }
-        } else {
-          wide = true;
+        for (int j = 0; j < total; ++j) {
+          const unsigned long long other = __shfl_sync(0xffffffffu, mine, j);
+          better += other > mine || (other == mine && j < lane);
         }
       }
-      if (lane < total && better < p.top_k) { id = own.y; rank = better; }
+      if (lane < total && better < p.top_k) { id = own_id; rank = better; }
     }
     listed = total <= 32;
   }

@@ -86,6 +86,23 @@ def test_scores_closer_than_fp32_tells_apart():
     check(y, 4, "sigmoid", torch.zeros(64, device=dev()), groups=8, top_groups=3)
 
 
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("e,groups", [(256, 8), (128, 4), (512, 32), (96, 3), (64, 8), (1024, 16)])
+def test_groups_closer_than_fp32_tells_apart(scoring, e, groups):
+    """The best two of all groups the same but for single bits of one logit, in every order; then the same among the experts of one group."""
+    size, g = e // groups, torch.Generator().manual_seed(e)
+    x = torch.randn((64, e), generator=g) - 4
+    for r in range(64):
+        best = (torch.arange(groups) * size)[:, None] + torch.randint(0, size - 1, (groups, 1), generator=g) + torch.tensor([0, 1])
+        x[r, best] = torch.tensor([1.0, 0.5])
+        x[r, best[:, 0]] += torch.randint(-2, 3, (groups,), generator=g) * 2.0 ** -23
+        x[r, :size] = 0.25 + torch.randint(-2, 3, (size,), generator=g) * 2.0 ** -24
+    bias = torch.full((e,), 0.125, device=dev())
+    check(x.to(dev()), 5, scoring, bias, groups, (groups + 1) // 2)
+    check(x.to(dev()), 5, scoring, bias)
+    check(x[:, :size].contiguous().to(dev()), 3, scoring, bias[:size])
+
+
 def test_many_tokens_strides_and_capture():
     x = logits(3001, 256, "f32", seed=9)
     bias = torch.randn(256, device=dev()) * 0.05
