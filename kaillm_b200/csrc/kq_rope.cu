@@ -65,7 +65,7 @@ __device__ __forceinline__ T* target_of(const RopeParams& p, int64_t t, int head
              : static_cast<T*>(p.v) + page * p.v_page + place * p.v_slot + h * p.v_head;
 }
 
-// Rows of 16-byte pieces.  A lane owns two pieces A and B of a head, half the rotated width apart (behind the rotated part, half of what is
+// Rows of pieces of 16 bytes, or 8 where the rotated width or an address asks for it.  A lane owns two pieces A and B of a head, half the rotated width apart (behind the rotated part, half of what is
 // left), so that the values of a pair stand at the same place of A and B, or interleaved next to each other in one of them; D / 2V lanes
 // share a head (V values per piece), rounded up to a power of two for the sum of squares, and the other lanes take further heads.  So nothing
 // but that sum crosses lanes, and out_A = A * c0 + A' * c1, out_B = B * c2 + B' * c3 (A', B': the partners) with factors made of the
@@ -77,11 +77,11 @@ __device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) { f32x2 r; asm(
 __device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) { f32x2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
 __device__ __forceinline__ f32x2 swap2(f32x2 v) { const float2 u = unpack2(v); return pack2(u.y, u.x); }
 
-template <typename T> __device__ __forceinline__ f32x2 widen(const uint4& v, int i) {   // values 2i, 2i + 1 of a piece
+template <typename T, typename Piece> __device__ __forceinline__ f32x2 widen(const Piece& v, int i) {   // values 2i, 2i + 1 of a piece
   const T* e = reinterpret_cast<const T*>(&v);
   return pack2(to_f32<T>(e[2 * i]), to_f32<T>(e[2 * i + 1]));
 }
-template <typename T> __device__ __forceinline__ void narrow(uint4& v, int i, f32x2 x) {
+template <typename T, typename Piece> __device__ __forceinline__ void narrow(Piece& v, int i, f32x2 x) {
   const float2 u = unpack2(x);
   if constexpr (sizeof(T) == 4) {
     reinterpret_cast<float2*>(&v)[i] = u;
@@ -92,20 +92,22 @@ template <typename T> __device__ __forceinline__ void narrow(uint4& v, int i, f3
   }
 }
 
-// V values of a norm weight from d on (without a weight: ones)
-template <typename T, int V>
+// The values of a norm weight for a piece from d on (without a weight: ones)
+template <typename T, typename Piece, int V>
 __device__ __forceinline__ void weights_of(const RopeParams& p, const void* w, int d, float (&out)[V]) {
   if (!w) {
 #pragma unroll
     for (int e = 0; e < V; ++e) out[e] = 1.f;
   } else if (p.w_f32) {
+    constexpr int N = sizeof(Piece) / 4;
 #pragma unroll
-    for (int e = 0; e < V; e += 4) {
-      const float4 f = *reinterpret_cast<const float4*>(static_cast<const float*>(w) + d + e);
-      out[e] = f.x; out[e + 1] = f.y; out[e + 2] = f.z; out[e + 3] = f.w;
+    for (int e = 0; e < V; e += N) {
+      const Piece f = *reinterpret_cast<const Piece*>(static_cast<const float*>(w) + d + e);
+#pragma unroll
+      for (int i = 0; i < N; ++i) out[e + i] = reinterpret_cast<const float*>(&f)[i];
     }
   } else {
-    const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const T*>(w) + d);
+    const Piece u = *reinterpret_cast<const Piece*>(static_cast<const T*>(w) + d);
 #pragma unroll
     for (int e = 0; e < V; ++e) out[e] = to_f32<T>(reinterpret_cast<const T*>(&u)[e]);
   }
@@ -113,9 +115,9 @@ __device__ __forceinline__ void weights_of(const RopeParams& p, const void* w, i
 
 enum RopeForm { HALVES, NEIGHBOURS, MIXED };   // all values turn, in pairs half a head apart; all, interleaved; some do not
 
-// A lane's pieces of a head and what they are multiplied by.  Only MIXED has lanes that differ, and choose their partners.
-template <typename T, RopeForm FORM> struct RopeLane {
-  static constexpr int V = 16 / (int)sizeof(T), P = V / 2;                        // values, pairs of them in a piece
+// A lane's pieces of a head and what they are multiplied by.  Only MIXED has lanes that differ, and choose their partners; it covers the others.
+template <typename T, RopeForm FORM, typename Piece> struct RopeLane {
+  static constexpr int V = (int)(sizeof(Piece) / sizeof(T)), P = V / 2;                        // values, pairs of them in a piece
   int log2;                                                                       // of the lanes of a head
   bool active, turned, apart;
   int da, db;                                                                     // first values of the pieces
@@ -133,8 +135,8 @@ template <typename T, RopeForm FORM> struct RopeLane {
 
   __device__ __forceinline__ void factors(const RopeParams& p, const void* w, const float2* s_turn) {
     float wa[V], wb[V];
-    weights_of<T, V>(p, active ? w : nullptr, da, wa);
-    weights_of<T, V>(p, active ? w : nullptr, db, wb);
+    weights_of<T, Piece>(p, active ? w : nullptr, da, wa);
+    weights_of<T, Piece>(p, active ? w : nullptr, db, wb);
     const bool on = turned && active;
 #pragma unroll
     for (int e = 0; e < V; e += 2) {
@@ -150,10 +152,10 @@ template <typename T, RopeForm FORM> struct RopeLane {
     }
   }
   // all lanes of the warp together; a lane without a head has zeros
-  __device__ __forceinline__ void turn(const RopeParams& p, uint4& ra, uint4& rb, bool normed) const {
+  __device__ __forceinline__ void turn(const RopeParams& p, Piece& ra, Piece& rb, bool normed) const {
     f32x2 x[P], y[P];
 #pragma unroll
-    for (int e = 0; e < P; ++e) { x[e] = widen<T>(ra, e); y[e] = widen<T>(rb, e); }
+    for (int e = 0; e < P; ++e) { x[e] = widen<T, Piece>(ra, e); y[e] = widen<T, Piece>(rb, e); }
     f32x2 inv = 0;
     if (normed) {
       f32x2 sq = mul2(x[0], x[0]);
@@ -170,13 +172,13 @@ template <typename T, RopeForm FORM> struct RopeLane {
       const f32x2 px = apart ? y[e] : turned ? swap2(x[e]) : 0, py = apart ? x[e] : turned ? swap2(y[e]) : 0;
       f32x2 u = fma2(px, c1[e], mul2(x[e], c0[e])), v = fma2(py, c3[e], mul2(y[e], c2[e]));
       if (normed) { u = mul2(u, inv); v = mul2(v, inv); }
-      narrow<T>(ra, e, u);
-      narrow<T>(rb, e, v);
+      narrow<T, Piece>(ra, e, u);
+      narrow<T, Piece>(rb, e, v);
     }
   }
-  __device__ __forceinline__ void put(T* dst, const uint4& ra, const uint4& rb) const {
-    *reinterpret_cast<uint4*>(dst + da) = ra;
-    *reinterpret_cast<uint4*>(dst + db) = rb;
+  __device__ __forceinline__ void put(T* dst, const Piece& ra, const Piece& rb) const {
+    *reinterpret_cast<Piece*>(dst + da) = ra;
+    *reinterpret_cast<Piece*>(dst + db) = rb;
   }
 };
 
@@ -198,10 +200,10 @@ __device__ __forceinline__ bool rows_of(const RopeParams& p, int64_t t, T** k, T
 
 // A CTA per token, or with SPREAD three (queries, keys and values: blockIdx.z); its warps share the token's steps (a step: as many heads as a
 // warp holds).  The first rows of all kinds are on their way while the angles are formed.
-template <typename T, int WARPS, int AHEAD, RopeForm FORM, bool SPREAD>
+template <typename T, int WARPS, int AHEAD, RopeForm FORM, bool SPREAD, typename Piece>
 __global__ void __launch_bounds__(WARPS * 32, SPREAD ? 4 : 16 / WARPS) rope_rows_kernel(const RopeParams p, int lanes_log2) {
   __shared__ float2 s_turn[RP_MAX_DIM / 2];
-  RopeLane<T, FORM> L(p, lanes_log2);
+  RopeLane<T, FORM, Piece> L(p, lanes_log2);
   const int warp = threadIdx.x >> 5, sub = L.head_of_step();
   const int64_t t = blockIdx.x;
   const bool q_here = !SPREAD || blockIdx.z == 0, k_here = !SPREAD || blockIdx.z == 1, v_here = p.store && (!SPREAD || blockIdx.z == 2);
@@ -210,11 +212,11 @@ __global__ void __launch_bounds__(WARPS * 32, SPREAD ? 4 : 16 / WARPS) rope_rows
   pdl_trigger();
   pdl_wait();
   const T* src = static_cast<const T*>(p.qkv) + t * p.qkv_t + h0 * p.dim;
-  auto load = [&](const T* from, bool on, uint4& va, uint4& vb) {
-    va = vb = make_uint4(0, 0, 0, 0);
-    if (on) { va = *reinterpret_cast<const uint4*>(from + L.da); vb = *reinterpret_cast<const uint4*>(from + L.db); }
+  auto load = [&](const T* from, bool on, Piece& va, Piece& vb) {
+    va = vb = Piece{};
+    if (on) { va = *reinterpret_cast<const Piece*>(from + L.da); vb = *reinterpret_cast<const Piece*>(from + L.db); }
   };
-  uint4 a[AHEAD], b[AHEAD], ka, kb, va, vb;
+  Piece a[AHEAD], b[AHEAD], ka, kb, va, vb;
 #pragma unroll
   for (int i = 0; i < AHEAD; ++i) load(src + i * step * p.dim, q_here && L.active && h0 + i * step < p.heads, a[i], b[i]);
   const T* k_src = src + p.heads * p.dim;
@@ -244,7 +246,7 @@ __global__ void __launch_bounds__(WARPS * 32, SPREAD ? 4 : 16 / WARPS) rope_rows
     for (int i = 0; i < AHEAD; ++i) {
       const int hi = h + i * step;
       if (hi - sub >= p.heads) break;
-      uint4 ra = a[i], rb = b[i];
+      Piece ra = a[i], rb = b[i];
       load(src, L.active && hi + AHEAD * step < p.heads, a[i], b[i]);
       src += step * p.dim;
       L.turn(p, ra, rb, p.qw != nullptr);
@@ -255,7 +257,7 @@ __global__ void __launch_bounds__(WARPS * 32, SPREAD ? 4 : 16 / WARPS) rope_rows
   if (!k_here || h0 - sub >= p.kv_heads) return;
   if (!SPREAD && p.kw != p.qw) L.factors(p, p.kw, s_turn);
   for (int h = h0; h - sub < p.kv_heads; h += step) {
-    uint4 ra = ka, rb = kb;
+    Piece ra = ka, rb = kb;
     k_src += step * p.dim;
     load(k_src, L.active && h + step < p.kv_heads, ka, kb);
     L.turn(p, ra, rb, p.kw != nullptr);
@@ -263,9 +265,12 @@ __global__ void __launch_bounds__(WARPS * 32, SPREAD ? 4 : 16 / WARPS) rope_rows
   }
 }
 
-// 16 bytes, or with live = false 16 bytes of zeros and no read
+// a piece, or with live = false a piece of zeros and no read
 __device__ __forceinline__ void copy_piece(uint4* dst, const void* src, bool live) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_piece(uint2* dst, const void* src, bool live) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "r"(live ? 8 : 0) : "memory");
 }
 
 // Many tokens: a warp per token walks its values, queries and keys through a ring in shared memory, two steps in use and the others under
@@ -275,12 +280,12 @@ __device__ __forceinline__ void copy_piece(uint4* dst, const void* src, bool liv
 // multiprocessor.  Steps of the ring and least warps of a multiprocessor: 16-bit 6 and 18 (41.5; 8 and 18 43.2, 5 and 20 41.8, 6 and 16
 // 44.9), fp32 10 and 16 (4096 tokens 42.4; 6 and 18 46.9), whose heads take twice the steps.
 template <typename T> constexpr int RING_WARPS = sizeof(T) == 4 ? 16 : 18;
-template <typename T, RopeForm FORM>
+template <typename T, RopeForm FORM, typename Piece>
 __global__ void __launch_bounds__(32, RING_WARPS<T>) rope_ring_kernel(const RopeParams p, int lanes_log2) {
   constexpr int RING_STEPS = sizeof(T) == 4 ? 10 : 6;
   __shared__ float2 s_turn[RP_MAX_DIM / 2];
-  __shared__ uint4 s_ring[RING_STEPS][2][32];
-  RopeLane<T, FORM> L(p, lanes_log2);
+  __shared__ Piece s_ring[RING_STEPS][2][32];
+  RopeLane<T, FORM, Piece> L(p, lanes_log2);
   const int lane = threadIdx.x, h0 = L.head_of_step();
   const int64_t t = blockIdx.x;
   const int per = 32 >> lanes_log2, nq = (p.heads + per - 1) >> (5 - lanes_log2), nk = (p.kv_heads + per - 1) >> (5 - lanes_log2), nv = p.store ? nk : 0;
@@ -302,7 +307,7 @@ __global__ void __launch_bounds__(32, RING_WARPS<T>) rope_ring_kernel(const Rope
   };
 #pragma unroll
   for (int s = 0; s < RING_STEPS - 2; ++s) fetch(s);
-  auto take = [&](uint4& ra, uint4& rb) {
+  auto take = [&](Piece& ra, Piece& rb) {
     asm volatile("cp.async.wait_group %0;" ::"n"(RING_STEPS - 3) : "memory");
     ra = s_ring[from][0][lane];
     rb = s_ring[from][1][lane];
@@ -315,7 +320,7 @@ __global__ void __launch_bounds__(32, RING_WARPS<T>) rope_ring_kernel(const Rope
   T *k_dst, *v_dst;
   int64_t k_head;
   const bool kept = L.active && rows_of<T>(p, t, &k_dst, &v_dst, &k_head);
-  uint4 ra, rb, sa, sb;
+  Piece ra, rb, sa, sb;
   for (int i = 0, h = h0; i < nv; ++i, h += per) {
     take(ra, rb);
     if (kept && h < p.kv_heads) L.put(v_dst + h * p.v_head, ra, rb);
@@ -389,32 +394,33 @@ __global__ void __launch_bounds__(RP_THREADS) rope_any_kernel(const RopeParams p
   }
 }
 
-// rope_rows_kernel's case: every row, piece pair and target made of 16-byte pieces at 16-byte addresses
-template <typename T>
+// every row, piece pair and target made of pieces at their own alignment
+template <typename T, typename Piece>
 bool in_pieces(const RopeParams& p) {
-  constexpr int V = 16 / (int)sizeof(T);
+  constexpr int V = (int)(sizeof(Piece) / sizeof(T));
   const int64_t strides = p.qkv_t | p.k_page | p.k_slot | p.k_head | p.v_page | p.v_slot | p.v_head;   // zeros where there is no cache
   const uintptr_t at = (uintptr_t)p.qkv | (uintptr_t)p.q | (uintptr_t)p.k | (uintptr_t)p.v | (uintptr_t)p.qw | (uintptr_t)p.kw;
-  return p.dim % (2 * V) == 0 && p.half % V == 0 && p.dim <= 64 * V && strides % V == 0 && at % 16 == 0;
+  return p.dim % (2 * V) == 0 && p.half % V == 0 && p.dim <= 64 * V && strides % V == 0 && at % sizeof(Piece) == 0;
 }
 
-template <typename T, RopeForm FORM>
+template <typename T, RopeForm FORM, typename Piece>
 int run_rows(const RopeParams& p, cudaStream_t st) {
   int log2 = 0;
-  while ((1 << log2) * (32 / (int)sizeof(T)) < p.dim) ++log2;
+  while ((1 << log2) * 2 * (int)(sizeof(Piece) / sizeof(T)) < p.dim) ++log2;
   const bool pdl = options().pdl != 0;
-  // Few tokens, more than a few, more than a wave of ring_kernel's warps; with 40 + 2 x 8 heads of 128, us: 16 tokens 2.9 spread; 600 7.0 by two warps
+  // (pieces of 8 bytes: few, and the ring.)  Few tokens, more than a few, more than a wave of ring_kernel's warps; with 40 + 2 x 8 heads of 128, us: 16 tokens 2.9 spread; 600 7.0 by two warps
   // each, 16 spread, 9.0 by the ring; 2000 16.6, 54.7, 16.0; 5000 33.5, 132, 28.8
-  if (p.tokens >= 20 * sm_count()) {
-    KQ_CUDA_TRY(launch_pdl(rope_ring_kernel<T, FORM>, dim3((unsigned)p.tokens), dim3(32), (size_t)0, st, pdl, p, log2));
-  } else if (p.tokens >= 4 * sm_count()) {
+  if (p.tokens >= (sizeof(Piece) == 16 ? 20 : 4) * sm_count()) {
+    KQ_CUDA_TRY(launch_pdl(rope_ring_kernel<T, FORM, Piece>, dim3((unsigned)p.tokens), dim3(32), (size_t)0, st, pdl, p, log2));
+  } else if (sizeof(Piece) == 16 && p.tokens >= 4 * sm_count()) {
     // two warps walk a token's heads
-    KQ_CUDA_TRY(launch_pdl(rope_rows_kernel<T, 2, 2, FORM, false>, dim3((unsigned)p.tokens), dim3(64), (size_t)0, st, pdl, p, log2));
+    if constexpr (sizeof(Piece) == 16)
+      KQ_CUDA_TRY(launch_pdl(rope_rows_kernel<T, 2, 2, FORM, false, Piece>, dim3((unsigned)p.tokens), dim3(64), (size_t)0, st, pdl, p, log2));
   } else {
     // few: a step per warp, queries, keys and values apart, spread over the multiprocessors
     const int steps = ((p.heads > p.kv_heads ? p.heads : p.kv_heads) + (32 >> log2) - 1) >> (5 - log2);
     const dim3 grid((unsigned)p.tokens, (unsigned)((steps + 3) / 4), p.store ? 3 : 2);
-    KQ_CUDA_TRY(launch_pdl(rope_rows_kernel<T, 4, 1, FORM, true>, grid, dim3(128), (size_t)0, st, pdl, p, log2));
+    KQ_CUDA_TRY(launch_pdl(rope_rows_kernel<T, 4, 1, FORM, true, Piece>, grid, dim3(128), (size_t)0, st, pdl, p, log2));
   }
   options().launches += 1;
   return KQ_OK;
@@ -422,7 +428,11 @@ int run_rows(const RopeParams& p, cudaStream_t st) {
 
 template <typename T>
 int run_rope(const RopeParams& p, cudaStream_t st) {
-  if (in_pieces<T>(p)) return 2 * p.half < p.dim ? run_rows<T, MIXED>(p, st) : p.interleaved ? run_rows<T, NEIGHBOURS>(p, st) : run_rows<T, HALVES>(p, st);
+  if (in_pieces<T, uint4>(p))
+    return 2 * p.half < p.dim ? run_rows<T, MIXED, uint4>(p, st) : p.interleaved ? run_rows<T, NEIGHBOURS, uint4>(p, st) : run_rows<T, HALVES, uint4>(p, st);
+  // heads of 80 of which 40 turn, 16-bit, us, by rope_any_kernel / in pieces of 8 bytes: one token 3.4 / 2.7, 1500 tokens with 56 heads 31.8 / 21.0,
+  // 3317 with 73 heads 86.6 / 36.9 (issue: 10 of 16 lanes, half the values per instruction)
+  if (in_pieces<T, uint2>(p)) return run_rows<T, MIXED, uint2>(p, st);
   const int all = p.heads + (p.store ? 2 : 1) * p.kv_heads;
   const bool pdl = options().pdl != 0;
   // few tokens: the heads of one token over several CTAs

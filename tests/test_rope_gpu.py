@@ -107,10 +107,23 @@ def test_store(dtype, t, page, d, slot64, heads_first):
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("h,kv,d,rotated,interleaved", [(40, 8, 128, 128, False), (9, 3, 64, 64, True), (5, 2, 256, 64, False), (5, 3, 80, 48, True), (2, 1, 128, 0, False),
-                                                        (7, 7, 16, 16, False), (3, 1, 256, 256, True), (6, 2, 96, 96, False), (5, 5, 80, 48, False)])
+                                                        (7, 7, 16, 16, False), (3, 1, 256, 256, True), (6, 2, 96, 96, False), (5, 5, 80, 48, False),
+                                                        (5, 2, 80, 40, False), (3, 3, 72, 72, True), (4, 1, 40, 8, False), (2, 2, 256, 24, True)])
 def test_many_tokens(dtype, h, kv, d, rotated, interleaved):
     """So many that a warp takes a token."""
-    t, page = 20 * 160 + 1, 16
+    many(dtype, 20 * 160 + 1, h, kv, d, rotated, interleaved)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("t", [12, 700])
+@pytest.mark.parametrize("h,kv,d,rotated,interleaved", [(5, 2, 80, 40, False), (71, 1, 80, 40, True), (3, 3, 72, 72, True), (4, 1, 40, 8, False), (2, 2, 256, 24, True),
+                                                        (9, 2, 20, 20, False), (3, 1, 128, 128, True)])
+def test_small_pieces(dtype, t, h, kv, d, rotated, interleaved):
+    many(dtype, t, h, kv, d, rotated, interleaved)
+
+
+def many(dtype, t, h, kv, d, rotated, interleaved):
+    page = 16
     qkv, pos, w = inputs(t, h, kv, d, dtype, True, seed=d)
     qkv[5, d - 1] = float("nan")                   # of the first head of one token
     freq = inv_freq(rotated)
