@@ -14,7 +14,7 @@
 // keys: no atomics, the same bits every time.
 //
 // A worker is a CTA whose warps take turns at the tiles and join their results at the end of an item, or, where there are items enough
-// for every warp of the wave, a warp on its own, which has nothing to join.
+// for every warp of the wave, a warp on its own, which has nothing to join.  Where no sequence can be long, workers take whole items.
 #include <type_traits>
 
 #include "kq_common.cuh"
@@ -44,7 +44,7 @@ struct AttnParams {
   void* out;                                           // [batch][heads][dim]
   float* lse;                                          // [batch][heads] or null
   float* part_o; float2* part_ml; int2* meta;          // two partial results per worker; which item starts in a worker and ends in which other
-  int split;                                           // 0: one CTA per item
+  int split;                                           // 0: workers take whole items, in turn
   int solo;                                            // a worker is a warp (of the computing ones), not a CTA
 };
 
@@ -76,12 +76,19 @@ struct Walk {
 
   __device__ void load(const AttnParams& p) { tiles2 = b + 1 < p.batch ? tiles_of<TK>(p, b + 1, &first2, &end2) : 0; }
 
-  __device__ void begin_item(const AttnParams& p, int item) {
+  // without division: whole items from `item` on, each `stride`-th; pos: the next one, left: items behind its end
+  __device__ void begin_items(const AttnParams& p, int item) {
     const int per = p.kv_heads * p.row_tiles;
-    b = item / per; sub = item - b * per; at = START;
-    tiles = tiles2 = tiles_of<TK>(p, b, &first, &end);
-    first2 = first; end2 = end;
-    pos = 0; left = tiles;
+    pos = item; left = (int64_t)p.batch * per;
+    if (pos < left) { b = item / per; sub = item - b * per; tiles = tiles_of<TK>(p, b, &first, &end); }
+  }
+  __device__ bool next_item(const AttnParams& p, int stride, Segment* s) {
+    if (pos >= left) return false;
+    s->b = b; s->sub = sub; s->first = first; s->end = end; s->tiles = tiles;
+    s->t0 = 0; s->t1 = tiles; s->last = -1;
+    const int64_t item = pos + stride;
+    begin_items(p, (int)min(item, (int64_t)0x7fffffff));
+    return true;
   }
 
   // the worker whose share holds `unit`; s_div: of the workers the first s_div[1] have s_div[0] + 1 units, the others s_div[0]
@@ -146,7 +153,8 @@ struct Walk {
     }
   }
 
-  __device__ bool next(const AttnParams& p, const int64_t* s_div, Segment* s) {
+  __device__ bool next(const AttnParams& p, const int64_t* s_div, int stride, Segment* s) {
+    if (!p.split) return next_item(p, stride, s);
     while (left > 0) {
       const int cost = START + tiles, take = (int)min((int64_t)(cost - at), left);
       s->b = b; s->sub = sub; s->first = first; s->end = end; s->tiles = tiles;
@@ -308,11 +316,11 @@ __global__ void __launch_bounds__(FM_WARPS * 32, LEAST) attend_fma_kernel(const 
     walk.begin_share(p, s_red, s_div, FM_WARPS * 32, blockIdx.x, gridDim.x);
     if (tid == 0) p.meta[blockIdx.x] = make_int2(-1, 0);
   } else {
-    walk.begin_item(p, blockIdx.x);
+    walk.begin_items(p, blockIdx.x);
   }
   __syncthreads();
   Segment s;
-  while (walk.next(p, s_div, &s)) {
+  while (walk.next(p, s_div, gridDim.x, &s)) {
     const int b = s.b, first = s.first, end = s.end, t0 = s.t0, t1 = s.t1;
     const int h = s.sub / p.row_tiles, x = s.sub - h * p.row_tiles;
     const int head0 = h * p.group + x * p.rows, rows = min(p.rows, p.group - x * p.rows);
@@ -571,8 +579,9 @@ __global__ void __launch_bounds__(MmaShape<DP, TWO>::THREADS, 1) attend_mma_kern
     walk.begin_share(p, s_red, s_div, S::THREADS, worker_of_warp(), SOLO ? gridDim.x * NC : gridDim.x);
     if (warp < NC && lane == 0 && (SOLO || warp == 0)) p.meta[worker_of_warp()] = make_int2(-1, 0);
   } else {
-    walk.begin_item(p, blockIdx.x);
+    walk.begin_items(p, SOLO ? warp % NC * gridDim.x + blockIdx.x : blockIdx.x);      // over the multiprocessors first
   }
+  const int item_step = (SOLO ? NC : 1) * gridDim.x;
   __syncthreads();
   Segment s;
 
@@ -585,7 +594,7 @@ __global__ void __launch_bounds__(MmaShape<DP, TWO>::THREADS, 1) attend_mma_kern
     const bool one_page = p.page_size % 16 == 0;                  // 16 keys from a multiple of 16 on lie in one page
     int n = SOLO ? 0 : warp - NC, n0 = 0;                       // this warp's next tile; tiles before the segment
     int slot = warp - NC, use = 0;                                // every fourth slot, round by round
-    while (walk.next(p, s_div, &s)) {
+    while (walk.next(p, s_div, item_step, &s)) {
       const int h = s.sub / p.row_tiles;
       const T* k_lane = static_cast<const T*>(p.k) + ((int64_t)h * p.k_head + (lane / LPR) * p.k_slot + piece * 8);
       const T* v_lane = static_cast<const T*>(p.v) + ((int64_t)h * p.v_head + (lane / LPR) * p.v_slot + piece * 8);
@@ -652,7 +661,7 @@ __global__ void __launch_bounds__(MmaShape<DP, TWO>::THREADS, 1) attend_mma_kern
   const uint32_t v_at = ring + (KEYS + (lane >> 3 & 1) * 8 + (lane & 7)) * S::ROW + (lane >> 4) * 16;
   uint32_t q[DP / 16][TWO ? 4 : 2];
   int n0 = 0, n = SOLO ? 0 : warp, slot = warp, use = 0;
-  bool more = walk.next(p, s_div, &s);
+  bool more = walk.next(p, s_div, item_step, &s);
   auto load_q = [&]() {
     const int h = s.sub / p.row_tiles, x = s.sub - h * p.row_tiles;
     const int head0 = h * p.group + x * p.rows, rows = min(p.rows, p.group - x * p.rows);
@@ -767,7 +776,7 @@ __global__ void __launch_bounds__(MmaShape<DP, TWO>::THREADS, 1) attend_mma_kern
       if (slot >= NS) { slot -= NS; ++use; }
     }
     n0 += count;
-    more = walk.next(p, s_div, &s);
+    more = walk.next(p, s_div, item_step, &s);
     if (more) load_q();                                           // arrives while the warps join
 
 #pragma unroll
@@ -856,7 +865,8 @@ __global__ void __launch_bounds__(MmaShape<DP, TWO>::THREADS, 1) attend_mma_kern
 template <typename T>
 int launch_both(void (*kern)(const AttnParams), AttnParams& p, int threads, int smem, int ctas_per_sm, cudaStream_t st) {
   const bool pdl = options().pdl != 0;
-  const unsigned grid = p.split ? (unsigned)(sm_count() * ctas_per_sm) : (unsigned)((int64_t)p.batch * p.kv_heads * p.row_tiles);
+  const int64_t items = (int64_t)p.batch * p.kv_heads * p.row_tiles;
+  const unsigned grid = (unsigned)(p.split || p.solo ? sm_count() * ctas_per_sm : items);
   KQ_CUDA_TRY(launch_pdl(kern, dim3(grid), dim3(threads), (size_t)smem, st, pdl, p));
   options().launches += 1;
   if (p.split) {
@@ -914,14 +924,15 @@ int run_f32(AttnParams& p, cudaStream_t st) {
 // From how many items on a worker is a warp.  As warps / as CTAs, us, 148 multiprocessors: 256 sequences of 1..500 tokens with 8 key heads
 // 59.3 / 88.8, 64 of 1..1000 34.4 / 41.8, 64 of 4096 187.9 / 185.7, 16 of 900..3100 (128 items) 31.4 / 32.7, 16 of 4000 with heads of 64 31.8 / 37.9;
 // 66 items of 100..7001 with heads of 256 57.0 / 53.8, 64 items of 8000 59.2 / 54.5, 8 items of 131071 102.7 / 98.7: few items are cut into
-// many more parts.  Where short lengths need no division at all (a CTA per item, no join): 1024 items of 1..200 21.3 / 38.9, within a wave the CTAs.
-bool solo_pays(int64_t items, bool split) { return split ? 4 * items >= 3 * (int64_t)sm_count() : items > 2 * (int64_t)sm_count(); }
+// many more parts.  Short lengths need no division, and no join: each item is a CTA's, or above one per multiprocessor a warp's: 1024 items of
+// 1..200 19.8 / 37.4 (divided all the same: 21.4), 408 of 55 with heads of 256 9.6 / 19.0 (16.9), 160 of 1..60 6.3 / 9.1 (8.9); 96 items
+// of 200 10.6 / 6.8.
+bool solo_pays(int64_t items, bool split) { return split ? 4 * items >= 3 * (int64_t)sm_count() : items > (int64_t)sm_count(); }
 
 template <typename T>
 int run_16bit(AttnParams& p, cudaStream_t st) {
   set_rows(p, 16);
   p.solo = solo_pays((int64_t)p.batch * p.kv_heads * p.row_tiles, p.split);
-  p.split |= p.solo;
   if (p.rows <= 8)
     return p.dim <= 64 ? run_mma<T, 64, false>(p, st) : p.dim <= 96 ? run_mma<T, 96, false>(p, st) : p.dim <= 128 ? run_mma<T, 128, false>(p, st)
          : p.dim <= 192 ? run_mma<T, 192, false>(p, st) : run_mma<T, 256, false>(p, st);
@@ -1022,7 +1033,9 @@ int kq_paged_attention(const void* q, int dtype, int64_t batch, int64_t heads, i
   p.solo = 0;
   int64_t most = table_width * page_size;          // keys that a sequence can show
   if (window > 0 && window < most) most = window;
-  p.split = most > 256;      // short sequences: one launch, one CTA per item
+  // Short sequences: one launch.  Up to 1024 instead of 256 keys, divided / whole, us: 64 sequences of 1..500 with 8 key heads 23.7 / 20.6, 24 of
+  // them 13.7 / 17.7, 128 of 1..1000 58.3 / 66.0
+  p.split = most > 256;
   cudaStream_t st = (cudaStream_t)stream;
   switch (dtype) {
     case KQ_F32: return run_f32(p, st);
