@@ -221,53 +221,47 @@ template <typename T> struct RowOut {
   }
 };
 
-// Adds the partial results of the item that starts in a worker and ends in worker meta.y, for one row, in the order of the keys; 64
-// threads per worker.
+// Adds the partial results of the item that starts in a worker and ends in worker meta.y, for one row, in the order of the keys; a
+// thread has two dimensions, 64 threads (128 above 128 dimensions) a worker.
 template <typename T>
-__global__ void __launch_bounds__(256) attend_join_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(512) attend_join_kernel(const AttnParams p) {
   pdl_trigger();
   pdl_wait();
-  const int c = blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6), r = blockIdx.y, lane = threadIdx.x & 63;
+  const int log2 = p.dim > 128 ? 7 : 6;
+  const int c = blockIdx.x * (blockDim.x >> log2) + (threadIdx.x >> log2), r = blockIdx.y, d = (threadIdx.x & ((1 << log2) - 1)) * 2;
   const int2 it = p.meta[c];
   if (it.x < 0) return;
   const int per = p.kv_heads * p.row_tiles;
   const int b = it.x / per, sub = it.x - b * per, h = sub / p.row_tiles, x = sub - h * p.row_tiles;
   const int head0 = h * p.group + x * p.rows;
-  if (r >= min(p.rows, p.group - x * p.rows)) return;
-  for (int d0 = 0; d0 < p.dim; d0 += 128) {
-    const int d = d0 + lane * 2;
-    const bool in = d < p.dim;
-    const float2* ml0 = p.part_ml + r;
-    const float* o0 = p.part_o + (int64_t)r * p.dim + (in ? d : 0);
-    float m = -INFINITY, l = 0.f;
-    float2 o = make_float2(0.f, 0.f);
-    // maxima, sums and values are loaded together, eight parts at a time: the chain is two loads long
-    for (int i0 = c; i0 <= it.y; i0 += 8) {
-      float2 ml[8], v[8];
+  if (r >= min(p.rows, p.group - x * p.rows) || d >= p.dim) return;
+  const float2* ml0 = p.part_ml + r;
+  const float* o0 = p.part_o + (int64_t)r * p.dim + d;
+  float m = -INFINITY, l = 0.f;
+  float2 o = make_float2(0.f, 0.f);
+  // maxima, sums and values are loaded together, eight parts at a time: the chain is two loads long
+  for (int i0 = c; i0 <= it.y; i0 += 8) {
+    float2 ml[8], v[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int i = min(i0 + k, it.y), at = (2 * i + (i == c)) * p.rows;      // the first part is in slot 2 c + 1, the others in 2 i
-        ml[k] = ml0[at];
-        v[k] = *reinterpret_cast<const float2*>(o0 + (int64_t)at * p.dim);
-      }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        if (i0 + k <= it.y) {
-          const float mn = fmaxf(m, ml[k].x), use = mn == -INFINITY ? 0.f : mn;
-          const float f = ex2(m - use), g = ex2(ml[k].x - use);
-          m = mn;
-          l = l * f + ml[k].y * g;
-          o.x = o.x * f + v[k].x * g;
-          o.y = o.y * f + v[k].y * g;
-        }
-      }
+    for (int k = 0; k < 8; ++k) {
+      const int i = min(i0 + k, it.y), at = (2 * i + (i == c)) * p.rows;      // the first part is in slot 2 c + 1, the others in 2 i
+      ml[k] = ml0[at];
+      v[k] = *reinterpret_cast<const float2*>(o0 + (int64_t)at * p.dim);
     }
-    if (in) {
-      const RowOut<T> out(p, -1, b, head0 + r, r, m, l, d == 0);
-      out.put(d, o.x);
-      out.put(d + 1, o.y);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (i0 + k <= it.y) {
+        const float mn = fmaxf(m, ml[k].x), use = mn == -INFINITY ? 0.f : mn;
+        const float f = ex2(m - use), g = ex2(ml[k].x - use);
+        m = mn;
+        l = l * f + ml[k].y * g;
+        o.x = o.x * f + v[k].x * g;
+        o.y = o.y * f + v[k].y * g;
+      }
     }
   }
+  const RowOut<T> out(p, -1, b, head0 + r, r, m, l, d == 0);
+  out.put2(d, o.x, o.y);
 }
 
 // Where key j of sequence b lies: page name and place inside the page; false where there is no such page.
@@ -870,7 +864,7 @@ int launch_both(void (*kern)(const AttnParams), AttnParams& p, int threads, int 
   KQ_CUDA_TRY(launch_pdl(kern, dim3(grid), dim3(threads), (size_t)smem, st, pdl, p));
   options().launches += 1;
   if (p.split) {
-    KQ_CUDA_TRY(launch_pdl(attend_join_kernel<T>, dim3(grid, (unsigned)p.rows), dim3(p.solo ? 256 : 64), (size_t)0, st, pdl, p));
+    KQ_CUDA_TRY(launch_pdl(attend_join_kernel<T>, dim3(grid, (unsigned)p.rows), dim3((p.solo ? 4 : 1) * (p.dim > 128 ? 128 : 64)), (size_t)0, st, pdl, p));
     options().launches += 1;
   }
   return KQ_OK;
