@@ -67,7 +67,7 @@ def build_torch_ext(force: bool = False) -> str:
 
     out = os.path.join(HERE, "_C_gguf.so")
     src = os.path.join(CSRC, "torch_bindings.cpp")
-    if not force and not _newer(out, [src, os.path.join(ROOT, "include", "kq_gguf.h")]):
+    if not force and not _newer(out, [src, os.path.join(CSRC, "kq_direct.h"), os.path.join(ROOT, "include", "kq_gguf.h")]):
         return out
     inc = []
     for p in cpp_extension.include_paths("cuda"):
@@ -77,7 +77,7 @@ def build_torch_ext(force: bool = False) -> str:
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
            "-DTORCH_EXTENSION_NAME=_C_gguf", *inc, src, "-o", out,
-           "-L", HERE, "-lkq", "-L", libdir, "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda",
+           "-L", HERE, "-lkq", "-L", libdir, "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-lc10", "-lc10_cuda",
            "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{libdir}"]
     _run(cmd)
     return out

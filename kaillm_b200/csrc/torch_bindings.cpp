@@ -14,6 +14,7 @@
 #include <Python.h>
 
 #include <algorithm>
+#include <cstring>
 
 #include <ATen/ATen.h>
 #include <ATen/MemoryOverlap.h>
@@ -24,6 +25,7 @@
 #include <torch/library.h>
 
 #include "../../include/kq_gguf.h"
+#include "kq_direct.h"
 
 namespace {
 
@@ -551,6 +553,24 @@ TORCH_LIBRARY_IMPL(_C_gguf, CompositeExplicitAutograd, ops) {
   ops.impl("ggml_moe_get_block_size", &ggml_moe_get_block_size);
 }
 
-static struct PyModuleDef kq_module_def = {PyModuleDef_HEAD_INIT, "_C_gguf", nullptr, -1, nullptr};
+// direct(name, overload): the operator's function without the dispatcher, for calls from Python (kq_direct.h)
+static PyMethodDef kq_direct_defs[] = {
+    {"qk_norm_rope", (PyCFunction)(void*)kq_direct::Direct<&qk_norm_rope>::call, METH_FASTCALL, nullptr},
+    {"qk_norm_rope_store", (PyCFunction)(void*)kq_direct::Direct<&qk_norm_rope_store>::call, METH_FASTCALL, nullptr},
+    {"paged_attention", (PyCFunction)(void*)kq_direct::Direct<&paged_attention>::call, METH_FASTCALL, nullptr},
+    {"plan_pages", (PyCFunction)(void*)kq_direct::Direct<&plan_pages>::call, METH_FASTCALL, nullptr},
+    {"moe_route", (PyCFunction)(void*)kq_direct::Direct<&moe_route>::call, METH_FASTCALL, nullptr},
+};
+static PyObject* kq_direct_of(PyObject*, PyObject* args) {
+  const char* name = nullptr;
+  PyObject* overload = nullptr;
+  if (!PyArg_ParseTuple(args, "sO", &name, &overload)) return nullptr;
+  for (PyMethodDef& d : kq_direct_defs)
+    if (!std::strcmp(d.ml_name, name)) return PyCFunction_New(&d, overload);
+  PyErr_Format(PyExc_KeyError, "%s has no direct call", name);
+  return nullptr;
+}
+static PyMethodDef kq_module_methods[] = {{"direct", kq_direct_of, METH_VARARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
+static struct PyModuleDef kq_module_def = {PyModuleDef_HEAD_INIT, "_C_gguf", nullptr, -1, kq_module_methods};
 
 extern "C" PyObject* PyInit__C_gguf(void) { return PyModule_Create(&kq_module_def); }

@@ -86,13 +86,19 @@ def fused_moe_swiglu(X: torch.Tensor, W1: torch.Tensor, W2: torch.Tensor, topk_w
     return torch.ops._C_gguf.fused_moe_swiglu(X, W1, W2, topk_weights, topk_ids, quant_type, quant_type2, block)
 
 
-# The overloads of the operators that a decode step calls in every layer; looking one up, and each Python function around it, costs as
-# much as a tenth of the call, so `attention` and `linear` call these
-QK_NORM_ROPE = torch.ops._C_gguf.qk_norm_rope.default
-QK_NORM_ROPE_STORE = torch.ops._C_gguf.qk_norm_rope_store.default
-PAGED_ATTENTION = torch.ops._C_gguf.paged_attention.default
-PLAN_PAGES = torch.ops._C_gguf.plan_pages.default
-MOE_ROUTE = torch.ops._C_gguf.moe_route.default
+def _direct(name: str):
+    from . import _C_gguf
+
+    return _C_gguf.direct(name, getattr(torch.ops._C_gguf, name).default)
+
+
+# The operators that a decode step calls in every layer, for `attention` and `linear`: positional arguments only; plain calls go past the
+# dispatcher, everything else to the overload in torch.ops (a dispatched call of one token takes 3 to 4 us longer)
+QK_NORM_ROPE = _direct("qk_norm_rope")
+QK_NORM_ROPE_STORE = _direct("qk_norm_rope_store")
+PAGED_ATTENTION = _direct("paged_attention")
+PLAN_PAGES = _direct("plan_pages")
+MOE_ROUTE = _direct("moe_route")
 
 
 def qk_norm_rope(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, num_heads: int, num_kv_heads: int,
