@@ -30,9 +30,11 @@ struct PageParams {
 
 __device__ __forceinline__ int to_int(int64_t v) { return (int)min(v, (int64_t)0x7fffffff); }
 
+__device__ __forceinline__ uint32_t pages_of(uint32_t tokens, int page_size) { return tokens / page_size + (tokens % page_size != 0); }
+
 __global__ void __launch_bounds__(PG_THREADS) plan_pages_kernel(const PageParams p, int range) {
   __shared__ int s_start[PG_THREADS + 1];
-  __shared__ int s_seen[PG_THREADS];
+  __shared__ int2 s_seen[PG_THREADS];                                 // tokens, pages
   __shared__ int64_t s_first[PG_THREADS];
   __shared__ int64_t s_warp[2][32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -45,9 +47,9 @@ __global__ void __launch_bounds__(PG_THREADS) plan_pages_kernel(const PageParams
     const int r = r0 + tid;
     int seen = 0, fresh = 0;
     if (r < p.requests) { seen = max(p.seen[r], 0); fresh = max(p.fresh[r], 0); }
-    const int64_t total = (int64_t)seen + fresh;
-    const int64_t held = ((int64_t)seen + p.page_size - 1) / p.page_size;
-    const int64_t need = max((int64_t)0, min((total + p.page_size - 1) / p.page_size, (int64_t)p.width) - held);
+    const uint32_t total = (uint32_t)seen + fresh;                    // below 2^32, as every position; divisions in 32 bits
+    const int held = pages_of(seen, p.page_size);
+    const int64_t need = max((int64_t)0, (int64_t)min(pages_of(total, p.page_size), (uint32_t)p.width) - held);
     int64_t a = fresh, n = need;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -68,7 +70,7 @@ __global__ void __launch_bounds__(PG_THREADS) plan_pages_kernel(const PageParams
     __syncthreads();
     if (warp > 0) { a += s_warp[0][warp - 1]; n += s_warp[1][warp - 1]; }
     s_start[tid] = to_int(run_new + a - fresh);
-    s_seen[tid] = seen;
+    s_seen[tid] = make_int2(seen, held);
     s_first[tid] = run_need + n - need;
     if (tid == PG_THREADS - 1) s_start[PG_THREADS] = to_int(run_new + a);
     if (blockIdx.x == 0 && r < p.requests) {
@@ -86,16 +88,16 @@ __global__ void __launch_bounds__(PG_THREADS) plan_pages_kernel(const PageParams
         const int mid = (a0 + a1) >> 1;
         if (s_start[mid] <= t) a0 = mid; else a1 = mid;
       }
-      const int64_t pos = (int64_t)s_seen[a0] + (t - s_start[a0]);
-      const int64_t at = pos / p.page_size, have = ((int64_t)s_seen[a0] + p.page_size - 1) / p.page_size;
-      const int place = (int)(pos - at * p.page_size);
+      const int2 held_by = s_seen[a0];
+      const uint32_t pos = (uint32_t)held_by.x + (t - s_start[a0]), at = pos / p.page_size;
+      const int have = held_by.y, place = (int)(pos - at * p.page_size);
       int name = -1;
-      if (at < p.width) {
+      if (at < (uint32_t)p.width) {
         int32_t* entry = p.table + (int64_t)(r0 + a0) * p.table_r + at;
-        if (at < have) {
+        if ((int)at < have) {
           name = *entry;
         } else {
-          const int64_t from = s_first[a0] + (at - have);
+          const int64_t from = s_first[a0] + ((int)at - have);
           if (from >= 0 && from < p.num_free) name = p.free_pages[from];
           if (place == 0) *entry = name;
         }
