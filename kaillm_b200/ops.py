@@ -87,6 +87,11 @@ def fused_moe_swiglu(X: torch.Tensor, W1: torch.Tensor, W2: torch.Tensor, topk_w
 
 
 def _direct(name: str):
+    if not hasattr(torch.ops._C_gguf, name):       # the namespace is another library's, with the reference's operators only
+        def missing(*args):
+            raise ImportError(f"torch.ops._C_gguf was registered by another library, which has no {name}")
+
+        return missing
     from . import _C_gguf
 
     return _C_gguf.direct(name, getattr(torch.ops._C_gguf, name).default)

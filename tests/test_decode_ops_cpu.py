@@ -1,6 +1,8 @@
 """Bad arguments of the operators between a decode step's projections come back as the documented codes, before any GPU work; the
 plain forms that their GPU tests use agree with each other."""
 import ctypes
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -97,6 +99,33 @@ def test_plain_forms():
     assert ids.tolist() == [[1, 0]] and w.sum() == pytest.approx(1.0)
     t, total, starts, pos, slots, taken = pages([[3, -1]], [7], [3], [9, 4], 1, 8, 4)
     assert (t, total, starts, pos, slots, taken) == ([[3, 4]], [10], [0, 3], [7, 8, 9, 0], [31, 32, 33, -1], 2)
+
+
+def test_beside_another_library_of_the_same_namespace():
+    """Where the reference's operators are registered already, this package uses those, and says that it has no others."""
+    code = """
+import torch
+lib = torch.library.Library("_C_gguf", "DEF")
+lib.define("ggml_mul_mat_vec_a8(Tensor W, Tensor X, int type, int row) -> Tensor")
+lib.impl("ggml_mul_mat_vec_a8", lambda W, X, type, row: X + row, "CPU")
+from kaillm_b200 import attention, linear, ops
+assert ops.ggml_mul_mat_vec_a8(torch.zeros(1), torch.zeros(1), 2, 3).item() == 3
+try:
+    linear.route_experts(torch.zeros(1, 4), 2)
+except ImportError as e:
+    assert "moe_route" in str(e)
+else:
+    raise AssertionError
+"""
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=300)
+
+
+def test_calls_that_are_not_plain_reach_the_overload():
+    from kaillm_b200 import linear, ops
+
+    for bad in (lambda: linear.route_experts(torch.zeros(2, 8), 2), lambda: ops.MOE_ROUTE(1), lambda: ops.PAGED_ATTENTION(), lambda: ops.PLAN_PAGES(*[None] * 7)):
+        with pytest.raises((RuntimeError, NotImplementedError, TypeError)):
+            bad()
 
 
 def test_a_stack_refuses_attention_that_does_not_fit():
