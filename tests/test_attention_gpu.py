@@ -218,6 +218,54 @@ def test_side_stream():
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_a_cache_beyond_32_bit_offsets(dtype):
+    """Pages whose first element lies behind 2^32, written by the rotation and read back."""
+    kv, d, page, n = 8, 128, 16, 75
+    pages = 2 ** 32 // (page * kv * d) + 40
+    kc, vc = (torch.empty((pages, page, kv, d), dtype=DT[dtype], device=dev()) for _ in range(2))
+    table = torch.tensor([[pages - 1, pages - 30, 3, pages - 2, pages - 17]], dtype=torch.int32, device=dev())
+    g = torch.Generator().manual_seed(3)
+    qkv = torch.randn((n, (16 + 2 * kv) * d), generator=g).to(DT[dtype]).to(dev())
+    at = torch.arange(n, device=dev())
+    slots = table[0].long()[at // page] * page + at % page
+    freq = torch.rand(d // 2, generator=g).to(dev())
+    q = attention.qk_norm_rope_store(qkv, at, freq, 16, kc, vc, slots)
+    _, k = attention.qk_norm_rope(qkv, at, freq, 16, kv)
+    assert torch.equal(kc[table[0].long()].flatten(0, 1)[:n], k) and torch.equal(vc[table[0].long()].flatten(0, 1)[:n], qkv[:, 24 * d:].unflatten(1, (kv, d)))
+    lens = torch.tensor([n], dtype=torch.int32, device=dev())
+    got = attention.paged_attention(q[-1:], kc, vc, table, lens, scale=0.1)
+    few = table[0].long()
+    small = torch.arange(5, dtype=torch.int32, device=dev())[None]
+    want, _, eo, _ = attend(q[-1:], kc[few], vc[few], small, [n], 0.1, 0, 0.0)
+    check_attention(got, want, eo, dtype)
+    wide = torch.cat([table, torch.full((1, 60), -1, dtype=torch.int32, device=dev())], 1)      # divided among workers
+    check_attention(attention.paged_attention(q[-1:], kc, vc, wide, lens, scale=0.1), want, eo, dtype)
+
+
+def test_two_graphs_at_once():
+    """Captured calls with scratch of their own, replayed on two streams at the same time."""
+    sets = []
+    for seed, lens in ((1, [3000, 7, 900, 1500]), (2, [1, 4000, 2500, 0, 333])):
+        k, v, table = paged_cache(lens, 4, 128, 16, "bf16", dev(), seed)
+        q = torch.randn((len(lens), 16, 128), generator=torch.Generator().manual_seed(seed)).bfloat16().to(dev())
+        n = torch.tensor(lens, dtype=torch.int32, device=dev())
+        want = attention.paged_attention(q, k, v, table, n)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = [attention.paged_attention(q, k, v, table, n) for _ in range(3)]
+        sets.append((graph, outs, want, torch.cuda.Stream(), (q, k, v, table, n)))
+    for _ in range(20):
+        for graph, outs, want, stream, _ in sets:
+            with torch.cuda.stream(stream):
+                for o in outs:
+                    o.zero_()
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, want) for _, outs, want, _, _ in sets for o in outs)
+
+
 def test_no_wait_has_run_out():
     run([5000, 0, 77], 8, 2, 128, 16, "bf16")
     assert capi.paged_attention_status() == 0
