@@ -533,9 +533,15 @@ __device__ __forceinline__ void ring_wait(uint32_t bar, uint32_t parity, volatil
 }
 
 // 16-bit types: m16n8k16 products.  The query heads of a tile are the 16 rows, a step is 16 or 32 cached keys.  Scores: A = q (registers), B =
-// keys; values: A = weights (the score accumulators are already in A's layout), B = values (transposed by ldmatrix).  The weights
-// enter as two 16-bit parts, so that they count with 16 bits and more; up to eight heads leave the upper eight rows free, and the
-// low parts ride there at no cost (TWO = false); above that they are a second product.
+// keys; values: A = weights (the score accumulators are already in A's layout), B = values (transposed by ldmatrix).
+//
+// The weights enter as two 16-bit parts: 22 bits of them for fp16, 17 for bf16.  Up to eight heads leave the upper eight rows free, and
+// the low parts ride there (TWO = false); above that they are a second product.  Before its rounding to bf16 an output is off by 1.3 to
+// 1.9e-6 (of the norm; a step of bf16 is 4e-3); a third part makes that 3 to 7e-7 and costs 64 sequences of 0..16384 tokens 2 %, 16 heads
+// per key head 11 %, so it is left out.
+// The products cut the sum that they add to off instead of rounding it.  Each tile's sum therefore starts at zero and is added to the
+// running one in a rounded fp32 addition: the running sum as the accumulator drifted towards zero by 2.6e-6 over the longest of
+// these sequences, 5.2e-6 with 12 heads per key head, and further with the length (now 2 to 3e-7); one addition per value and tile costs up to 1 %.
 //
 // Bound by memory where sequences are long: 64 of 0..16384 tokens, 40 / 8 heads of 128, bf16 (2.1 GB) 357 us, 6.0 TB/s; one of 131071 (537 MB)
 // 98 us, 5.5 TB/s; 16 of 900..3100 (131 MB) 31.1 us, 4.2 TB/s, of which 3 us pass until the first keys are there and 5 us in the join.  The
@@ -551,6 +557,7 @@ __global__ void __launch_bounds__(MmaShape<DP, TWO>::THREADS, 1) attend_mma_kern
   constexpr int R = S::R, NC = S::NC, NS = S::SLOTS, KEYS = S::KEYS, NT = KEYS / 8;
   static_assert(NS % NC == 0 && NC == MM_COPIERS, "private rings");
   constexpr uint32_t ALL = KEYS == 32 ? 0xffffffffu : 0xffffu;
+  constexpr int OV = TWO ? 4 : 2;                                // values of a lane per 8 columns
   constexpr float LIFT = std::is_same<T, __half>::value ? 12.f : 0.f;   // weights up to 2^12: fp16's small numbers begin at 2^-24
   extern __shared__ __align__(128) uint8_t tl_smem[];
   float* s_join = reinterpret_cast<float*>(tl_smem + NS * S::SLOT);
@@ -679,11 +686,11 @@ __global__ void __launch_bounds__(MmaShape<DP, TWO>::THREADS, 1) attend_mma_kern
   while (more) {
     const Segment now = s;
     const int count = now.t1 - now.t0;
-    float o[DP / 8][4];
+    float o[DP / 8][OV];
 #pragma unroll
     for (int i = 0; i < DP / 8; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+      for (int e = 0; e < OV; ++e) o[i][e] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};       // rows g and g + 8, m less LIFT; l: of the lane's own keys
 
     for (; n - n0 < count; n += stride) {
@@ -736,10 +743,7 @@ __global__ void __launch_bounds__(MmaShape<DP, TWO>::THREADS, 1) attend_mma_kern
           const float f = ex2(m[half] - base);
           l[half] *= f;
 #pragma unroll
-          for (int i = 0; i < DP / 8; ++i) {
-            o[i][2 * half] *= f; o[i][2 * half + 1] *= f;
-            if constexpr (!TWO) { o[i][2] *= f; o[i][3] *= f; }
-          }
+          for (int i = 0; i < DP / 8; ++i) { o[i][2 * half] *= f; o[i][2 * half + 1] *= f; }
         }
         m[half] = mn;
 #pragma unroll
@@ -751,21 +755,26 @@ __global__ void __launch_bounds__(MmaShape<DP, TWO>::THREADS, 1) attend_mma_kern
       }
 #pragma unroll
       for (int cc = 0; cc < DP / 16; ++cc) {
-        {
+        float sum[2][4] = {};                                     // of this tile
 #pragma unroll
-          for (int j = 0; j < KEYS / 16; ++j) {
-            uint32_t vb[4];
-            ldsm4_t(vb, v_at + off + cc * 32 + j * 16 * S::ROW);
+        for (int j = 0; j < KEYS / 16; ++j) {
+          uint32_t vb[4];
+          ldsm4_t(vb, v_at + off + cc * 32 + j * 16 * S::ROW);
 #pragma unroll
-            for (int n2 = 0; n2 < 2; ++n2) {
-              if constexpr (TWO) {
-                mma16816<T>(o[2 * cc + n2], hi[j][0], hi[j][1], hi[j][2], hi[j][3], vb[2 * n2], vb[2 * n2 + 1]);
-                mma16816<T>(o[2 * cc + n2], lo[j][0], lo[j][1], lo[j][2], lo[j][3], vb[2 * n2], vb[2 * n2 + 1]);
-              } else {
-                mma16816<T>(o[2 * cc + n2], hi[j][0], lo[j][0], hi[j][2], lo[j][2], vb[2 * n2], vb[2 * n2 + 1]);
-              }
+          for (int n2 = 0; n2 < 2; ++n2) {
+            if constexpr (TWO) {
+              mma16816<T>(sum[n2], hi[j][0], hi[j][1], hi[j][2], hi[j][3], vb[2 * n2], vb[2 * n2 + 1]);
+              mma16816<T>(sum[n2], lo[j][0], lo[j][1], lo[j][2], lo[j][3], vb[2 * n2], vb[2 * n2 + 1]);
+            } else {
+              mma16816<T>(sum[n2], hi[j][0], lo[j][0], hi[j][2], lo[j][2], vb[2 * n2], vb[2 * n2 + 1]);
             }
           }
+        }
+#pragma unroll
+        for (int n2 = 0; n2 < 2; ++n2) {
+          if constexpr (!TWO) { sum[n2][0] += sum[n2][2]; sum[n2][1] += sum[n2][3]; }      // high and low parts
+#pragma unroll
+          for (int e = 0; e < OV; ++e) o[2 * cc + n2][e] += sum[n2][e];
         }
       }
       __syncwarp();
@@ -782,10 +791,6 @@ __global__ void __launch_bounds__(MmaShape<DP, TWO>::THREADS, 1) attend_mma_kern
       l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
       l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
       if (t4 == 0) s_ml[warp * R + g + half * 8] = make_float2(m[half], l[half]);
-    }
-    if constexpr (!TWO) {                                         // high and low parts
-#pragma unroll
-      for (int i = 0; i < DP / 8; ++i) { o[i][0] += o[i][2]; o[i][1] += o[i][3]; }
     }
     const int h = now.sub / p.row_tiles, x = now.sub - h * p.row_tiles;
     const int head0 = h * p.group + x * p.rows, rows = min(p.rows, p.group - x * p.rows);
