@@ -102,6 +102,14 @@ class StepAttention:
         self.seq_lens.copy_(total)
         self.taken.copy_(taken)
 
+    def check(self) -> None:
+        """Synchronises; raises if a bounded wait inside `paged_attention` ran out on this device (its outputs are then undefined)."""
+        from . import capi
+
+        status = capi.paged_attention_status(device=self.seq_lens.device)
+        if status:
+            raise RuntimeError(f"paged attention: kernel status {status} (a bounded wait ran out)")
+
     def layer(self, index: int, qkv: torch.Tensor) -> torch.Tensor:
         """The attention output [m, num_heads * head dim] of layer `index` for this step's merged projection."""
         k_cache, v_cache = self.caches[index]

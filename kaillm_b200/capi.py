@@ -374,10 +374,11 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
             scratch.data_ptr(), scratch.numel(), _stream(q.device)))
 
 
-def paged_attention_status(clear: bool = False) -> int:
-    """kq_paged_attention_status on the current device (synchronises): non-zero when a wait inside the kernel has run out."""
+def paged_attention_status(clear: bool = False, device: torch.device | None = None) -> int:
+    """kq_paged_attention_status on `device` (default: the current one; synchronises): non-zero when a wait inside the kernel has run out."""
     v = ctypes.c_int()
-    _check(lib.kq_paged_attention_status(ctypes.byref(v), int(clear)))
+    with torch.cuda.device(device):
+        _check(lib.kq_paged_attention_status(ctypes.byref(v), int(clear)))
     return v.value
 
 

@@ -267,6 +267,8 @@ class DecoderStack:
             if st:
                 raise RuntimeError(f"decoder stack: kernel status {st} (a bounded wait inside the last GEMV ran out)")
             break   # the status word sits at offset 0 for every shape
+        if self.attention is not None:
+            self.attention.check()
         if self.p2p is not None:
             self.p2p.check()
             if self.wait_in_consumer:

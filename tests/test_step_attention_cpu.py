@@ -1,0 +1,29 @@
+"""What a decode step's attention reports and refuses, without a GPU."""
+import pytest
+import torch
+
+from kaillm_b200 import capi, sharded
+from kaillm_b200.attention import StepAttention
+
+
+def step_attention(layers=1, seqs=2, heads=4, kv=2, d=16, width=2):
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32)    # noqa: E731
+    return StepAttention([[torch.zeros(3, 8, kv, d), torch.zeros(3, 8, kv, d)] for _ in range(layers)], heads, torch.ones(d // 2), i32(seqs, width), i32(seqs), i32(3), i32(1))
+
+
+def layer(qkv=128, o=64):
+    return {name: (torch.zeros((n, k // 32 * 34), dtype=torch.uint8), 8, n, k) for name, (n, k) in
+            {"qkv": (qkv, 64), "o": (64, o), "gate_up": (128, 64), "down": (64, 64)}.items()}
+
+
+def test_a_stack_reports_an_attention_that_gave_up(monkeypatch):
+    status = {"value": 0}
+    monkeypatch.setattr(capi, "read_status", lambda *a: 0)
+    monkeypatch.setattr(capi, "paged_attention_status", lambda clear=False, device=None: status["value"])
+    stack = sharded.DecoderStack([layer()], 2, 64, torch.device("cpu"), attention=step_attention())
+    plain = sharded.DecoderStack([layer()], 2, 64, torch.device("cpu"))
+    stack.check()
+    status["value"] = 1
+    plain.check()
+    with pytest.raises(RuntimeError, match="paged attention"):
+        stack.check()
