@@ -301,28 +301,6 @@ at::Tensor new_cuda(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor
   return at::Tensor(at::detail::empty_cuda(sizes, type, like.device(), std::nullopt));
 }
 
-// Several outputs of a call in one allocation, each a tensor of its own over its part of the storage (16-byte aligned).
-struct Outputs {
-  explicit Outputs(const at::Tensor& like_) : like(like_) {}
-  void add(at::IntArrayRef sizes, at::ScalarType type) {
-    parts.push_back({c10::DimVector(sizes), type, bytes});
-    bytes = (bytes + (int64_t)c10::elementSize(type) * c10::multiply_integers(sizes) + 15) / 16 * 16;
-  }
-  void allocate() { whole = new_cuda({bytes}, at::kByte, like); }
-  at::Tensor operator[](size_t i) const {
-    const Part& p = parts[i];
-    at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), c10::scalarTypeToTypeMeta(p.type));
-    t.unsafeGetTensorImpl()->set_storage_offset(whole.storage_offset() + p.at / (int64_t)c10::elementSize(p.type));
-    t.unsafeGetTensorImpl()->set_sizes_contiguous(p.sizes);
-    return t;
-  }
-  struct Part { c10::DimVector sizes; at::ScalarType type; int64_t at; };
-  const at::Tensor& like;
-  c10::SmallVector<Part, 5> parts;
-  int64_t bytes = 0;
-  at::Tensor whole;
-};
-
 void no_gradient(const char* fn, std::initializer_list<const at::Tensor*> ts) {
   if (!at::GradMode::is_enabled()) return;
   for (const at::Tensor* t : ts) TORCH_CHECK(!t->defined() || !t->requires_grad(), fn, ": has no derivative, and an input requires one");
@@ -455,14 +433,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> plan_page
   TORCH_CHECK(seq_lens.size(0) == r && new_lens.size(0) == r && taken.size(0) == 1, fn, ": one length per row of block_table, and one value in taken");
   TORCH_CHECK(num_tokens >= 0 && page_size > 0, fn, ": page_size must be positive and num_tokens not negative");
   const c10::cuda::CUDAGuard guard(block_table.device());
-  Outputs outs(block_table);
-  outs.add({r}, at::kInt);
-  outs.add({r + 1}, at::kInt);
-  outs.add({num_tokens}, at::kInt);
-  outs.add({num_tokens}, at::kLong);
-  outs.add({1}, at::kInt);
-  outs.allocate();
-  at::Tensor total = outs[0], starts = outs[1], positions = outs[2], slots = outs[3], after = outs[4];
+  at::Tensor total = new_cuda({r}, at::kInt, block_table), starts = new_cuda({r + 1}, at::kInt, block_table), after = new_cuda({1}, at::kInt, block_table);
+  at::Tensor positions = new_cuda({num_tokens}, at::kInt, block_table), slots = new_cuda({num_tokens}, at::kLong, block_table);
   TORCH_CHECK(kq_plan_pages(block_table.data_ptr<int32_t>(), block_table.stride(0), block_table.size(1), seq_lens.data_ptr<int32_t>(), new_lens.data_ptr<int32_t>(), r,
                             free_pages.data_ptr<int32_t>(), free_pages.size(0), taken.data_ptr<int32_t>(), page_size, num_tokens,
                             total.data_ptr<int32_t>(), starts.data_ptr<int32_t>(), positions.data_ptr<int32_t>(), slots.data_ptr<int64_t>(),
@@ -485,11 +457,7 @@ std::tuple<at::Tensor, at::Tensor> moe_route(const at::Tensor& logits, int64_t t
   no_gradient(fn, {&logits, &bias});
   TORCH_CHECK(top_k > 0 && top_k <= e, fn, ": top_k=", top_k, " is not between 1 and ", e);
   const c10::cuda::CUDAGuard guard(logits.device());
-  Outputs outs(logits);
-  outs.add({t, top_k}, at::kFloat);
-  outs.add({t, top_k}, at::kInt);
-  outs.allocate();
-  at::Tensor w = outs[0], ids = outs[1];
+  at::Tensor w = new_cuda({t, top_k}, at::kFloat, logits), ids = new_cuda({t, top_k}, at::kInt, logits);
   TORCH_CHECK(kq_moe_route(logits.data_ptr(), dt, t, e, logits.stride(0), top_k, sigmoid, bias.defined() ? bias.data_ptr<float>() : nullptr, groups, top_groups,
                            renormalize, (float)scale, w.data_ptr<float>(), ids.data_ptr<int32_t>(),
                            (void*)at::cuda::getCurrentCUDAStream(logits.get_device()).stream()) == KQ_OK, fn, ": ", kq_last_error());
