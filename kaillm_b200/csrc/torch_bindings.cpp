@@ -21,6 +21,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/CUDAEvent.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
 
@@ -301,9 +302,11 @@ at::Tensor new_cuda(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor
   return at::Tensor(at::detail::empty_cuda(sizes, type, like.device(), std::nullopt));
 }
 
+// no input that backward or forward differentiation would follow (a tangent also counts under no_grad, which is backward's alone)
 void no_gradient(const char* fn, std::initializer_list<const at::Tensor*> ts) {
-  if (!at::GradMode::is_enabled()) return;
-  for (const at::Tensor* t : ts) TORCH_CHECK(!t->defined() || !t->requires_grad(), fn, ": has no derivative, and an input requires one");
+  const bool backward = at::GradMode::is_enabled(), forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+  for (const at::Tensor* t : ts)
+    TORCH_CHECK(!t->defined() || !((backward && t->requires_grad()) || (forward && t->_fw_grad(0).defined())), fn, ": has no derivative, and an input requires one");
 }
 
 // defined, on `like`'s device and of one of the given types
