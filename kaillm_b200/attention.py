@@ -76,7 +76,12 @@ class StepAttention:
     caches: per layer a pair (k_cache, v_cache) [pages, page size, kv heads, head dim].  block_table int32 [m, pages per sequence],
     seq_lens int32 [m] (tokens in the caches), free_pages int32 and taken int32 [1] are the program's own tensors; every step moves
     them on in place, so a captured step does so at each replay.  q_weights / k_weights: per layer the norm weights of queries and
-    keys, or None.  The other arguments are those of `qk_norm_rope_store` and `paged_attention`."""
+    keys, or None.  The other arguments are those of `qk_norm_rope_store` and `paged_attention`.
+
+    A sequence whose row of block_table is full, or for which free_pages has run out, has no place for its new token: seq_lens counts
+    it, but its key and value are in no cache, and the outputs from then on are without it.  A step cannot stop for that (it does not
+    look at the GPU's values), so `dropped` [m] turns to -1 for such a sequence and stays so, and `check` raises.  A program that has
+    dealt with it (ended the sequence, or started it again with more pages) sets its entry of `dropped` back to 0."""
 
     def __init__(self, caches, num_heads: int, inv_freq: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
                  free_pages: torch.Tensor, taken: torch.Tensor, *, q_weights=None, k_weights=None, eps: float = 1e-6,
@@ -93,6 +98,7 @@ class StepAttention:
         self.q_weights, self.k_weights = (w if w is not None else [None] * len(self.caches) for w in (q_weights, k_weights))
         self.eps, self.interleaved, self.factor, self.scale, self.window, self.softcap = eps, interleaved, factor, scale, window, softcap
         self.one_each = torch.ones_like(seq_lens)
+        self.dropped = torch.zeros_like(seq_lens, dtype=torch.int64)
         self.positions = self.slots = None
 
     def begin_step(self) -> None:
@@ -101,14 +107,19 @@ class StepAttention:
                                                                  self.page_size, self.seq_lens.shape[0])
         self.seq_lens.copy_(total)
         self.taken.copy_(taken)
+        torch.minimum(self.dropped, self.slots, out=self.dropped)       # a slot is -1 where there is no page
 
     def check(self) -> None:
-        """Synchronises; raises if a bounded wait inside `paged_attention` ran out on this device (its outputs are then undefined)."""
+        """Synchronises; raises if a sequence has had no room for a token, or if a bounded wait inside `paged_attention` ran out on this
+        device (its outputs are then undefined)."""
         from . import capi
 
         status = capi.paged_attention_status(device=self.seq_lens.device)
         if status:
             raise RuntimeError(f"paged attention: kernel status {status} (a bounded wait ran out)")
+        lost = self.dropped.nonzero().flatten().tolist()
+        if lost:
+            raise RuntimeError(f"no page for new tokens of the sequences {lost}: their rows of block_table are full, or free_pages has run out")
 
     def layer(self, index: int, qkv: torch.Tensor) -> torch.Tensor:
         """The attention output [m, num_heads * head dim] of layer `index` for this step's merged projection."""

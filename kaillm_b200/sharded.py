@@ -261,7 +261,7 @@ class DecoderStack:
         return buf.permute(1, 0, 2).reshape(self.m, n)     # a transposing copy: the baseline the peer-store gather removes
 
     def check(self) -> None:
-        """Synchronises; raises if a bounded wait inside any kernel of the stack ran out."""
+        """Synchronises; raises if a bounded wait inside any kernel of the stack ran out, or a sequence has had no room for a token."""
         for name, (qt, m, n, k) in self.ws_shape.items():
             st = self._capi.read_status(qt, m, n, k, self.scratch)
             if st:

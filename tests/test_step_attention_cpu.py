@@ -27,3 +27,34 @@ def test_a_stack_reports_an_attention_that_gave_up(monkeypatch):
     plain.check()
     with pytest.raises(RuntimeError, match="paged attention"):
         stack.check()
+
+
+@pytest.mark.parametrize("free,width", [([5, 6], 2), ([5, 6, 7, 8, 9, 4], 1)])
+def test_a_token_without_a_page_is_reported(monkeypatch, free, width):
+    """The list runs out for the second sequence; the row of both ends."""
+    from kaillm_b200 import attention
+    from tests.attention_util import pages
+
+    def plan(table, seen, new, free_pages, taken, page, tokens):
+        t, *rest, after = pages(table.tolist(), seen.tolist(), new.tolist(), free_pages.tolist(), int(taken), page, tokens)
+        table.copy_(torch.tensor(t, dtype=torch.int32))
+        total, starts, positions, slots = (torch.tensor(v) for v in rest)
+        return total.int(), starts.int(), positions.int(), slots, torch.tensor([after], dtype=torch.int32)
+
+    monkeypatch.setattr(attention, "plan_pages", plan)
+    monkeypatch.setattr(capi, "paged_attention_status", lambda clear=False, device=None: 0)
+    att = step_attention(width=width)
+    att.free_pages = torch.tensor(free, dtype=torch.int32)
+    for _ in range(8):                       # the first page of each
+        att.begin_step()
+    att.check()
+    if width == 2:                           # one more page, for one of them
+        att.free_pages = torch.tensor(free + [7], dtype=torch.int32)
+    att.begin_step()
+    lost = [1] if width == 2 else [0, 1]
+    for _ in range(2):                       # and it stays so
+        with pytest.raises(RuntimeError, match=str(lost).replace("[", r"\[")):
+            att.check()
+        att.begin_step()
+    att.dropped.zero_()
+    att.check()
