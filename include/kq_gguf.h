@@ -335,7 +335,7 @@ int kq_moe_combine(const void* y, int dtype, const void* weights, int w_dtype, i
  *   v_cache = NULL: k_out = [tokens, kv_heads, head_dim] dense, the values are left alone; otherwise k_out is the key cache, and
  *              keys and values of token t go to slots[t] (int32 / int64 as slots64); a slot outside [0, num_pages * page_size) is
  *              skipped, and two tokens with the same slot leave it with values of either
- * head_dim: even, at most 512.  Outputs must not overlap the inputs. */
+ * head_dim: even, at most 512.  Outputs must overlap neither the inputs nor each other (equal pointers are refused). */
 int kq_qk_norm_rope(const void* qkv, int dtype, int64_t tokens, int64_t stride_t, int64_t heads, int64_t kv_heads,
                     int64_t head_dim, const void* positions, int positions64, const float* inv_freq, int64_t rotated,
                     int interleaved, float factor, const void* q_weight, const void* k_weight, int w_dtype, float eps,

@@ -39,7 +39,7 @@ def qk_norm_rope_store(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: tor
                        factor: float = 1.0) -> torch.Tensor:
     """`qk_norm_rope` that returns the queries and writes the rotated keys and the values of token t into slot slots[t] of the caches
     (slot = page * page size + place; int32 or int64; a slot outside the cache, -1 for instance, is skipped).  Slots should be
-    distinct: one that is named twice holds values of either token."""
+    distinct: one that is named twice holds values of either token.  The caches must not overlap each other or qkv."""
     return QK_NORM_ROPE_STORE(qkv, positions, inv_freq, num_heads, k_cache, v_cache, slots, q_weight, k_weight, eps, interleaved, factor)
 
 

@@ -473,6 +473,10 @@ extern "C" int kq_qk_norm_rope(const void* qkv, int dtype, int64_t tokens, int64
     set_error("%s: misaligned pointer", fn);
     return KQ_EINVAL;
   }
+  if (q_out == qkv || k_out == qkv || v_cache == qkv || k_out == q_out || v_cache == k_out || v_cache == q_out) {
+    set_error("%s: outputs must be neither inputs nor each other", fn);
+    return KQ_EINVAL;
+  }
   RopeParams p;
   p.qkv = qkv; p.qkv_t = tokens > 1 ? stride_t : 0; p.positions = positions; p.pos64 = positions64; p.inv_freq = inv_freq;
   p.qw = q_weight; p.kw = k_weight; p.w_f32 = w_dtype == KQ_F32; p.eps = eps; p.factor = factor; p.inv_dim = 1.f / (float)head_dim; p.tokens = tokens;

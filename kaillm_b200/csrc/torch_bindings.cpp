@@ -14,7 +14,9 @@
 #include <Python.h>
 
 #include <algorithm>
+#include <cstdlib>
 #include <cstring>
+#include <utility>
 
 #include <ATen/ATen.h>
 #include <ATen/MemoryOverlap.h>
@@ -354,6 +356,45 @@ void cache_checks(const char* fn, const at::Tensor& k, const at::Tensor& v, cons
   no_gradient(fn, {&k, &v});
 }
 
+// addresses [first, second) that a view spans
+std::pair<uintptr_t, uintptr_t> span_of(const at::Tensor& t) {
+  const uintptr_t begin = (uintptr_t)t.const_data_ptr();
+  if (t.numel() == 0) return {begin, begin};
+  int64_t last = 0;
+  for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+  return {begin, begin + (uintptr_t)(last + 1) * t.element_size()};
+}
+bool spans_meet(const at::Tensor& a, const at::Tensor& b) {
+  const auto x = span_of(a), y = span_of(b);
+  return x.first < y.second && y.first < x.second;
+}
+// whether some sum of stride[i] * d[i], |d[i]| < size[i], is `off`; strides descending.  A stride that is no less than what the later ones
+// reach leaves two values of d to try; where there are more (views of no usual layout) the answer is no.
+bool reachable(int64_t off, const std::pair<int64_t, int64_t>* dims, int n) {
+  if (n == 0) return off == 0;
+  int64_t rest = 0;
+  for (int i = 1; i < n; ++i) rest += dims[i].first * (dims[i].second - 1);
+  if (std::abs(off) > rest + dims[0].first * (dims[0].second - 1)) return false;
+  int tried = 0;
+  for (int64_t d = std::max((off - rest) / dims[0].first - 1, 1 - dims[0].second); d < dims[0].second && off - d * dims[0].first >= -rest; ++d)
+    if (off - d * dims[0].first <= rest && tried++ < 4 && reachable(off - d * dims[0].first, dims + 1, n - 1)) return true;
+  return false;
+}
+// Whether two caches of one size and type share an element: exact for equal strides (also where keys and values lie page by page or
+// head by head in one tensor) and for dense tensors
+bool caches_meet(const at::Tensor& a, const at::Tensor& b) {
+  if (!spans_meet(a, b)) return false;
+  c10::SmallVector<std::pair<int64_t, int64_t>, 4> dims;
+  for (int64_t i = 0; i < a.dim(); ++i)
+    if (a.size(i) > 1) {
+      if (a.stride(i) != b.stride(i)) return at::get_overlap_status(a, b) != at::MemOverlapStatus::No && at::get_overlap_status(a, b) != at::MemOverlapStatus::TooHard;
+      dims.push_back({a.stride(i), a.size(i)});
+    }
+  std::sort(dims.begin(), dims.end(), [](const auto& x, const auto& y) { return x.first > y.first; });
+  const int64_t bytes = (int64_t)((intptr_t)b.const_data_ptr() - (intptr_t)a.const_data_ptr()), size = a.element_size();
+  return bytes % size != 0 || reachable(bytes / size, dims.data(), (int)dims.size());
+}
+
 std::tuple<at::Tensor, at::Tensor> qk_norm_rope(const at::Tensor& qkv, const at::Tensor& positions, const at::Tensor& inv_freq, int64_t heads,
                                                 int64_t kv, const std::optional<at::Tensor>& q_weight, const std::optional<at::Tensor>& k_weight,
                                                 double eps, bool interleaved, double factor) {
@@ -378,6 +419,8 @@ at::Tensor qk_norm_rope_store(const at::Tensor& qkv, const at::Tensor& positions
   at::assert_no_internal_overlap(v_cache);
   cache_checks(fn, k_cache, v_cache, qkv);
   TORCH_CHECK(k_cache.size(0) > 0 && k_cache.size(1) > 0, fn, ": the caches have no pages");
+  TORCH_CHECK(!caches_meet(k_cache, v_cache), fn, ": the caches of keys and values overlap");
+  TORCH_CHECK(!spans_meet(qkv, k_cache) && !spans_meet(qkv, v_cache), fn, ": qkv lies in a cache");
   const RopeCall c = rope_checks(fn, qkv, positions, inv_freq, heads, k_cache.size(2), q_weight, k_weight);
   TORCH_CHECK(k_cache.size(3) == c.d, fn, ": the caches hold heads of ", k_cache.size(3), " values, qkv of ", c.d);
   check_on(fn, "slots", slots, qkv, {at::kInt, at::kLong});

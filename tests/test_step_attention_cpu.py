@@ -58,3 +58,12 @@ def test_a_token_without_a_page_is_reported(monkeypatch, free, width):
         att.begin_step()
     att.dropped.zero_()
     att.check()
+
+
+def test_qk_norm_rope_refuses_outputs_that_are_inputs_or_each_other():
+    from tests.test_decode_ops_cpu import EINVAL, S3, _rope
+
+    cache = dict(v=0x6000, ks=S3(4096, 256, 128), vs=S3(4096, 256, 128), slots=0x7000, pages=3, page=16)
+    for bad in (dict(q=0x1000), dict(k=0x1000), dict(q=0x5000), dict(cache, v=0x5000), dict(cache, v=0x1000), dict(cache, v=0x4000)):
+        assert _rope(**bad) == EINVAL, bad
+        assert "outputs" in capi.lib.kq_last_error().decode()
