@@ -391,8 +391,10 @@ int kq_plan_pages(int32_t* block_table, int64_t table_stride, int64_t table_widt
  *   the experts of the top_groups best groups stay
  *   ids [tokens, top_k] int32: the best c, descending, ties (of groups too) to the lowest index; weights [tokens, top_k] fp32:
  *   p of the chosen, divided by their sum if renormalize != 0 (zeros where that is 0), times scale
- * NaN counts as -infinity and +infinity as the largest finite number; experts at -infinity come last, with weight 0 for softmax
- * and sigmoid alike.  At most 1024 experts, top_k 32, 32 groups. */
+ * NaN counts as -infinity and +infinity as the largest finite number, in the bias too.  An expert with a logit of -infinity has p = 0
+ * and, when chosen, weight 0, for softmax and sigmoid alike.  Without a bias such experts come last; with one they count with c = bias
+ * as everywhere in the formula, so they CAN come before others (and in groups count for theirs): where they must not, their bias has
+ * to be -infinity as well, which places an expert last whatever its logit.  At most 1024 experts, top_k 32, 32 groups. */
 int kq_moe_route(const void* logits, int dtype, int64_t tokens, int64_t experts, int64_t stride_t, int64_t top_k,
                  int sigmoid, const float* bias, int64_t groups, int64_t top_groups, int renormalize, float scale,
                  float* weights, int32_t* ids, void* stream);

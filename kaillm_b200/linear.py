@@ -142,7 +142,8 @@ def route_experts(router_logits: torch.Tensor, top_k: int, *, scoring: str = "so
     scoring "softmax" or "sigmoid" over the experts; bias (float32 [experts]): added for the choice only.  groups > 1: only the experts
     of the top_groups best of `groups` equal runs of experts can be chosen; a run counts its best expert, with a bias the sum of its
     two best.  Ids come best first, ties to the lowest index.  renormalize: the weights of a token sum to 1; then times scale.
-    NaN counts as -inf; masked experts (-inf) come last with weight 0.  At most 1024 experts, top_k 32, 32 groups; no gradient."""
+    NaN counts as -inf.  An expert at -inf has probability 0 and weight 0: without a bias it comes last; with one it counts with its bias
+    alone and can be chosen before others, unless its bias is -inf too.  At most 1024 experts, top_k 32, 32 groups; no gradient."""
     if scoring not in ("softmax", "sigmoid"):
         raise ValueError(f"scoring must be 'softmax' or 'sigmoid', got {scoring!r}")
     return ops.MOE_ROUTE(router_logits, top_k, scoring == "sigmoid", bias, groups, top_groups, renormalize, scale)
