@@ -178,7 +178,12 @@ __device__ __forceinline__ float unordered(uint32_t k) { return __uint_as_float(
 // (4 + |x|) u of itself; a sigmoid by p (1 - p) (4 + |x|) u + 4 p u < 5.5 u; a softmax by 30 p u (its sum of up to 1024 terms
 // included), so two of them, or the four of two groups, by 30 u together; the sum with the bias by another u of itself.  64 u are asked for.
 constexpr float RT_CLOSE = 1.f / (1 << 18);
-__device__ __forceinline__ bool close(float hi, float lo) { return !(hi - lo > RT_CLOSE * fmaxf(1.f, fabsf(hi))); }
+__device__ __forceinline__ bool close(float hi, float lo, float size = 1.f) { return !(hi - lo > RT_CLOSE * fmaxf(size, fabsf(hi))); }
+// the scores of two groups' best are each rounded at their own size, which their sum may have lost
+__device__ __forceinline__ float size_of(float a, float b) {
+  const float size = fabsf(a) + fabsf(b);
+  return size <= 3.4028234663852886e38f ? fmaxf(size, 1.f) : 1.f;
+}
 __device__ __forceinline__ float fast_exp(float x) {        // relative error 2^-22 + |x| 2^-24
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
@@ -276,6 +281,7 @@ __global__ void __launch_bounds__(RT_WARPS * 32, NV >= 32 ? 2 : NV == 16 ? 5 : N
   bool wide = false;                             // too close to call
   if (p.groups > 1) {
     uint32_t mine = 0;                           // lane's group's score, or in the general form that of group `lane`
+    float size = 1.f;                            // of the two scores in it
     bool whole = p.group_size % NV == 0;         // whole lanes make up a group, a power of two of them
     const int lanes = p.group_size / NV;
     whole = whole && (lanes & (lanes - 1)) == 0;
@@ -289,6 +295,7 @@ __global__ void __launch_bounds__(RT_WARPS * 32, NV >= 32 ? 2 : NV == 16 ? 5 : N
         a = max(a, oa);
       }
       mine = p.bias && p.group_size > 1 ? ordered(unordered(a) + unordered(b)) : a;
+      size = size_of(unordered(a), unordered(b));
       if (!FULL && e0 >= p.experts) mine = 0;
     } else {
       for (int g = 0; g < p.groups; ++g) {
@@ -305,12 +312,14 @@ __global__ void __launch_bounds__(RT_WARPS * 32, NV >= 32 ? 2 : NV == 16 ? 5 : N
           const int owner = __ffs(__ballot_sync(0xffffffffu, a == best)) - 1;
           const uint32_t second = __reduce_max_sync(0xffffffffu, lane == owner ? b : a);
           score = ordered(unordered(best) + unordered(second));
+          if (lane == g) size = size_of(unordered(best), unordered(second));
         }
         if (lane == g) mine = score;
       }
     }
     // lane g takes group g's score and counts the better ones
     const int group_of_lane = whole ? lane >> (__ffs(lanes) - 1) : lane;
+    const uint32_t own = mine;
     if (whole) mine = __shfl_sync(0xffffffffu, mine, min(lane * lanes, 31));
     if (lane >= p.groups) mine = 0;
     int better = 0;
@@ -321,7 +330,8 @@ __global__ void __launch_bounds__(RT_WARPS * 32, NV >= 32 ? 2 : NV == 16 ? 5 : N
     uint32_t kept = __ballot_sync(0xffffffffu, keep);
     if (p.bias && p.top_groups < p.groups) {     // the order of the kept ones does not matter
       const uint32_t last = __reduce_min_sync(0xffffffffu, keep ? mine : 0xffffffffu), next = __reduce_max_sync(0xffffffffu, keep ? 0u : mine);
-      wide = close(unordered(last), unordered(next));
+      const uint32_t compared = own == last || own == next ? __float_as_uint(size) : 0u;       // lanes behind the groups have 0
+      wide = close(unordered(last), unordered(next), __uint_as_float(__reduce_max_sync(0xffffffffu, compared)));
       if (wide && whole && p.sigmoid) {          // the same for all lanes
         kept = groups_wide<T, NV>(p, t, lanes);
         wide = false;
