@@ -174,9 +174,15 @@ __device__ __forceinline__ uint32_t ordered(float v) {      // compares as v doe
   return u ^ (u >> 31 ? 0xffffffffu : 0x80000000u);
 }
 __device__ __forceinline__ float unordered(uint32_t k) { return __uint_as_float(k ^ (k >> 31 ? 0x80000000u : 0xffffffffu)); }
-// fp32 scores nearer than this (times the larger of 1 and their size) may be in the wrong order.  With u = 2^-24 an exponential is off by
-// (4 + |x|) u of itself; a sigmoid by p (1 - p) (4 + |x|) u + 4 p u < 5.5 u; a softmax by 30 p u (its sum of up to 1024 terms
-// included), so two of them, or the four of two groups, by 30 u together; the sum with the bias by another u of itself.  64 u are asked for.
+// fp32 scores nearer than this (times the larger of 1 and their size) may be in the wrong order.  With u = 2^-24:
+//   an exponential is off by (4 + 3 |x|) u of itself (x, times a rounded log2(e), 2^-22 of the instruction)
+//   a sigmoid by p (1 - p) (4 + 3 |x|) u + 3 p u < 5 u, two of them by 10 u, the four of two groups by 20 u
+//   the sum of a softmax by 17.5 u of itself in its terms (the mean of |x| with the weights p stays below 4.5 for 1024 experts) and 14 u
+//   in its additions (7 in a lane's four partial sums, 2 to join them, 5 over the lanes): 31.5 u, which two scores have in common
+//   the terms of two probabilities, or of the four of two groups, by (6 u + 3 |x| u) p each: 8.5 u for two, 10.5 u for four, as they
+//   sum to 1 at most and p |x| stays below 0.37
+//   a sum with the bias by u of its size: 2 u for two, 6 u with those of two groups
+// so 48 u at most; 64 u are asked for.
 constexpr float RT_CLOSE = 1.f / (1 << 18);
 __device__ __forceinline__ bool close(float hi, float lo, float size = 1.f) { return !(hi - lo > RT_CLOSE * fmaxf(size, fabsf(hi))); }
 // the scores of two groups' best are each rounded at their own size, which their sum may have lost
@@ -251,10 +257,12 @@ __global__ void __launch_bounds__(RT_WARPS * 32, NV >= 32 ? 2 : NV == 16 ? 5 : N
     for (int i = 1; i < NV; ++i) top = fmaxf(top, x[i]);
     top = unordered(__reduce_max_sync(0xffffffffu, ordered(top)));
     top = fmaxf(top, -3.4028234663852886e38f);   // a row of masked experts only: probabilities of zero instead of NaN
-    sum = 0.f;
+    float part[NV < 4 ? NV : 4] = {};            // few additions in a row: RT_CLOSE counts on them
 #pragma unroll
-    for (int i = 0; i < NV; ++i) sum += fast_exp(x[i] - top);
-    sum = fmaxf(warp_sum(sum), 1.1754943508222875e-38f);
+    for (int i = 0; i < NV; ++i) part[i % 4] += fast_exp(x[i] - top);
+    if constexpr (NV >= 4) part[0] = (part[0] + part[1]) + (part[2] + part[3]);
+    else if constexpr (NV == 2) part[0] += part[1];
+    sum = fmaxf(warp_sum(part[0]), 1.1754943508222875e-38f);
   }
   // order-preserving keys of the scores; 0: no expert, or taken
   uint32_t key[NV];
