@@ -216,7 +216,7 @@ class DecoderStack:
                 raise ValueError("a sharded stack takes no attention: the caches are not sharded")
             if len(attention.caches) != len(weights) or attention.seq_lens.shape[0] != m:
                 raise ValueError(f"attention is for {len(attention.caches)} layers and {attention.seq_lens.shape[0]} sequences, the stack has {len(weights)} and {m}")
-            if weights[0]["qkv"][2] != (heads + 2 * kv) * d or weights[0]["o"][3] != heads * d:
+            if any(layer["qkv"][2] != (heads + 2 * kv) * d or layer["o"][3] != heads * d for layer in weights):
                 raise ValueError(f"{heads} query and {kv} key and value heads of {d} do not match the q/k/v and o projections")
         # gathers without a hand-shake: the next producer polls the gathered values against the arrival sentinel
         self.wait_in_consumer = bool(wait_in_consumer) and p2p is not None

@@ -67,3 +67,11 @@ def test_qk_norm_rope_refuses_outputs_that_are_inputs_or_each_other():
     for bad in (dict(q=0x1000), dict(k=0x1000), dict(q=0x5000), dict(cache, v=0x5000), dict(cache, v=0x1000), dict(cache, v=0x4000)):
         assert _rope(**bad) == EINVAL, bad
         assert "outputs" in capi.lib.kq_last_error().decode()
+
+
+def test_a_stack_checks_the_projections_of_every_layer():
+    make = lambda *layers: sharded.DecoderStack(list(layers), 2, 64, torch.device("cpu"), attention=step_attention(layers=len(layers)))    # noqa: E731
+    assert make(layer(), layer()).attention is not None
+    for bad in ((layer(), layer(qkv=160)), (layer(), layer(), layer(o=96))):
+        with pytest.raises(ValueError, match="projections"):
+            make(*bad)
