@@ -350,7 +350,8 @@ int kq_qk_norm_rope(const void* qkv, int dtype, int64_t tokens, int64_t stride_t
  *   - a table entry outside [0, num_pages) and tokens beyond table_width * page_size count as absent
  *   - a sequence that shows no token: zeros, lse = -infinity
  * q: [batch, heads, head_dim] with strides q_stride_batch, q_stride_head, head_dim dense; out: dense; lse: [batch, heads] fp32 log
- * of the sum of exponentials, or NULL.  q, caches and out have one dtype; scores, softmax and sums are fp32.  head_dim: a
+ * of the sum of exponentials, or NULL.  q, caches and out have one dtype; scores, the softmax's maximum and sums and the sums of the
+ * values are fp32; for 16-bit types the weights enter the product with the values with 22 (KQ_F16) or 17 bits (KQ_BF16).  head_dim: a
  * multiple of 16 up to 256 (KQ_EUNSUPPORTED otherwise); caches and their strides and out 16-byte aligned; out is not q.  scale and
  * softcap: at most 1e30.  Where a visible value is not finite, neither are the outputs of its column (NaN also where one infinity alone
  * would give infinity).

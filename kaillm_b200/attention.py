@@ -51,7 +51,11 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     scale: 1 / sqrt(D) by default.  softcap > 0: scores become softcap * tanh(score / softcap).  block_table int32 [batch, pages]:
     token j of sequence b is place j % page size of page block_table[b, j // page size]; entries outside the cache count as absent.
     A sequence without visible tokens gives zeros (lse -inf).  The token's own key has to be in the cache
-    (`qk_norm_rope_store` first) and counted in seq_lens.  D: a multiple of 16 up to 256; float32, float16 or bfloat16."""
+    (`qk_norm_rope_store` first) and counted in seq_lens.  D: a multiple of 16 up to 256; float32, float16 or bfloat16.
+
+    Scores, the softmax's maximum and sums and the sums of the values are fp32; for 16-bit types the weights enter the product with the
+    values with 22 (float16) or 17 bits (bfloat16).  A visible value that is not finite spoils its column of the output: for 16-bit types
+    an infinity too gives NaN.  Keys and values that no sequence sees may hold anything."""
     out, lse = PAGED_ATTENTION(q, k_cache, v_cache, block_table, seq_lens, q.shape[-1] ** -0.5 if scale is None else scale, window, softcap,
                                return_lse)
     return (out, lse) if return_lse else out
