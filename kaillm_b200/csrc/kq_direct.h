@@ -1,8 +1,8 @@
 // Calls of an operator from Python that do not pass through the dispatcher: Direct<&fn>::call is a CPython function whose `self` is the
 // operator's overload in torch.ops.  Plain arguments (dense CUDA tensors of no subclass, int, float, bool, None) go straight to
 // fn, which checks them itself; anything else, and a call while a mode, a transform, a tracer or a profiler wants to see operators,
-// goes to the overload.  Parsing a call against its schema and boxing it costs as much as the launch (routing of 8 tokens 3.6 us a call, by the
-// overload 5.8; 2.5 of both are the launch), and an eager step of one token waits for nothing else.
+// goes to the overload.  Parsing a call against its schema and boxing it costs as much as the launch (routing of 8 tokens 4.2 us a call, by the
+// overload 6.6; 2.5 of both are the launch), and an eager step of one token waits for nothing else.
 #pragma once
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/record_function.h>

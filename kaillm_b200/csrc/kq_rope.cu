@@ -409,7 +409,8 @@ int run_rows(const RopeParams& p, cudaStream_t st) {
   while ((1 << log2) * 2 * (int)(sizeof(Piece) / sizeof(T)) < p.dim) ++log2;
   const bool pdl = options().pdl != 0;
   // (pieces of 8 bytes: few, and the ring.)  Few tokens, more than a few, more than a wave of ring_kernel's warps; with 40 + 2 x 8 heads of 128, us: 16 tokens 2.9 spread; 600 7.0 by two warps
-  // each, 16 spread, 9.0 by the ring; 2000 16.6, 54.7, 16.0; 5000 33.5, 132, 28.8
+  // each, 16 spread, 9.0 by the ring; 2000 16.6, 54.7, 16.0; 5000 33.5, 132, 28.8.  Where the spread form and two warps cross is not measured: at
+  // 600 the spread one is behind already, so some hundred tokens below the switch run slower than they could
   if (p.tokens >= (sizeof(Piece) == 16 ? 20 : 4) * sm_count()) {
     KQ_CUDA_TRY(launch_pdl(rope_ring_kernel<T, FORM, Piece>, dim3((unsigned)p.tokens), dim3(32), (size_t)0, st, pdl, p, log2));
   } else if (sizeof(Piece) == 16 && p.tokens >= 4 * sm_count()) {

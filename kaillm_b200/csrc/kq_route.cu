@@ -8,9 +8,9 @@
 // a few hundred scores lie closer than fp32 tells apart once in some hundred tokens, and a router's choice should not depend on the
 // last bit of an exponential: candidates whose scores come within RT_CLOSE of one another are ranked again in fp64, and so are the groups
 // of a sigmoid that whole lanes make up; what else is open sends the whole token through fp64 (route_wide), which takes a warp 5 us: left to
-// that, one such token among the last ones was felt in the time of the call (16384 x 256 in 8 groups 21.3 us, with groups_wide 17.4).
+// that, one such token among the last ones was felt in the time of the call (16384 x 256 in 8 groups 21.3 us, with groups_wide 17.4; 17.1 now).
 //
-// Bound by instructions, several hundred per token (17 MB and 2.7 us of memory for 16384 x 256 fp32 logits; 16.9 us): the best of 32 lanes
+// Bound by instructions, several hundred per token (886 for 16384 x 256 fp32 logits, 17 MB and 2.7 us of memory; 17.1 us): the best of 32 lanes
 // is one redux.sync on order-preserving integers, and where whole lanes make up a group all groups are scored at once.  With up to 102, 64 and
 // 51 registers for 16, 8 and fewer experts per lane, as below; left to the compiler 16384 x 256 takes 17.4 us, x 128 11.8 instead of 11.4.
 #include "kq_common.cuh"
