@@ -25,6 +25,7 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <ATen/core/stack.h>
 #include <torch/library.h>
 
 #include "../../include/kq_gguf.h"
@@ -510,6 +511,14 @@ std::tuple<at::Tensor, at::Tensor> moe_route(const at::Tensor& logits, int64_t t
   return {w, ids};
 }
 
+// The same refusal where autograd looks at a call: inside torch.func's transforms the kernel sees tensors without the level that is
+// being differentiated.
+void refuse_derivatives(const c10::OperatorHandle& op, c10::DispatchKeySet keys, torch::jit::Stack* stack) {
+  for (const c10::IValue& v : torch::jit::last(*stack, op.schema().arguments().size()))
+    if (v.isTensor()) no_gradient(op.schema().name().c_str(), {&v.toTensor()});
+  op.redispatchBoxed(keys & c10::after_autograd_keyset, stack);
+}
+
 int64_t ggml_moe_get_block_size(int64_t type) { return kq_moe_block_size((int)type); }
 
 }  // namespace
@@ -561,6 +570,11 @@ TORCH_LIBRARY_IMPL(_C_gguf, CUDA, ops) {
   ops.impl("paged_attention", &paged_attention);
   ops.impl("plan_pages", &plan_pages);
   ops.impl("moe_route", &moe_route);
+}
+
+TORCH_LIBRARY_IMPL(_C_gguf, Autograd, ops) {
+  for (const char* name : {"qk_norm_rope", "qk_norm_rope_store", "paged_attention", "plan_pages", "moe_route"})
+    ops.impl(name, torch::CppFunction::makeFromBoxedFunction<&refuse_derivatives>());
 }
 
 TORCH_LIBRARY_IMPL(_C_gguf, CompositeExplicitAutograd, ops) {
