@@ -352,8 +352,8 @@ int kq_qk_norm_rope(const void* qkv, int dtype, int64_t tokens, int64_t stride_t
  * q: [batch, heads, head_dim] with strides q_stride_batch, q_stride_head, head_dim dense; out: dense; lse: [batch, heads] fp32 log
  * of the sum of exponentials, or NULL.  q, caches and out have one dtype; scores, the softmax's maximum and sums and the sums of the
  * values are fp32; for 16-bit types the weights enter the product with the values with 22 (KQ_F16) or 17 bits (KQ_BF16).  head_dim: a
- * multiple of 16 up to 256 (KQ_EUNSUPPORTED otherwise); caches and their strides and out 16-byte aligned; out is not q.  scale and
- * softcap: at most 1e30.  Where a visible value is not finite, neither are the outputs of its column (NaN also where one infinity alone
+ * multiple of 16 up to 256 (KQ_EUNSUPPORTED otherwise); caches and their strides and out 16-byte aligned; out overlaps no input.  scale
+ * is positive, softcap not negative, both at most 1e30.  Where a visible value is not finite, neither are the outputs of its column (NaN also where one infinity alone
  * would give infinity).
  * scratch: kq_paged_attention_workspace_bytes(...) bytes for the current device (0 for sizes that are not served), 256-byte aligned,
  * not initialised; calls that may overlap need one each. */
@@ -378,8 +378,8 @@ int kq_paged_attention_status(int* status, int clear);
  *   positions, slots [num_tokens] of the new tokens, request by request; slot -1 (and position 0 behind the last token) for
  *                padding, tokens beyond the row and tokens without a page
  *   taken_out    [1]             taken + pages asked for: above num_free means that some were not there
- * num_tokens must not be below the sum of new_lens: tokens that do not fit get neither a slot nor a table entry.  No output but
- * block_table may be an input. */
+ * num_tokens must not be below the sum of new_lens: tokens that do not fit get neither a slot nor a table entry.  Outputs and block_table
+ * must overlap neither the inputs nor each other (equal pointers are refused). */
 int kq_plan_pages(int32_t* block_table, int64_t table_stride, int64_t table_width, const int32_t* seq_lens,
                   const int32_t* new_lens, int64_t requests, const int32_t* free_pages, int64_t num_free,
                   const int32_t* taken, int64_t page_size, int64_t num_tokens, int32_t* total_lens, int32_t* starts,
@@ -395,7 +395,8 @@ int kq_plan_pages(int32_t* block_table, int64_t table_stride, int64_t table_widt
  * NaN counts as -infinity and +infinity as the largest finite number, in the bias too.  An expert with a logit of -infinity has p = 0
  * and, when chosen, weight 0, for softmax and sigmoid alike.  Without a bias such experts come last; with one they count with c = bias
  * as everywhere in the formula, so they CAN come before others (and in groups count for theirs): where they must not, their bias has
- * to be -infinity as well, which places an expert last whatever its logit.  At most 1024 experts, top_k 32, 32 groups. */
+ * to be -infinity as well, which places an expert last whatever its logit.  At most 1024 experts, top_k 32, 32 groups.
+ * Outputs must overlap neither the inputs nor each other (equal pointers are refused). */
 int kq_moe_route(const void* logits, int dtype, int64_t tokens, int64_t experts, int64_t stride_t, int64_t top_k,
                  int sigmoid, const float* bias, int64_t groups, int64_t top_groups, int renormalize, float scale,
                  float* weights, int32_t* ids, void* stream);

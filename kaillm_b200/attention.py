@@ -48,7 +48,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     """Attention of one token per sequence, q [batch, heads, D], over the first seq_lens[b] cached tokens (the last `window` of them
     if window > 0): [batch, heads, D], and with return_lse the fp32 log of the sum of exponentials [batch, heads].
 
-    scale: 1 / sqrt(D) by default.  softcap > 0: scores become softcap * tanh(score / softcap).  block_table int32 [batch, pages]:
+    scale (positive): 1 / sqrt(D) by default.  softcap > 0: scores become softcap * tanh(score / softcap).  block_table int32 [batch, pages]:
     token j of sequence b is place j % page size of page block_table[b, j // page size]; entries outside the cache count as absent.
     A sequence without visible tokens gives zeros (lse -inf).  The token's own key has to be in the cache
     (`qk_norm_rope_store` first) and counted in seq_lens.  D: a multiple of 16 up to 256; float32, float16 or bfloat16.

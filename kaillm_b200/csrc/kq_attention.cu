@@ -1020,7 +1020,8 @@ int kq_paged_attention(const void* q, int dtype, int64_t batch, int64_t heads, i
     set_error("%s: misaligned pointer", fn);
     return KQ_EINVAL;
   }
-  if (q == out) { set_error("%s: out must not be q", fn); return KQ_EINVAL; }   // several workers read a row of q
+  // several workers read a row of q, and any of them the caches
+  if (out == q || out == k_cache || out == v_cache || lse == out) { set_error("%s: out must be neither an input nor lse", fn); return KQ_EINVAL; }
   const Scratch L = scratch_of(batch, heads, kv_heads, head_dim);
   if (!scratch || (uintptr_t)scratch % 256) { set_error("%s: scratch must be non-null and 256-byte aligned", fn); return KQ_ESCRATCH; }
   if (scratch_bytes < L.total) { set_error("%s: scratch too small (%zu < %zu)", fn, scratch_bytes, L.total); return KQ_ESCRATCH; }

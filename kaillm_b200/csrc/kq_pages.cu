@@ -143,7 +143,15 @@ extern "C" int kq_plan_pages(int32_t* block_table, int64_t table_stride, int64_t
     return KQ_EINVAL;
   }
   // other CTAs may still read what the first one would overwrite
-  if (taken == taken_out || (requests && (total_lens == seq_lens || total_lens == new_lens))) { set_error("%s: outputs must not be inputs", fn); return KQ_EINVAL; }
+  const void* outs[] = {total_lens, starts, positions, slots, taken_out};
+  const void* ins[] = {block_table, seq_lens, new_lens, free_pages, taken};
+  for (int i = 0; i < 5; ++i)
+    for (int j = 0; j < 5; ++j)
+      if (outs[i] && (outs[i] == ins[j] || (j < i && outs[i] == outs[j]))) { set_error("%s: outputs must be neither inputs nor each other", fn); return KQ_EINVAL; }
+  if (block_table && (block_table == seq_lens || block_table == new_lens || block_table == free_pages || block_table == taken)) {
+    set_error("%s: block_table is written, and must not be another input", fn);
+    return KQ_EINVAL;
+  }
   PageParams p;
   p.table = block_table; p.table_r = table_stride; p.width = (int)table_width; p.seen = seq_lens; p.fresh = new_lens;
   p.requests = (int)requests; p.free_pages = free_pages; p.num_free = (int)num_free; p.taken = taken; p.page_size = (int)page_size;

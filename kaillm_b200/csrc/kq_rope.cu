@@ -5,8 +5,8 @@
 //   (y_a, y_b) -> factor * (y_a cos t - y_b sin t, y_b cos t + y_a sin t),  t = position * inv_freq[i],  i < r / 2
 //   (a, b) = (i, i + r / 2), or (2i, 2i + 1) interleaved; values from r on are only normalised
 //
-// All of it in fp32 with one rounding at the end; the angle is the exact product, reduced to one turn in fp64 (position 10^6
-// times a frequency near 1 would be off by 0.06 rad in fp32), and its cosine and sine are formed once per token.
+// All of it in fp32 with one rounding at the end; the angle is the product in fp64 (exact below position 2^29), reduced there to one turn
+// (position 10^6 times a frequency near 1 would be off by 0.06 rad in fp32), and its cosine and sine are formed once per token, in fp32.
 #include <type_traits>
 
 #include "kq_common.cuh"

@@ -513,6 +513,8 @@ extern "C" int kq_moe_route(const void* logits, int dtype, int64_t tokens, int64
   if (!logits || !weights || !ids) { set_error("%s: null pointer", fn); return KQ_EINVAL; }
   if (tokens > 1 && stride_t < experts) { set_error("%s: rows of the logits overlap", fn); return KQ_EINVAL; }
   if ((uintptr_t)logits % (dtype == KQ_F32 ? 4 : 2) || ((uintptr_t)bias | (uintptr_t)weights | (uintptr_t)ids) % 4) { set_error("%s: misaligned pointer", fn); return KQ_EINVAL; }
+  const void *w = weights, *e = ids;
+  if (w == logits || e == logits || w == e || w == bias || e == bias) { set_error("%s: outputs must be neither inputs nor each other", fn); return KQ_EINVAL; }
   RouteParams p;
   p.logits = logits; p.stride_t = tokens > 1 ? stride_t : 0; p.tokens = tokens; p.experts = (int)experts; p.top_k = (int)top_k; p.sigmoid = sigmoid != 0;
   p.groups = (int)groups; p.top_groups = (int)top_groups; p.group_size = (int)(experts / groups); p.renormalize = renormalize != 0;

@@ -75,3 +75,17 @@ def test_a_stack_checks_the_projections_of_every_layer():
     for bad in ((layer(), layer(qkv=160)), (layer(), layer(), layer(o=96))):
         with pytest.raises(ValueError, match="projections"):
             make(*bad)
+
+
+def test_c_entries_refuse_outputs_that_are_inputs_or_each_other():
+    from tests.test_decode_ops_cpu import EINVAL, _attend, _plan, _route
+
+    ins, outs = {"table": 0x1000, "seen": 0x2000, "new": 0x3000, "free": 0x4000, "taken": 0x5000}, ["total", "starts", "pos", "slots", "out"]
+    bad = [(_plan, {o: at}) for o in outs for at in ins.values()] + [(_plan, {a: 0xb000, b: 0xb000}) for a in outs for b in outs if a != b]
+    bad += [(_plan, {"table": at}) for name, at in ins.items() if name != "table"]
+    bad += [(_route, dict(w=0x1000)), (_route, dict(ids=0x1000)), (_route, dict(w=0x3000)), (_route, dict(bias=0x2000)), (_route, dict(bias=0x3000))]
+    bad += [(_attend, dict(out=0x2000)), (_attend, dict(out=0x3000)), (_attend, dict(lse=0x6000))]
+    for call, args in bad:
+        assert call(**args) == EINVAL, (call, args)
+        message = capi.lib.kq_last_error().decode()
+        assert "must be neither" in message or "must not be another input" in message, (args, message)
