@@ -353,8 +353,8 @@ int kq_qk_norm_rope(const void* qkv, int dtype, int64_t tokens, int64_t stride_t
  * of the sum of exponentials, or NULL.  q, caches and out have one dtype; scores, the softmax's maximum and sums and the sums of the
  * values are fp32; for 16-bit types the weights enter the product with the values with 22 (KQ_F16) or 17 bits (KQ_BF16).  head_dim: a
  * multiple of 16 up to 256 (KQ_EUNSUPPORTED otherwise); caches and their strides and out 16-byte aligned; out overlaps no input.  scale
- * is positive, softcap not negative, both at most 1e30.  Where a visible value is not finite, neither are the outputs of its column (NaN also where one infinity alone
- * would give infinity).
+ * is positive, softcap not negative, both at most 1e30.  Where a visible value is not finite, neither are the outputs of its
+ * column (NaN also where one infinity alone would give infinity).
  * scratch: kq_paged_attention_workspace_bytes(...) bytes for the current device (0 for sizes that are not served), 256-byte aligned,
  * not initialised; calls that may overlap need one each. */
 size_t kq_paged_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim);

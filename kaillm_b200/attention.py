@@ -102,7 +102,8 @@ class StepAttention:
         self.q_weights, self.k_weights = (w if w is not None else [None] * len(self.caches) for w in (q_weights, k_weights))
         self.eps, self.interleaved, self.factor, self.scale, self.window, self.softcap = eps, interleaved, factor, scale, window, softcap
         self.one_each = torch.ones_like(seq_lens)
-        self.dropped = torch.zeros_like(seq_lens, dtype=torch.int64)
+        with torch.inference_mode(False):                # steps may write it in or outside of that mode
+            self.dropped = torch.zeros_like(seq_lens, dtype=torch.int64)
         self.positions = self.slots = None
 
     def begin_step(self) -> None:

@@ -89,3 +89,14 @@ def test_c_entries_refuse_outputs_that_are_inputs_or_each_other():
         assert call(**args) == EINVAL, (call, args)
         message = capi.lib.kq_last_error().decode()
         assert "must be neither" in message or "must not be another input" in message, (args, message)
+
+
+def test_attention_made_in_inference_mode_steps_outside(monkeypatch):
+    from kaillm_b200 import attention
+
+    with torch.inference_mode():
+        att = step_attention()
+    att.seq_lens, att.taken = att.seq_lens.clone(), att.taken.clone()
+    monkeypatch.setattr(attention, "plan_pages", lambda *a: (att.seq_lens + 1, None, att.seq_lens, torch.tensor([3, -1]), att.taken))
+    att.begin_step()
+    assert att.dropped.tolist() == [0, -1]
